@@ -5,6 +5,7 @@
 
 Outputs (git-ignored, shipped with the tree):
     ridge_amd/lib/libridge_gemm.so   GEMM kernel table, fills, hipBLASLt comparator
+    ridge_amd/lib/libridge_int8.so   the 8-bit operators (include/ridge_int8.h)
     ridge_amd/lib/libridge_model.so  the cost model behind a C ABI
     ridge_amd/bin/ridge-predict      the model CLI (reference tools/ridge-predict.cpp)
     ridge_amd/bin/ridge-check        correctness + throughput harness (bench/check-gemm.cu)
@@ -122,6 +123,20 @@ def parse_resource_remarks(text):
     return out
 
 
+def kernel_remarks(text):
+    """Maps every kernel's mangled name -> resource dict from -Rpass-analysis output."""
+    out, cur = {}, None
+    for line in text.splitlines():
+        m = re.search(r"Function Name: (\S+)", line)
+        if m:
+            cur = out.setdefault(m.group(1), {})
+            continue
+        f = re.search(r"remark:\s+([A-Za-z][A-Za-z /\[\]]*?):\s*(\S+)", line)
+        if cur is not None and f and f.group(1).strip() in _RESOURCE_KEYS:
+            cur[_RESOURCE_KEYS[f.group(1).strip()]] = int(f.group(2)) if f.group(2).isdigit() else f.group(2)
+    return out
+
+
 def write_resource_table(variants, res, path):
     lines = [
         "// Generated by ridge_amd/build.py from kernel-resource-usage remarks. Do not edit.",
@@ -173,6 +188,33 @@ def build_gemm(gate=True):
     _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", tmp] + objs +
          ["-L/opt/rocm/lib", "-lhipblaslt", "-Wl,-rpath,/opt/rocm/lib"])
     os.replace(tmp, so)
+    return so
+
+
+INT8_SRCS = ["int8_rows.hip", "int8_gemm.hip"]
+
+
+def build_int8(gate=True):
+    """libridge_int8.so. No kernel of it may use scratch memory."""
+    os.makedirs(BUILD, exist_ok=True)
+    os.makedirs(LIB, exist_ok=True)
+    objs, spilling = [], 0
+    for src in INT8_SRCS:
+        o = os.path.join(BUILD, src.replace(".hip", ".o"))
+        remarks = _run([HIPCC] + LIB_HIP_FLAGS + ["-Rpass-analysis=kernel-resource-usage", "-x", "hip", "-c",
+                                                  os.path.join(CSRC, src), "-o", o], capture=True)
+        kernels = kernel_remarks(remarks)
+        bad = {k: r for k, r in kernels.items() if r["scratch"] or r["vgpr_spill"] or r["sgpr_spill"]}
+        print("  %s: %d kernels, %d spilling" % (src, len(kernels), len(bad)))
+        for k, r in bad.items():
+            print("    SPILL %s: %s" % (k, r))
+        spilling += len(bad)
+        objs.append(o)
+    if spilling and gate:
+        raise SystemExit("spill gate: %d 8-bit kernel(s) use scratch" % spilling)
+    so = os.path.join(LIB, "libridge_int8.so")
+    _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", so + ".tmp"] + objs)
+    os.replace(so + ".tmp", so)
     return so
 
 
@@ -234,11 +276,13 @@ def build_oracle():
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--no-gate", action="store_true", help="do not fail on spilling variants")
-    ap.add_argument("--only", default="all", choices=["all", "gemm", "model", "tools", "oracle"])
+    ap.add_argument("--only", default="all", choices=["all", "gemm", "int8", "model", "tools", "oracle"])
     args = ap.parse_args(argv)
     print("ridge_amd build (%s)" % ARCH, flush=True)
     if args.only in ("all", "gemm"):
         build_gemm(gate=not args.no_gate)
+    if args.only in ("all", "int8"):
+        build_int8(gate=not args.no_gate)
     if args.only in ("all", "model"):
         build_model()
     if args.only in ("all", "tools"):

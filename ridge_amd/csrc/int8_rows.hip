@@ -1,0 +1,370 @@
+// int8_rows.hip -- the operators that make 8-bit rows (quantize, silu_mul, rms_norm) and
+// the one that reads them back, for the C ABI in include/ridge_int8.h.
+//
+// All three makers are one kernel around a different source of a row's f32 values: read
+// the row once, hold its values in registers, reduce the largest magnitude (and, for the
+// norm, the sum of squares) over the row's threads, round and write. Memory bounds them:
+// every input byte is read once and every output byte written once, in 16-byte and
+// 8-byte pieces a lane.
+//
+// A norm needs one reduction, not two: the sum of squares and the largest |s w| are taken
+// together, because the reciprocal root that multiplies a whole row moves out of the
+// maximum.
+
+#include "ridge_int8.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+namespace {
+
+constexpr int kWave = 64;
+constexpr int kVec = 8;  // elements a lane loads at once: 16 bytes of a 16-bit type
+
+// n elements of a row at once, with the alignment of one: rows may start anywhere, and
+// global accesses of any alignment are one instruction here. What a row has behind its
+// last whole vector goes one element a lane.
+template <typename T, int n>
+struct Memory {
+    typedef T Vec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
+};
+typedef signed char Bytes8 __attribute__((ext_vector_type(kVec), aligned(8)));
+
+template <int n, typename T>
+__device__ __forceinline__ void loadRow(const T* at, float (&v)[n]) {
+    const typename Memory<T, n>::Vec m = *(const typename Memory<T, n>::Vec*)at;
+#pragma unroll
+    for (int e = 0; e < n; ++e) v[e] = (float)m[e];
+}
+
+template <int n, typename T>
+__device__ __forceinline__ void storeRow(T* at, const float (&v)[n]) {
+    typename Memory<T, n>::Vec m;
+#pragma unroll
+    for (int e = 0; e < n; ++e) m[e] = (T)v[e];
+    *(typename Memory<T, n>::Vec*)at = m;
+}
+
+// Nearest whole numbers (halves to even) of v / scale. The quotient is the correctly
+// rounded one, by one correction of v * (1 / scale) with its exact remainder: a product
+// alone rounds values near a half the other way. The bounds also give a NaN a value: its
+// row's scale is one.
+template <int n>
+__device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], float scale, float inverse) {
+    typename Memory<signed char, n>::Vec b;
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+        float t = v[e] * inverse;
+        t = fmaf(fmaf(-t, scale, v[e]), inverse, t);
+        b[e] = (signed char)(int)fminf(fmaxf(rintf(t), -127.0f), 127.0f);
+    }
+    *(typename Memory<signed char, n>::Vec*)at = b;
+}
+
+struct RowArgs {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    int64_t ldx, ldq;
+    int rows, cols;
+    // rms_norm
+    const void* residual;
+    const void* weight;
+    void* residualOut;
+    int64_t ldResidual, ldResidualOut;
+    float eps;
+};
+
+// Sources of a row's values: load() gives n of them from column col on, and adds what the
+// norm sums up.
+template <typename T>
+struct Plain {
+    static constexpr bool kNorm = false;
+    const T* x;
+    __device__ Plain(const RowArgs& a, int64_t row) : x((const T*)a.x + row * a.ldx) {}
+    template <int n>
+    __device__ void load(int col, float (&v)[n], float&, bool) const {
+        loadRow(x + col, v);
+    }
+};
+
+template <typename T>
+struct Gated {
+    static constexpr bool kNorm = false;
+    const T* x;
+    int cols;
+    __device__ Gated(const RowArgs& a, int64_t row) : x((const T*)a.x + row * a.ldx), cols(a.cols) {}
+    template <int n>
+    __device__ void load(int col, float (&v)[n], float&, bool) const {
+        float u[n];
+        loadRow(x + col, v);
+        loadRow(x + cols + col, u);
+#pragma unroll
+        for (int e = 0; e < n; ++e) v[e] = v[e] / (1.0f + expf(-v[e])) * u[e];
+    }
+};
+
+// The residual's sum leaves with the row's last reading, so that it may replace x or the
+// residual.
+template <typename T, typename W>
+struct Normed {
+    static constexpr bool kNorm = true;
+    const T* x;
+    const T* residual;
+    const W* weight;
+    T* out;
+    __device__ Normed(const RowArgs& a, int64_t row)
+        : x((const T*)a.x + row * a.ldx),
+          residual(a.residual ? (const T*)a.residual + row * a.ldResidual : nullptr),
+          weight((const W*)a.weight),
+          out(a.residualOut ? (T*)a.residualOut + row * a.ldResidualOut : nullptr) {}
+    template <int n>
+    __device__ void load(int col, float (&v)[n], float& squares, bool last) const {
+        float w[n];
+        loadRow(x + col, v);
+        if (residual) {
+            float r[n];
+            loadRow(residual + col, r);
+#pragma unroll
+            for (int e = 0; e < n; ++e) v[e] += r[e];
+            if (last) storeRow(out + col, v);
+        }
+        loadRow(weight + col, w);
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+            squares = fmaf(v[e], v[e], squares);
+            v[e] *= w[e];
+        }
+    }
+};
+
+// Magnitudes are compared as integers: that is their order, and a NaN is above all.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Sum and maximum over the kThreads threads of a row, in an order that depends on
+// nothing but kThreads.
+template <int kThreads, bool kSum>
+__device__ __forceinline__ void reduceRow(float& sum, uint32_t& top) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d /= 2) {
+        if (kSum) sum += __shfl_xor(sum, d);
+        top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    }
+    if constexpr (kThreads > kWave) {
+        constexpr int kWaves = kThreads / kWave;
+        __shared__ float sums[kWaves];
+        __shared__ uint32_t tops[kWaves];
+        if (threadIdx.x % kWave == 0) {
+            sums[threadIdx.x / kWave] = sum;
+            tops[threadIdx.x / kWave] = top;
+        }
+        __syncthreads();
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            if (kSum) sum += sums[i];
+            top = max(top, tops[i]);
+        }
+        __syncthreads();  // the next row's partial results go to the same places
+    }
+}
+
+// One row a kThreads threads. kVecs vectors a thread hold the row; with kVecs = 0 a row
+// of any length is read twice.
+template <typename Source, int kThreads, int kVecs>
+__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads)
+void makeRowsKernel(RowArgs a) {
+    constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
+    constexpr int kRowsPerBlock = kBlock / kThreads;
+    constexpr bool kHeld = kVecs > 0;
+    const int lane = threadIdx.x % kThreads;
+    const int whole = a.cols / kVec * kVec;    // columns of whole vectors
+    const int single = whole + lane;           // and this lane's behind them
+    for (int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + threadIdx.x / kThreads; row < a.rows;
+         row += (int64_t)gridDim.x * kRowsPerBlock) {
+        const Source source(a, row);
+        float v[kHeld ? kVecs : 1][kVec], one[1];
+        float squares = 0.0f;
+        uint32_t top = 0;
+        // Calls f(column, values) for each of this lane's parts of the row.
+        auto parts = [&](auto&& f) {
+            if constexpr (kHeld) {
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    const int col = (i * kThreads + lane) * kVec;
+                    if (col < whole) f(col, v[i]);
+                }
+            } else {
+                for (int col = lane * kVec; col < whole; col += kThreads * kVec) f(col, v[0]);
+            }
+            if (single < a.cols) f(single, one);
+        };
+        parts([&](int col, auto& values) {
+            source.load(col, values, squares, kHeld);
+            for (float value : values) top = max(top, magnitude(value));
+        });
+        reduceRow<kThreads, Source::kNorm>(squares, top);
+        float root = 1.0f;
+        if constexpr (Source::kNorm) {
+            // A sum past the range of f32 would make the root 0 and the row silently so.
+            root = squares <= FLT_MAX ? 1.0f / sqrtf(squares / (float)a.cols + a.eps) : NAN;
+        }
+        float scale = __uint_as_float(top) * root / 127.0f;
+        scale = scale < FLT_MIN ? FLT_MIN : scale;  // a NaN stays one
+        const float inverse = 1.0f / scale;
+        if (lane == 0) a.scale[row] = scale;
+        int8_t* const q = a.q + row * a.ldq;
+        parts([&](int col, auto& values) {
+            if constexpr (!kHeld) source.load(col, values, squares, true);
+            if constexpr (Source::kNorm) {
+                for (float& value : values) value *= root;
+            }
+            storeRounded(q + col, values, scale, inverse);
+        });
+    }
+}
+
+constexpr int kDequantizeThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kDequantizeThreads)
+void dequantizeKernel(const int8_t* q, int64_t ldq, const float* scale, T* out, int64_t ldOut, int rows, int cols,
+                      int pieces) {
+    const int64_t total = (int64_t)rows * pieces;
+    for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+        const int row = (int)(i / pieces);
+        const int col = ((int)(i % pieces) * kDequantizeThreads + (int)threadIdx.x) * kVec;
+        if (col >= cols) continue;
+        const Bytes8 b = *(const Bytes8*)(q + row * ldq + col);  // rows are readable to a multiple of 16
+        const float s = scale[row];
+        float v[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[e] = (float)b[e] * s;
+        T* const at = out + row * ldOut + col;
+        if (col + kVec <= cols) {
+            storeRow(at, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+                if (col + e < cols) at[e] = (T)v[e];
+        }
+    }
+}
+
+constexpr int64_t kMostBlocks = 1 << 20;  // of a grid: blocks walk the rows behind it
+
+template <typename Source, int kThreads, int kVecs>
+hipError_t launchRows(const RowArgs& a, hipStream_t stream) {
+    constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
+    constexpr int kRowsPerBlock = kBlock / kThreads;
+    const int64_t blocks = std::min<int64_t>((a.rows + (int64_t)kRowsPerBlock - 1) / kRowsPerBlock, kMostBlocks);
+    makeRowsKernel<Source, kThreads, kVecs><<<dim3((unsigned)blocks), dim3(kBlock), 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+// The threads of a row, by its length: as many as hold it in at most four vectors each,
+// two for the norm on 1024 threads, whose registers would not hold more.
+template <typename Source>
+hipError_t launchByLength(const RowArgs& a, hipStream_t stream) {
+    if (a.cols <= 64 * kVec) return launchRows<Source, 64, 1>(a, stream);
+    if (a.cols <= 64 * kVec * 4) return launchRows<Source, 64, 4>(a, stream);
+    if (a.cols <= 256 * kVec * 4) return launchRows<Source, 256, 4>(a, stream);
+    constexpr int kMostVecs = Source::kNorm ? 2 : 4;
+    if (a.cols <= 1024 * kVec * kMostVecs) return launchRows<Source, 1024, kMostVecs>(a, stream);
+    return launchRows<Source, 1024, 0>(a, stream);
+}
+
+bool isType(int type) { return type == RIDGE_F16 || type == RIDGE_BF16 || type == RIDGE_F32; }
+
+bool aligned(const void* p, size_t to) { return p != nullptr && ((uintptr_t)p & (to - 1)) == 0; }
+
+size_t sizeOf(int type) { return type == RIDGE_F32 ? 4 : 2; }
+
+// What every maker of rows asks for: sizes within 31 bits, strides of at least a row,
+// and 8-bit rows at multiples of 16 bytes.
+bool rowsFit(const void* x, int64_t ldx, int64_t width, int type, const int8_t* q, int64_t ldq, const float* scale,
+             int64_t rows, int64_t cols) {
+    return isType(type) && rows <= INT32_MAX && cols > 0 && width <= INT32_MAX - 65536 && ldx >= width &&
+           ldq >= cols && ldq % 16 == 0 && aligned(x, sizeOf(type)) && aligned(q, 16) && aligned(scale, 4);
+}
+
+}  // namespace
+
+extern "C" int ridge_int8_quantize(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale,
+                                   int64_t rows, int64_t cols, void* stream) {
+    if (rows == 0 && cols > 0 && isType(type)) return hipSuccess;
+    if (rows < 0 || !rowsFit(x, ldx, cols, type, q, ldq, scale, rows, cols)) return hipErrorInvalidValue;
+    RowArgs a = {x, q, scale, ldx, ldq, (int)rows, (int)cols, nullptr, nullptr, nullptr, 0, 0, 0.0f};
+    hipStream_t s = (hipStream_t)stream;
+    switch (type) {
+        case RIDGE_F16: return launchByLength<Plain<_Float16>>(a, s);
+        case RIDGE_BF16: return launchByLength<Plain<__bf16>>(a, s);
+        default: return launchByLength<Plain<float>>(a, s);
+    }
+}
+
+extern "C" int ridge_int8_silu_mul(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale,
+                                   int64_t rows, int64_t cols, void* stream) {
+    if (rows == 0 && cols > 0 && isType(type)) return hipSuccess;
+    if (rows < 0 || cols > INT32_MAX / 2 || !rowsFit(x, ldx, 2 * cols, type, q, ldq, scale, rows, cols))
+        return hipErrorInvalidValue;
+    RowArgs a = {x, q, scale, ldx, ldq, (int)rows, (int)cols, nullptr, nullptr, nullptr, 0, 0, 0.0f};
+    hipStream_t s = (hipStream_t)stream;
+    switch (type) {
+        case RIDGE_F16: return launchByLength<Gated<_Float16>>(a, s);
+        case RIDGE_BF16: return launchByLength<Gated<__bf16>>(a, s);
+        default: return launchByLength<Gated<float>>(a, s);
+    }
+}
+
+extern "C" int ridge_int8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldResidual,
+                                   const void* weight, int weightType, float eps, int type, void* residualOut,
+                                   int64_t ldResidualOut, int8_t* q, int64_t ldq, float* scale, int64_t rows,
+                                   int64_t cols, void* stream) {
+    if (!isType(type) || (weightType != type && weightType != RIDGE_F32) || !(eps > 0.0f && eps <= FLT_MAX) ||
+        (residual == nullptr) != (residualOut == nullptr))
+        return hipErrorInvalidValue;
+    if (rows == 0 && cols > 0) return hipSuccess;
+    if (rows < 0 || !rowsFit(x, ldx, cols, type, q, ldq, scale, rows, cols) || !aligned(weight, sizeOf(weightType)))
+        return hipErrorInvalidValue;
+    if (residual && (!aligned(residual, sizeOf(type)) || !aligned(residualOut, sizeOf(type)) || ldResidual < cols ||
+                     ldResidualOut < cols))
+        return hipErrorInvalidValue;
+    RowArgs a = {x,        q,      scale,       ldx,        ldq,           (int)rows, (int)cols,
+                 residual, weight, residualOut, ldResidual, ldResidualOut, eps};
+    hipStream_t s = (hipStream_t)stream;
+    switch (type) {
+        case RIDGE_F16:
+            return weightType == RIDGE_F16
+                       ? launchByLength<Normed<_Float16, _Float16>>(a, s)
+                       : launchByLength<Normed<_Float16, float>>(a, s);
+        case RIDGE_BF16:
+            return weightType == RIDGE_BF16
+                       ? launchByLength<Normed<__bf16, __bf16>>(a, s)
+                       : launchByLength<Normed<__bf16, float>>(a, s);
+        default: return launchByLength<Normed<float, float>>(a, s);
+    }
+}
+
+extern "C" int ridge_int8_dequantize(const int8_t* q, int64_t ldq, const float* scale, void* out, int64_t ldOut,
+                                     int type, int64_t rows, int64_t cols, void* stream) {
+    if (rows == 0 && cols > 0 && isType(type)) return hipSuccess;
+    if (rows < 0 || !rowsFit(out, ldOut, cols, type, q, ldq, scale, rows, cols)) return hipErrorInvalidValue;
+    hipStream_t s = (hipStream_t)stream;
+    const int pieces = (int)((cols + kDequantizeThreads * kVec - 1) / (kDequantizeThreads * kVec));
+    const dim3 grid((unsigned)std::min(rows * pieces, kMostBlocks)), block(kDequantizeThreads);
+    switch (type) {
+        case RIDGE_F16:
+            dequantizeKernel<<<grid, block, 0, s>>>(q, ldq, scale, (_Float16*)out, ldOut, (int)rows, (int)cols, pieces);
+            break;
+        case RIDGE_BF16:
+            dequantizeKernel<<<grid, block, 0, s>>>(q, ldq, scale, (__bf16*)out, ldOut, (int)rows, (int)cols, pieces);
+            break;
+        default:
+            dequantizeKernel<<<grid, block, 0, s>>>(q, ldq, scale, (float*)out, ldOut, (int)rows, (int)cols, pieces);
+    }
+    return hipGetLastError();
+}
