@@ -38,14 +38,17 @@ struct Int8Args {
     TileOrder order;   // of ceil(M / BM) x ceil(N / BN) tiles
 };
 
-// Where chunk q = row * CPR + c of a tile lies in LDS (an involution). A fragment's read
-// has 16 lanes read one chunk of 16 consecutive rows, 256 bytes that LDS serves at once
-// where they lie in 16 different 16-byte slots of a 256-byte line: 16 / CPR rows share
-// such a line, and the mask gives the groups of rows that do different slots. It repeats
-// every 16 rows, so fragments 16 rows apart are a constant distance apart.
+// Where chunk q = row * CPR + c of a tile lies in LDS (an involution). LDS serves a
+// fragment's read 16 lanes at a time, lanes {0-3, 12-15, 20-27} and {4-11, 16-19, 28-31}
+// of each half of the wave: 16 rows of the tile, half of them at one chunk and half at the
+// next, which have to lie in 16 different 16-byte slots of a 256-byte line. The mask
+// repeats every 16 rows, so fragments 16 rows apart are a constant distance apart.
+// (Counted conflicts: none. The mask that would serve lanes 0-15 at once, (row / 4) % 4 at
+// 4 chunks a row, made every read take two turns: 256 x 256 x 64 tiles of K = 4096 on an
+// uncrowded chip 45.1 us against 40.2.)
 template <int CPR>
 __device__ __forceinline__ int swizzleRows(int q) {
-    return q ^ ((q / 16) % CPR);
+    return q ^ (CPR == 4 ? (q / 8) % 8 : (q / 16) % CPR);
 }
 
 // BK counts bytes, which are elements.
@@ -62,7 +65,8 @@ struct Int8Traits {
     static constexpr int kBytesA = BM * BK;
     static constexpr int kBytesB = BN * BK;
     static constexpr int kRegionA = kStages * kBytesA;   // LDS: A's stages, then B's
-    static constexpr int kLdsBytes = kStages * (kBytesA + kBytesB);
+    static constexpr int kRing = kStages * (kBytesA + kBytesB);
+    static constexpr int kLdsBytes = kRing + 4 * (BM + BN);   // and the tile's scales
     static constexpr int kPerWaveA = kBytesA / 1024 / kWaves;   // 1 KiB loads of a wave
     static constexpr int kPerWaveB = kBytesB / 1024 / kWaves;
     static constexpr int kLoadsPerTile = kPerWaveA + kPerWaveB;
@@ -73,6 +77,31 @@ struct Int8Traits {
     static_assert((kStages - 1) * kLoadsPerTile < 64, "in-flight loads exceed the vmcnt counter");
     static_assert(kLdsBytes <= 163840, "LDS is 160 KiB per workgroup on gfx950");
 };
+
+// Direct-to-LDS 4-byte load (globalLoadLds16's sibling): lane t's 4 bytes at base + offset
+// land at ldsAddr + 4 t.
+__device__ __forceinline__ void globalLoadLds4(const void* base, uint32_t offset, uint32_t ldsAddr) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "{m0}"(ldsAddr) : "memory");
+}
+
+// The lane's number, counted anew: kept through the K loop it costs a register that the
+// 256 x 256 x 128 tile has not got.
+__device__ __forceinline__ int laneAgain() {
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(lane));
+    return lane;
+}
+
+// A mask of the first `bytes` of 16 bytes (none for fewer than 1, all for 16 and more).
+__device__ __forceinline__ int4_t firstBytes(int bytes) {
+    int4_t mask;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const int n = min(max(bytes - 4 * d, 0), 4);
+        mask[d] = n == 4 ? -1 : (1 << (8 * n)) - 1;
+    }
+    return mask;
+}
 
 // A C element from its sum. The sum is exact and is rounded to f32's 24 bits here: a
 // relative 2^-24, far below what the result's type keeps.
@@ -125,6 +154,19 @@ struct Int8Block {
             for (int tn = 0; tn < TN; ++tn) acc[tm][tn] = int4_t{0, 0, 0, 0};
     }
 
+    // The scales of the tile's rows and columns on their way to LDS, 64 a wave load: the
+    // oldest loads of the wave, landed when its first K tile has. Issued before issueTile.
+    __device__ __forceinline__ void issueScales() const {
+        static_assert((T::BM + T::BN) / 64 <= T::kWaves && T::BM % 64 == 0 && T::BN % 64 == 0, "one load a wave");
+        const uint32_t to = ldsBase + T::kRing + wave * 256;
+        const int at = wave * 64 + lane;
+        if (wave < T::BM / 64) {
+            globalLoadLds4(args.scaleA + blockRow, 4u * (uint32_t)min(at, args.M - 1 - blockRow), to);
+        } else if (wave < (T::BM + T::BN) / 64) {
+            globalLoadLds4(args.scaleB + blockCol, 4u * (uint32_t)min(at - T::BM, args.N - 1 - blockCol), to);
+        }
+    }
+
     // The chunk of a tile that this lane's share of the wave's load i fetches.
     __device__ __forceinline__ int chunkOf(int i) const {
         return swizzleRows<CPR>((i * T::kWaves + wave) * 64 + lane);
@@ -167,13 +209,7 @@ struct Int8Block {
 
     // Clears what A's fragments of K tile kTile hold behind K.
     __device__ __forceinline__ void clearBehind(int kTile, int ks, int4_t (&a)[TM]) const {
-        const int left = args.K - (kTile * T::BK + ks * kInt8MfmaK + 16 * (lane / 16));
-        int4_t mask;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const int bytes = min(max(left - 4 * d, 0), 4);
-            mask[d] = bytes == 4 ? -1 : (1 << (8 * bytes)) - 1;
-        }
+        const int4_t mask = firstBytes(args.K - (kTile * T::BK + ks * kInt8MfmaK + 16 * (lane / 16)));
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) a[tm] &= mask;
     }
@@ -190,64 +226,100 @@ struct Int8Block {
 
     // Epilogue of one wave through a private LDS region, 16 rows a pass: a lane's four
     // columns are scaled, rounded and written there, and read back row by row, so that
-    // every store but a row's last is 16 bytes a lane. Every wave has to be past its last
-    // read of the ring.
+    // every store but a row's last is 16 bytes a lane. A wave's LDS instructions run in
+    // order, so only the compiler has to be kept from moving them; the next pass is
+    // computed while the read-backs are on their way. Every wave has to be past its last
+    // read of the ring. (256 x 256 tiles, 4096 cubed: 10.7k cycles with a wait on either
+    // side of the region and the scales read from memory at the end, 6.9k so.)
     static constexpr int kChunks = T::WN * (int)sizeof(Out) / 16;   // 16-byte chunks of a region's row
     static constexpr int kRegionBytes = 16 * T::WN * (int)sizeof(Out);
     static constexpr int kPer = 16 / (int)sizeof(Out);              // elements of a chunk
-    static_assert(T::kWaves * kRegionBytes <= T::kLdsBytes, "epilogue regions must fit the ring");
+    static constexpr int kReads = 16 * kChunks / 64;                // read-backs of a pass
+    static_assert(T::kWaves * kRegionBytes <= T::kRing && 16 * kChunks % 64 == 0, "epilogue regions must fit the ring");
+    typedef Out Quad __attribute__((ext_vector_type(4)));
+    typedef Out Chunk __attribute__((ext_vector_type(kPer)));
+    typedef Out Placed __attribute__((ext_vector_type(kPer), aligned(sizeof(Out))));
 
     __device__ __forceinline__ void store() const {
-        typedef Out Quad __attribute__((ext_vector_type(4)));
-        typedef Out Chunk __attribute__((ext_vector_type(kPer)));
-        typedef Out Placed __attribute__((ext_vector_type(kPer), aligned(sizeof(Out))));
         RIDGE_LDS_AS char* region = (RIDGE_LDS_AS char*)(const_cast<char*>(lds)) + wave * kRegionBytes;
+        const RIDGE_LDS_AS float* scales = (const RIDGE_LDS_AS float*)((const RIDGE_LDS_AS char*)(lds) + T::kRing);
         auto swz = [](int row, int chunk) { return chunk ^ ((row * kChunks / 16) % kChunks); };
+        const int lane = laneAgain();
         const int g = lane / 16, r16 = lane % 16;
         const int row0 = blockRow + waveM * T::WM, col0 = blockCol + waveN * T::WN;
-        const Out* bias = (const Out*)args.bias;
-        float sb[TN][4], add[TN][4];
+        float4_t sb[TN], add[TN];
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn)
+        for (int tn = 0; tn < TN; ++tn) {
+            sb[tn] = *(const RIDGE_LDS_AS float4_t*)(scales + T::BM + waveN * T::WN + tn * 16 + 4 * g);
+            add[tn] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        if (args.bias != nullptr) {
+            const Out* bias = (const Out*)args.bias;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = min(col0 + tn * 16 + 4 * g + e, args.N - 1);
-                sb[tn][e] = args.scaleB[col];
-                add[tn][e] = bias ? (float)bias[col] : 0.0f;
-            }
+            for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) add[tn][e] = (float)bias[min(col0 + tn * 16 + 4 * g + e, args.N - 1)];
+        }
+        Quad quads[TN];
+        auto compute = [&](int tm) {
+            const float sa = scales[waveM * T::WM + 16 * tm + r16];
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    quads[tn][e] = (Out)scaledSum(acc[tm][tn][e], sa, sb[tn][e], add[tn][e]);
+        };
+        compute(0);
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const float sa = args.scaleA[min(row0 + 16 * tm + r16, args.M - 1)];
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn) {
-                Quad v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (Out)scaledSum(acc[tm][tn][e], sa, sb[tn][e], add[tn][e]);
                 const int at = tn * 16 + 4 * g;
                 *(RIDGE_LDS_AS Quad*)(region + (r16 * kChunks + swz(r16, at / kPer)) * 16 +
-                                      (at % kPer) * sizeof(Out)) = v;
+                                      (at % kPer) * sizeof(Out)) = quads[tn];
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("" ::: "memory");
+            Chunk v[kReads];
 #pragma unroll
-            for (int j = 0; j < 16 * kChunks / 64; ++j) {
-                const int q = j * 64 + lane, r = q / kChunks, c = q % kChunks;
-                const Chunk v = *(const RIDGE_LDS_AS Chunk*)(region + (r * kChunks + swz(r, c)) * 16);
-                const int row = row0 + 16 * tm + r, col = col0 + c * kPer;
+            for (int j = 0; j < kReads; ++j) {
+                const int q = j * 64 + lane;
+                v[j] = *(const RIDGE_LDS_AS Chunk*)(region + (q / kChunks * kChunks + swz(q / kChunks, q % kChunks)) * 16);
+            }
+            asm volatile("" ::: "memory");
+            if (tm + 1 < TM) compute(tm + 1);
+#pragma unroll
+            for (int j = 0; j < kReads; ++j) {
+                const int q = j * 64 + lane;
+                const int row = row0 + 16 * tm + q / kChunks, col = col0 + q % kChunks * kPer;
                 if (row < args.M && col < args.N) {
                     Out* dst = (Out*)args.C + (int64_t)row * args.ldc + col;
                     if (col + kPer <= args.N) {
-                        *(Placed*)dst = v;
+                        *(Placed*)dst = v[j];
                     } else {
 #pragma unroll
                         for (int e = 0; e < kPer; ++e)
-                            if (col + e < args.N) dst[e] = v[e];
+                            if (col + e < args.N) dst[e] = v[j][e];
                     }
                 }
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     }
 };
+
+// Scheduling hint for a k-step of the uniform loop: one LDS read behind every second
+// product, so that the next step's reads hide under this step. (256 x 256 x 128, cycles of
+// the K loop at 4096 cubed: none 93.6k, one read a product 82.9k, one in two 82.4k, one in
+// four 89.4k.)
+template <int TM, int TN>
+__device__ __forceinline__ void interleaveReads() {
+    constexpr int kMfmas = TM * TN, kReads = TM + TN;
+#pragma unroll
+    for (int i = 0; i < kMfmas / 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        if (i < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    if (kReads > kMfmas / 2) __builtin_amdgcn_sched_group_barrier(0x100, kReads - kMfmas / 2, 0);
+}
 
 // Every wavefront runs the same phase at the same time: fragments are double-buffered
 // across k-steps, and the tile boundary sits inside the last k-step of a tile. Once tile
@@ -261,6 +333,7 @@ __device__ __forceinline__ void int8UniformLoop(Blk& blk) {
     constexpr int L = T::kLoadsPerTile;
     const int numK = blk.numK, numFull = blk.numFull;
 
+    blk.issueScales();
     staticFor<STAGES>([&](auto sC) {
         if (sC.value < numK) blk.template issueTile<false>(sC.value, sC.value);
     });
@@ -302,6 +375,7 @@ __device__ __forceinline__ void int8UniformLoop(Blk& blk) {
                     }
                     if (!steady && kt >= numFull) blk.clearBehind(kt, ks, fa[cur]);
                     blk.mfmaStep(fa[cur], fb[cur]);
+                    interleaveReads<T::TM, T::TN>();
                 });
             }
         });
@@ -310,6 +384,80 @@ __device__ __forceinline__ void int8UniformLoop(Blk& blk) {
     for (; kt0 + U - 1 + STAGES < numFull; kt0 += U) pass(kt0, std::true_type{});
     for (; kt0 < numK; kt0 += U) pass(kt0, std::false_type{});
     barrierLds();
+}
+
+// Ping-pong schedule for eight wavefronts, two on a SIMD: waves 0-3 and 4-7 alternate a
+// memory phase (refill the stage freed by tile kt - 1 with tile kt + STAGES - 1, read all
+// of tile kt's fragments) with a matrix phase (all its products), one barrier apart, so
+// that one wave's products cover the other's LDS and global traffic. Group 0 reads tile t
+// in phase 2 t, group 1 in phase 2 t + 1.
+//  * A stage is refilled after both groups have read it: tile t + STAGES - 1 goes where
+//    tile t - 1 was and is issued in phase 2 t or 2 t + 1.
+//  * Tile t + 1 is in LDS before the barrier of phases 2 t + 1 | 2 t + 2: group 0 comes to
+//    it behind its matrix phase and group 1 behind its memory phase, and each first waits
+//    until only tiles t + 2 .. t + STAGES - 1 of its own loads are outstanding.
+template <typename T, typename Blk>
+__device__ __forceinline__ void int8PingPongLoop(Blk& blk) {
+    static_assert(T::kWaves == 8 && T::kStages >= 3, "two groups of four waves, and a refill ahead of two tiles");
+    constexpr int STAGES = T::kStages;
+    constexpr int KS = T::KS;
+    constexpr int L = T::kLoadsPerTile;
+    const int numK = blk.numK, numFull = blk.numFull;
+
+    blk.issueScales();
+    staticFor<STAGES - 1>([&](auto sC) {
+        if (sC.value < numK) blk.template issueTile<false>(sC.value, sC.value);
+    });
+    if (numK >= STAGES - 1) {
+        waitVmcnt<(STAGES - 2) * L>();
+    } else {
+        waitVmcnt<0>();
+    }
+    barrierLds();
+
+    // STEADY: the refill tile kt + STAGES - 1 exists and K fills it.
+    auto tileBody = [&](auto sC, auto groupC, int kt, auto steadyC) {
+        constexpr int s = sC.value;
+        constexpr int sRefill = (s + STAGES - 1) % STAGES;
+        constexpr int group = groupC.value;
+        constexpr bool steady = steadyC.value;
+        const bool refill = steady || kt + STAGES - 1 < numK;
+        if (refill) blk.template issueTile<steady>(kt + STAGES - 1, sRefill);
+        int4_t fa[KS][T::TM], fb[KS][T::TN];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) blk.template readFrags<s>(ks, fa[ks], fb[ks]);
+        auto wait = [&] {
+            if (refill) waitVmcnt<(STAGES - 2) * L>();
+            else waitVmcnt<0>();
+        };
+        if constexpr (group == 1) wait();
+        phaseBarrier();
+        if (!steady && kt >= numFull) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) blk.clearBehind(kt, ks, fa[ks]);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) blk.mfmaStep(fa[ks], fb[ks]);
+        if constexpr (group == 0) wait();
+        phaseBarrier();
+    };
+    auto runGroup = [&](auto groupC) {
+        if constexpr (groupC.value == 1) barrierLds();
+        int kt0 = 0;
+        for (; kt0 + 2 * STAGES - 2 < numFull; kt0 += STAGES)
+            staticFor<STAGES>([&](auto sC) { tileBody(sC, groupC, kt0 + sC.value, std::true_type{}); });
+        for (; kt0 < numK; kt0 += STAGES)
+            staticFor<STAGES>([&](auto sC) {
+                if (kt0 + sC.value < numK) tileBody(sC, groupC, kt0 + sC.value, std::false_type{});
+            });
+        // Matches group 1's at the start: behind it every wave is past its last read.
+        if constexpr (groupC.value == 0) barrierLds();
+    };
+    if (blk.wave / 4 == 0) {
+        runGroup(std::integral_constant<int, 0>{});
+    } else {
+        runGroup(std::integral_constant<int, 1>{});
+    }
 }
 
 constexpr int kInt8GroupM = 8;
@@ -323,7 +471,7 @@ __host__ __device__ inline int int8TilesN(int N) {
     return (N + T::BN - 1) / T::BN;
 }
 
-template <typename T, typename Out>
+template <typename T, typename Out, bool PINGPONG>
 __global__ __launch_bounds__(T::kThreads)
 void int8GemmKernel(Int8Args args) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLdsBytes];
@@ -332,8 +480,154 @@ void int8GemmKernel(Int8Args args) {
     tileOf<T::BM, T::BN, kInt8GroupM>(xcdRemap(blockIdx.x, tilesM * tilesN), tilesM * T::BM, tilesN * T::BN,
                                       args.order, row, col);
     Int8Block<T, Out> blk(lds, args, row, col);
-    int8UniformLoop<T>(blk);
+    if constexpr (PINGPONG) {
+        int8PingPongLoop<T>(blk);
+    } else {
+        int8UniformLoop<T>(blk);
+    }
     blk.store();
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens: up to 16 TM rows of A, where B's bytes are all there is to move.
+//
+// A workgroup owns 16 TN channels and all tokens, and its WAVES wavefronts share K: wave
+// w takes the 128-byte pieces w, w + WAVES, ... of every row, so that the workgroup reads
+// its rows front to back. A wave streams its pieces through a ring of its own in LDS
+// (eight lanes load a row's 128 bytes, one fragment read takes 16 rows: straight to
+// registers the 16 lanes of a load would be 16 rows apart) and waits for nothing but its
+// own loads: there is no barrier before the end, where the sums meet. They are 32-bit
+// integers, whose order does not matter.
+// ---------------------------------------------------------------------------
+template <int TM_, int TN_, int WAVES_, int STAGES_>
+struct Int8FewTraits {
+    static constexpr int TM = TM_, TN = TN_, kWaves = WAVES_, kStages = STAGES_;
+    static constexpr int kThreads = kWaves * kWaveSize;
+    static constexpr int kPiece = 128;                       // bytes of a row a wave takes at once
+    static constexpr int CPR = kPiece / 16;
+    static constexpr int KS = kPiece / kInt8MfmaK;
+    static constexpr int kTiles = TM * TN;                   // 16 x 16 tiles of C
+    static constexpr int kPieceBytes = 16 * (TM + TN) * kPiece;
+    static constexpr int kLoads = kPieceBytes / 1024;        // of a wave for a piece
+    static constexpr int kWaveBytes = kStages * kPieceBytes;
+    static constexpr int kLdsBytes = kWaves * kWaveBytes;
+    static_assert(kLdsBytes <= 163840, "LDS is 160 KiB per workgroup on gfx950");
+    static_assert((kStages - 1) * kLoads < 64, "in-flight loads exceed the vmcnt counter");
+    static_assert(kTiles * 1024 <= kWaveBytes, "a wave's sums replace its ring");
+};
+
+template <typename T, typename Out>
+__global__ __launch_bounds__(T::kThreads)
+void int8FewKernel(Int8Args args) {
+    constexpr int TM = T::TM, TN = T::TN, KS = T::KS, CPR = T::CPR, STAGES = T::kStages, L = T::kLoads;
+    __shared__ __attribute__((aligned(1024))) char lds[T::kLdsBytes];
+    const int lane = threadIdx.x % kWaveSize;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const int col0 = blockIdx.x * 16 * TN;
+    const int r16 = lane % 16, g = lane / 16;
+
+    // A piece in LDS: 16 TN rows of B, then 16 TM rows of A. Load i fills eight of them.
+    const char* gB = (const char*)args.B + (int64_t)col0 * args.ldb;
+    uint32_t off[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+        const int q = swizzleRows<CPR>(64 * i + lane), row = q / CPR;
+        off[i] = (uint32_t)(q % CPR) * 16u + (i < 2 * TN ? (uint32_t)min(row, args.N - 1 - col0) * (uint32_t)args.ldb
+                                                         : (uint32_t)min(row - 16 * TN, args.M - 1) * (uint32_t)args.lda);
+    }
+    const uint32_t ring = ldsAddress(lds) + wave * T::kWaveBytes;
+    const int pieces = (args.K + T::kPiece - 1) / T::kPiece;
+    auto issue = [&](int piece, int stage) {
+        const int64_t at = (int64_t)piece * T::kPiece;
+        // How far behind the last chunk of K this lane's chunk is.
+        const int last = min((args.K - 1) / 16 - piece * CPR, CPR - 1);
+        auto past = [&](int i) { return (uint32_t)max(swizzleRows<CPR>(64 * i + lane) % CPR - last, 0) * 16u; };
+#pragma unroll
+        for (int i = 0; i < L; ++i)
+            globalLoadLds16((i < 2 * TN ? gB : (const char*)args.A) + at, off[i] - past(i),
+                            ring + stage * T::kPieceBytes + i * 1024);
+    };
+    int4_t acc[TM][TN];
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) acc[tm][tn] = int4_t{0, 0, 0, 0};
+
+    const int mine = (pieces - wave + T::kWaves - 1) / T::kWaves;   // this wave's pieces; none or less: 0
+    const RIDGE_LDS_AS char* const own = (const RIDGE_LDS_AS char*)(lds) + wave * T::kWaveBytes;
+    const int rd = swizzleRows<CPR>(r16 * CPR + g) * 16;             // k-step 0; step ks flips chunk bit 2
+    staticFor<STAGES>([&](auto sC) {
+        if (sC.value < mine) issue(wave + sC.value * T::kWaves, sC.value);
+    });
+    for (int i0 = 0; i0 < mine; i0 += STAGES) {
+        staticFor<STAGES>([&](auto sC) {
+            constexpr int s = sC.value;
+            const int i = i0 + s;
+            if (i < mine) {
+                if (i + STAGES - 1 < mine) {
+                    waitVmcnt<(STAGES - 1) * L>();
+                } else {
+                    waitVmcnt<0>();
+                }
+                int4_t a[KS][TM], b[KS][TN];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const RIDGE_LDS_AS char* at = own + s * T::kPieceBytes + (rd ^ (ks * 64));
+#pragma unroll
+                    for (int tn = 0; tn < TN; ++tn) b[ks][tn] = *(const RIDGE_LDS_AS int4_t*)(at + tn * 2048);
+#pragma unroll
+                    for (int tm = 0; tm < TM; ++tm) a[ks][tm] = *(const RIDGE_LDS_AS int4_t*)(at + (TN + tm) * 2048);
+                }
+                const int piece = wave + i * T::kWaves;
+                // The stage has been read before it is filled again.
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (i + STAGES < mine) issue(piece + STAGES * T::kWaves, s);
+                if (piece * T::kPiece + T::kPiece > args.K) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const int4_t mask = firstBytes(args.K - (piece * T::kPiece + ks * kInt8MfmaK + 16 * g));
+#pragma unroll
+                        for (int tm = 0; tm < TM; ++tm) a[ks][tm] &= mask;
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+                        for (int tm = 0; tm < TM; ++tm)
+                            acc[tm][tn] =
+                                __builtin_amdgcn_mfma_i32_16x16x64_i8(b[ks][tn], a[ks][tm], acc[tm][tn], 0, 0, 0);
+            }
+        });
+    }
+
+    int4_t* sums = (int4_t*)(lds + wave * T::kWaveBytes);
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) sums[(tm * TN + tn) * kWaveSize + lane] = acc[tm][tn];
+    __syncthreads();
+    // Wave w finishes the tiles w, w + WAVES, ...: lane l has token 16 tm + l % 16 and the
+    // four channels from 16 tn + 4 (l / 16) on.
+    for (int t = wave; t < T::kTiles; t += T::kWaves) {
+        int4_t total = int4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < T::kWaves; ++w)
+            total += *(const int4_t*)(lds + w * T::kWaveBytes + (t * kWaveSize + lane) * 16);
+        const int row = 16 * (t / TN) + r16, col = col0 + 16 * (t % TN) + 4 * g;
+        if (row < args.M) {
+            const float sa = args.scaleA[row];
+            Out* dst = (Out*)args.C + (int64_t)row * args.ldc + col;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (col + e < args.N) {
+                    const float add = args.bias ? (float)((const Out*)args.bias)[col + e] : 0.0f;
+                    dst[e] = (Out)scaledSum(total[e], sa, args.scaleB[col + e], add);
+                }
+            }
+        }
+    }
 }
 
 }  // namespace ridge
