@@ -6,6 +6,7 @@
 Outputs (git-ignored, shipped with the tree):
     ridge_amd/lib/libridge_gemm.so   GEMM kernel table, fills, hipBLASLt comparator
     ridge_amd/lib/libridge_int8.so   the 8-bit operators (include/ridge_int8.h)
+    ridge_amd/lib/_ridge_int8.so     their calls on torch's tensors, a Python extension
     ridge_amd/lib/libridge_model.so  the cost model behind a C ABI
     ridge_amd/bin/ridge-predict      the model CLI (reference tools/ridge-predict.cpp)
     ridge_amd/bin/ridge-check        correctness + throughput harness (bench/check-gemm.cu)
@@ -214,6 +215,24 @@ def build_int8(gate=True):
         raise SystemExit("spill gate: %d 8-bit kernel(s) use scratch" % spilling)
     so = os.path.join(LIB, "libridge_int8.so")
     _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", so + ".tmp"] + objs)
+    os.replace(so + ".tmp", so)
+    build_int8_binding()
+    return so
+
+
+def build_int8_binding():
+    """_ridge_int8.so: host code over libridge_int8.so, torch's tensors and its streams."""
+    import sysconfig
+    import torch
+    torch_dir = os.path.dirname(torch.__file__)
+    so = os.path.join(LIB, "_ridge_int8.so")
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+          "-I" + INCLUDE, "-isystem", os.path.join(torch_dir, "include"), "-isystem",
+          os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), "-isystem", "/opt/rocm/include",
+          "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "int8_binding.cpp"), "-o", so + ".tmp",
+          "-L" + LIB, "-lridge_int8", "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+          "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
     os.replace(so + ".tmp", so)
     return so
 
