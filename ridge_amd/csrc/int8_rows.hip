@@ -48,10 +48,11 @@ __device__ __forceinline__ void storeRow(T* at, const float (&v)[n]) {
     *(typename Memory<T, n>::Vec*)at = m;
 }
 
-// Nearest whole numbers (halves to even) of v / scale. The quotient is the correctly
-// rounded one, by one correction of v * (1 / scale) with its exact remainder: a product
-// alone rounds values near a half the other way. The bounds also give a NaN a value: its
-// row's scale is one.
+// Nearest whole numbers (halves to even) of v / scale, which is at most 127 and a rounding.
+// The quotient is the correctly rounded one, by one correction of v * (1 / scale) with its
+// exact remainder: a product alone rounds values near a half the other way. Adding 1.5 *
+// 2^23 leaves the whole number in the low bits. A row whose scale is not finite gets bytes
+// that mean nothing.
 template <int n>
 __device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], float scale, float inverse) {
     typename Memory<signed char, n>::Vec b;
@@ -59,7 +60,7 @@ __device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], fl
     for (int e = 0; e < n; ++e) {
         float t = v[e] * inverse;
         t = fmaf(fmaf(-t, scale, v[e]), inverse, t);
-        b[e] = (signed char)(int)fminf(fmaxf(rintf(t), -127.0f), 127.0f);
+        b[e] = (signed char)__float_as_uint(t + 12582912.0f);
     }
     *(typename Memory<signed char, n>::Vec*)at = b;
 }
@@ -77,6 +78,18 @@ struct RowArgs {
     int64_t ldResidual, ldResidualOut;
     float eps;
 };
+
+// v / d for d of 1 and more, rounded correctly but where d comes near the range's end and
+// the quotient is nothing beside it: Newton's step on the reciprocal, the product, and
+// its exact remainder's correction. Six instructions where a division of any two numbers
+// takes ten.
+__device__ __forceinline__ float quotient(float v, float d) {
+    float r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    float q = v * r;
+    q = fmaf(fmaf(-d, q, v), r, q);
+    return d > 1e37f ? v * 0.0f : q;
+}
 
 // Sources of a row's values: load() gives n of them from column col on, and adds what the
 // norm sums up.
@@ -103,7 +116,7 @@ struct Gated {
         loadRow(x + col, v);
         loadRow(x + cols + col, u);
 #pragma unroll
-        for (int e = 0; e < n; ++e) v[e] = v[e] / (1.0f + expf(-v[e])) * u[e];
+        for (int e = 0; e < n; ++e) v[e] = quotient(v[e], 1.0f + expf(-v[e])) * u[e];
     }
 };
 
@@ -265,15 +278,18 @@ hipError_t launchRows(const RowArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// The threads of a row, by its length: as many as hold it in at most four vectors each,
-// two for the norm on 1024 threads, whose registers would not hold more.
+// The threads of a row, by its length: as many as hold it in at most four vectors each. A
+// norm's 1024 threads have not got the registers for that: it reads rows of more than
+// 16384 columns twice.
 template <typename Source>
 hipError_t launchByLength(const RowArgs& a, hipStream_t stream) {
     if (a.cols <= 64 * kVec) return launchRows<Source, 64, 1>(a, stream);
     if (a.cols <= 64 * kVec * 4) return launchRows<Source, 64, 4>(a, stream);
     if (a.cols <= 256 * kVec * 4) return launchRows<Source, 256, 4>(a, stream);
-    constexpr int kMostVecs = Source::kNorm ? 2 : 4;
-    if (a.cols <= 1024 * kVec * kMostVecs) return launchRows<Source, 1024, kMostVecs>(a, stream);
+    if (a.cols <= 512 * kVec * 4) return launchRows<Source, 512, 4>(a, stream);
+    if constexpr (!Source::kNorm) {
+        if (a.cols <= 1024 * kVec * 4) return launchRows<Source, 1024, 4>(a, stream);
+    }
     return launchRows<Source, 1024, 0>(a, stream);
 }
 
