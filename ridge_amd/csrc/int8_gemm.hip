@@ -23,7 +23,7 @@ hipError_t launchTiles(Int8Args args, hipStream_t stream) {
 template <typename T, typename Out>
 hipError_t launchFew(const Int8Args& args, hipStream_t stream) {
     const unsigned blocks = (unsigned)((args.N + 16 * T::TN - 1) / (16 * T::TN));
-    ridge::int8FewKernel<T, Out><<<dim3(blocks), dim3(T::kThreads), 0, stream>>>(args);
+    ridge::int8FewKernel<T, Out><<<dim3(blocks), dim3(T::kThreads), 0, stream>>>(ridge::fewArgs(args));
     return hipGetLastError();
 }
 
@@ -62,10 +62,11 @@ hipError_t launchGemm(const Int8Args& args, hipStream_t stream) {
     // would leave three CUs in four idle. us, few | 64 x 64 tiles, K = 4096: 1 x 4096 4.9 |
     // 7.4, 20 x 4096 5.7 | 7.6, 64 x 4096 8.3 | 8.2; 64 x 2000 x 8000 11.5 | 16.8; 1 x 1000
     // x 16384 7.1 | 20.5. With twice the channels the tiles are as fast: 16 x 8192 8.2 | 7.8.
-    if (args.N <= 16 * kCUs) {
+    static_assert(ridge::kFewMostN == 16 * kCUs, "a workgroup of 16 channels on each CU");
+    if (args.N <= ridge::kFewMostN && args.ldc <= UINT32_MAX) {
         if (args.M <= 16) return launchFew<ridge::Int8FewTraits<1, 1, 16, 2>, Out>(args, stream);
         if (args.M <= 32) return launchFew<ridge::Int8FewTraits<2, 1, 8, 2>, Out>(args, stream);
-        if (args.M <= 64) return launchFew<ridge::Int8FewTraits<4, 1, 8, 2>, Out>(args, stream);
+        if (args.M <= ridge::kFewMostM) return launchFew<ridge::Int8FewTraits<4, 1, 8, 2>, Out>(args, stream);
     }
     switch (chooseTile(args.M, args.N)) {
         case 0: return launchTiles<Tile256x256, Out, false>(args, stream);

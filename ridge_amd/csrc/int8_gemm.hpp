@@ -499,6 +499,28 @@ void int8GemmKernel(Int8Args args) {
 // own loads: there is no barrier before the end, where the sums meet. They are 32-bit
 // integers, whose order does not matter.
 // ---------------------------------------------------------------------------
+// In 64 bytes: arguments are written to device memory before a launch, and a second line
+// of them would cost 0.8 us of the host's time. Strides are multiples of 16 below 2^23.
+constexpr int kFewMostM = 64, kFewMostN = 4096;
+struct Int8FewArgs {
+    const int8_t* A;
+    const int8_t* B;
+    const float* scaleA;
+    const float* scaleB;
+    const void* bias;
+    void* C;
+    uint32_t strideAndM;   // lda / 16 in 19 bits, M
+    uint32_t strideAndN;   // ldb / 16 in 19 bits, N
+    int K;
+    uint32_t ldc;
+};
+static_assert(sizeof(Int8FewArgs) <= 64 && kFewMostM < (1 << 13) && kFewMostN < (1 << 13), "arguments of one write");
+
+inline Int8FewArgs fewArgs(const Int8Args& a) {
+    return {a.A, a.B, a.scaleA, a.scaleB, a.bias, a.C, (uint32_t)a.lda / 16 | (uint32_t)a.M << 19,
+            (uint32_t)a.ldb / 16 | (uint32_t)a.N << 19, a.K, (uint32_t)a.ldc};
+}
+
 template <int TM_, int TN_, int WAVES_, int STAGES_>
 struct Int8FewTraits {
     static constexpr int TM = TM_, TN = TN_, kWaves = WAVES_, kStages = STAGES_;
@@ -518,7 +540,9 @@ struct Int8FewTraits {
 
 template <typename T, typename Out>
 __global__ __launch_bounds__(T::kThreads)
-void int8FewKernel(Int8Args args) {
+void int8FewKernel(Int8FewArgs args) {
+    const int M = (int)(args.strideAndM >> 19), N = (int)(args.strideAndN >> 19);
+    const uint32_t lda = (args.strideAndM & 0x7ffff) * 16, ldb = (args.strideAndN & 0x7ffff) * 16;
     constexpr int TM = T::TM, TN = T::TN, KS = T::KS, CPR = T::CPR, STAGES = T::kStages, L = T::kLoads;
     __shared__ __attribute__((aligned(1024))) char lds[T::kLdsBytes];
     const int lane = threadIdx.x % kWaveSize;
@@ -527,13 +551,13 @@ void int8FewKernel(Int8Args args) {
     const int r16 = lane % 16, g = lane / 16;
 
     // A piece in LDS: 16 TN rows of B, then 16 TM rows of A. Load i fills eight of them.
-    const char* gB = (const char*)args.B + (int64_t)col0 * args.ldb;
+    const char* gB = (const char*)args.B + (int64_t)col0 * ldb;
     uint32_t off[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
         const int q = swizzleRows<CPR>(64 * i + lane), row = q / CPR;
-        off[i] = (uint32_t)(q % CPR) * 16u + (i < 2 * TN ? (uint32_t)min(row, args.N - 1 - col0) * (uint32_t)args.ldb
-                                                         : (uint32_t)min(row - 16 * TN, args.M - 1) * (uint32_t)args.lda);
+        off[i] = (uint32_t)(q % CPR) * 16u + (i < 2 * TN ? (uint32_t)min(row, N - 1 - col0) * ldb
+                                                         : (uint32_t)min(row - 16 * TN, M - 1) * lda);
     }
     const uint32_t ring = ldsAddress(lds) + wave * T::kWaveBytes;
     const int pieces = (args.K + T::kPiece - 1) / T::kPiece;
@@ -616,12 +640,12 @@ void int8FewKernel(Int8Args args) {
         for (int w = 0; w < T::kWaves; ++w)
             total += *(const int4_t*)(lds + w * T::kWaveBytes + (t * kWaveSize + lane) * 16);
         const int row = 16 * (t / TN) + r16, col = col0 + 16 * (t % TN) + 4 * g;
-        if (row < args.M) {
+        if (row < M) {
             const float sa = args.scaleA[row];
             Out* dst = (Out*)args.C + (int64_t)row * args.ldc + col;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (col + e < args.N) {
+                if (col + e < N) {
                     const float add = args.bias ? (float)((const Out*)args.bias)[col + e] : 0.0f;
                     dst[e] = (Out)scaledSum(total[e], sa, args.scaleB[col + e], add);
                 }

@@ -33,19 +33,32 @@ struct Memory {
 };
 typedef signed char Bytes8 __attribute__((ext_vector_type(kVec), aligned(8)));
 
-template <int n, typename T>
+// STREAM: past the caches. A template argument, because the compiler merges the two
+// accesses of a run-time choice and drops the hint.
+template <bool STREAM, int n, typename T>
 __device__ __forceinline__ void loadRow(const T* at, float (&v)[n]) {
-    const typename Memory<T, n>::Vec m = *(const typename Memory<T, n>::Vec*)at;
+    typedef typename Memory<T, n>::Vec Vec;
+    Vec m;
+    if constexpr (STREAM && n > 1) {
+        m = __builtin_nontemporal_load((const Vec*)at);
+    } else {
+        m = *(const Vec*)at;
+    }
 #pragma unroll
     for (int e = 0; e < n; ++e) v[e] = (float)m[e];
 }
 
-template <int n, typename T>
+template <bool STREAM, int n, typename T>
 __device__ __forceinline__ void storeRow(T* at, const float (&v)[n]) {
-    typename Memory<T, n>::Vec m;
+    typedef typename Memory<T, n>::Vec Vec;
+    Vec m;
 #pragma unroll
     for (int e = 0; e < n; ++e) m[e] = (T)v[e];
-    *(typename Memory<T, n>::Vec*)at = m;
+    if constexpr (STREAM && n > 1) {
+        __builtin_nontemporal_store(m, (Vec*)at);
+    } else {
+        *(Vec*)at = m;
+    }
 }
 
 // Nearest whole numbers (halves to even) of v / scale, which is at most 127 and a rounding.
@@ -65,18 +78,54 @@ __device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], fl
     *(typename Memory<signed char, n>::Vec*)at = b;
 }
 
+// A launch's arguments. They are written to device memory before it, 64 bytes at a time:
+// a kernel that takes more waits for a second write, 3.5 us of the host's time a call
+// instead of 2.7. What a kernel takes beyond these counts too: it must not ask for its
+// grid's size.
 struct RowArgs {
     const void* x;
     int8_t* q;
     float* scale;
-    int64_t ldx, ldq;
+    int64_t ldx, strideQ;
     int rows, cols;
-    // rms_norm
+    __device__ int64_t ldq() const { return strideQ; }
+};
+
+// The norm's, with all its matrices contiguous (the common case, which fits) or with
+// strides.
+template <bool DENSE>
+struct NormArgs;
+template <>
+struct NormArgs<true> {
+    const void* x;
+    int8_t* q;
+    float* scale;
     const void* residual;
     const void* weight;
     void* residualOut;
-    int64_t ldResidual, ldResidualOut;
+    int rows, cols;
     float eps;
+    __device__ int64_t ldq() const { return ((int64_t)cols + 15) / 16 * 16; }
+    __device__ int64_t ldxOf() const { return cols; }
+    __device__ int64_t ldResidualOf() const { return cols; }
+    __device__ int64_t ldResidualOutOf() const { return cols; }
+};
+static_assert(sizeof(RowArgs) <= 64 && sizeof(NormArgs<true>) <= 64, "arguments of one write");
+template <>
+struct NormArgs<false> {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    const void* residual;
+    const void* weight;
+    void* residualOut;
+    int rows, cols;
+    float eps;
+    int64_t ldx, strideQ, ldResidual, ldResidualOut;
+    __device__ int64_t ldq() const { return strideQ; }
+    __device__ int64_t ldxOf() const { return ldx; }
+    __device__ int64_t ldResidualOf() const { return ldResidual; }
+    __device__ int64_t ldResidualOutOf() const { return ldResidualOut; }
 };
 
 // v / d for d of 1 and more, rounded correctly but where d comes near the range's end and
@@ -93,28 +142,30 @@ __device__ __forceinline__ float quotient(float v, float d) {
 
 // Sources of a row's values: load() gives n of them from column col on, and adds what the
 // norm sums up.
-template <typename T>
+template <typename T, bool STREAM>
 struct Plain {
+    typedef RowArgs Args;
     static constexpr bool kNorm = false;
     const T* x;
-    __device__ Plain(const RowArgs& a, int64_t row) : x((const T*)a.x + row * a.ldx) {}
+    __device__ Plain(const Args& a, int64_t row) : x((const T*)a.x + row * a.ldx) {}
     template <int n>
     __device__ void load(int col, float (&v)[n], float&, bool) const {
-        loadRow(x + col, v);
+        loadRow<STREAM>(x + col, v);
     }
 };
 
-template <typename T>
+template <typename T, bool STREAM>
 struct Gated {
+    typedef RowArgs Args;
     static constexpr bool kNorm = false;
     const T* x;
     int cols;
-    __device__ Gated(const RowArgs& a, int64_t row) : x((const T*)a.x + row * a.ldx), cols(a.cols) {}
+    __device__ Gated(const Args& a, int64_t row) : x((const T*)a.x + row * a.ldx), cols(a.cols) {}
     template <int n>
     __device__ void load(int col, float (&v)[n], float&, bool) const {
         float u[n];
-        loadRow(x + col, v);
-        loadRow(x + cols + col, u);
+        loadRow<STREAM>(x + col, v);
+        loadRow<STREAM>(x + cols + col, u);
 #pragma unroll
         for (int e = 0; e < n; ++e) v[e] = quotient(v[e], 1.0f + expf(-v[e])) * u[e];
     }
@@ -122,30 +173,31 @@ struct Gated {
 
 // The residual's sum leaves with the row's last reading, so that it may replace x or the
 // residual.
-template <typename T, typename W>
+template <typename T, typename W, bool STREAM, bool DENSE>
 struct Normed {
+    typedef NormArgs<DENSE> Args;
     static constexpr bool kNorm = true;
     const T* x;
     const T* residual;
     const W* weight;
     T* out;
-    __device__ Normed(const RowArgs& a, int64_t row)
-        : x((const T*)a.x + row * a.ldx),
-          residual(a.residual ? (const T*)a.residual + row * a.ldResidual : nullptr),
+    __device__ Normed(const Args& a, int64_t row)
+        : x((const T*)a.x + row * a.ldxOf()),
+          residual(a.residual ? (const T*)a.residual + row * a.ldResidualOf() : nullptr),
           weight((const W*)a.weight),
-          out(a.residualOut ? (T*)a.residualOut + row * a.ldResidualOut : nullptr) {}
+          out(a.residualOut ? (T*)a.residualOut + row * a.ldResidualOutOf() : nullptr) {}
     template <int n>
     __device__ void load(int col, float (&v)[n], float& squares, bool last) const {
         float w[n];
-        loadRow(x + col, v);
+        loadRow<STREAM>(x + col, v);
         if (residual) {
             float r[n];
-            loadRow(residual + col, r);
+            loadRow<STREAM>(residual + col, r);
 #pragma unroll
             for (int e = 0; e < n; ++e) v[e] += r[e];
-            if (last) storeRow(out + col, v);
+            if (last) storeRow<STREAM>(out + col, v);
         }
-        loadRow(weight + col, w);
+        loadRow<false>(weight + col, w);
 #pragma unroll
         for (int e = 0; e < n; ++e) {
             squares = fmaf(v[e], v[e], squares);
@@ -185,11 +237,13 @@ __device__ __forceinline__ void reduceRow(float& sum, uint32_t& top) {
     }
 }
 
+constexpr int64_t kMostBlocks = 1 << 20;  // of a grid: its blocks walk the rows behind them
+
 // One row a kThreads threads. kVecs vectors a thread hold the row; with kVecs = 0 a row
 // of any length is read twice.
 template <typename Source, int kThreads, int kVecs>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads)
-void makeRowsKernel(RowArgs a) {
+void makeRowsKernel(typename Source::Args a) {
     constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
     constexpr int kRowsPerBlock = kBlock / kThreads;
     constexpr bool kHeld = kVecs > 0;
@@ -197,7 +251,7 @@ void makeRowsKernel(RowArgs a) {
     const int whole = a.cols / kVec * kVec;    // columns of whole vectors
     const int single = whole + lane;           // and this lane's behind them
     for (int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + threadIdx.x / kThreads; row < a.rows;
-         row += (int64_t)gridDim.x * kRowsPerBlock) {
+         row += kMostBlocks * kRowsPerBlock) {
         const Source source(a, row);
         float v[kHeld ? kVecs : 1][kVec], one[1];
         float squares = 0.0f;
@@ -229,7 +283,7 @@ void makeRowsKernel(RowArgs a) {
         scale = scale < FLT_MIN ? FLT_MIN : scale;  // a NaN stays one
         const float inverse = 1.0f / scale;
         if (lane == 0) a.scale[row] = scale;
-        int8_t* const q = a.q + row * a.ldq;
+        int8_t* const q = a.q + row * a.ldq();
         parts([&](int col, auto& values) {
             if constexpr (!kHeld) source.load(col, values, squares, true);
             if constexpr (Source::kNorm) {
@@ -242,12 +296,12 @@ void makeRowsKernel(RowArgs a) {
 
 constexpr int kDequantizeThreads = 256;
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kDequantizeThreads)
 void dequantizeKernel(const int8_t* q, int64_t ldq, const float* scale, T* out, int64_t ldOut, int rows, int cols,
                       int pieces) {
     const int64_t total = (int64_t)rows * pieces;
-    for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+    for (int64_t i = blockIdx.x; i < total; i += kMostBlocks) {
         const int row = (int)(i / pieces);
         const int col = ((int)(i % pieces) * kDequantizeThreads + (int)threadIdx.x) * kVec;
         if (col >= cols) continue;
@@ -258,7 +312,7 @@ void dequantizeKernel(const int8_t* q, int64_t ldq, const float* scale, T* out, 
         for (int e = 0; e < kVec; ++e) v[e] = (float)b[e] * s;
         T* const at = out + row * ldOut + col;
         if (col + kVec <= cols) {
-            storeRow(at, v);
+            storeRow<STREAM>(at, v);
         } else {
 #pragma unroll
             for (int e = 0; e < kVec; ++e)
@@ -267,10 +321,14 @@ void dequantizeKernel(const int8_t* q, int64_t ldq, const float* scale, T* out, 
     }
 }
 
-constexpr int64_t kMostBlocks = 1 << 20;  // of a grid: blocks walk the rows behind it
+// 16- and 32-bit matrices of this size and more are read and written past the caches: who
+// comes next would not find them there, and the 8-bit rows, which the next product reads,
+// stay. us, cached | past the caches, the norm and a reader of its rows: 16384 x 8192 249 |
+// 225, 4096 x 16384 137 | 123, 2048 x 4096 18.7 | 21.0.
+constexpr int64_t kStreamBytes = (int64_t)64 << 20;
 
 template <typename Source, int kThreads, int kVecs>
-hipError_t launchRows(const RowArgs& a, hipStream_t stream) {
+hipError_t launchRows(const typename Source::Args& a, hipStream_t stream) {
     constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
     constexpr int kRowsPerBlock = kBlock / kThreads;
     const int64_t blocks = std::min<int64_t>((a.rows + (int64_t)kRowsPerBlock - 1) / kRowsPerBlock, kMostBlocks);
@@ -282,7 +340,7 @@ hipError_t launchRows(const RowArgs& a, hipStream_t stream) {
 // norm's 1024 threads have not got the registers for that: it reads rows of more than
 // 16384 columns twice.
 template <typename Source>
-hipError_t launchByLength(const RowArgs& a, hipStream_t stream) {
+hipError_t launchByLength(const typename Source::Args& a, hipStream_t stream) {
     if (a.cols <= 64 * kVec) return launchRows<Source, 64, 1>(a, stream);
     if (a.cols <= 64 * kVec * 4) return launchRows<Source, 64, 4>(a, stream);
     if (a.cols <= 256 * kVec * 4) return launchRows<Source, 256, 4>(a, stream);
@@ -307,19 +365,52 @@ bool rowsFit(const void* x, int64_t ldx, int64_t width, int type, const int8_t* 
            ldq >= cols && ldq % 16 == 0 && aligned(x, sizeOf(type)) && aligned(q, 16) && aligned(scale, 4);
 }
 
+bool streams(int64_t rows, int64_t cols, int type) { return rows * cols >= kStreamBytes / (int64_t)sizeOf(type); }
+
+template <template <typename, bool> class Source, typename T>
+hipError_t launchPlain(const RowArgs& a, bool stream, hipStream_t s) {
+    return stream ? launchByLength<Source<T, true>>(a, s) : launchByLength<Source<T, false>>(a, s);
+}
+
+template <template <typename, bool> class Source>
+hipError_t launchTyped(const RowArgs& a, int type, bool stream, hipStream_t s) {
+    switch (type) {
+        case RIDGE_F16: return launchPlain<Source, _Float16>(a, stream, s);
+        case RIDGE_BF16: return launchPlain<Source, __bf16>(a, stream, s);
+        default: return launchPlain<Source, float>(a, stream, s);
+    }
+}
+
+template <typename T, typename W>
+hipError_t launchNorm(const NormArgs<false>& a, bool stream, hipStream_t s) {
+    if (stream) return launchByLength<Normed<T, W, true, false>>(a, s);
+    const NormArgs<true> d = {a.x, a.q, a.scale, a.residual, a.weight, a.residualOut, a.rows, a.cols, a.eps};
+    const bool dense = a.rows == 1 || (a.ldx == a.cols && a.strideQ == ((int64_t)a.cols + 15) / 16 * 16 &&
+                                       (!a.residual || (a.ldResidual == a.cols && a.ldResidualOut == a.cols)));
+    return dense ? launchByLength<Normed<T, W, false, true>>(d, s) : launchByLength<Normed<T, W, false, false>>(a, s);
+}
+
+template <typename T>
+hipError_t launchDequantize(const int8_t* q, int64_t ldq, const float* scale, void* out, int64_t ldOut, int rows,
+                            int cols, bool stream, hipStream_t s) {
+    const int pieces = (int)(((int64_t)cols + kDequantizeThreads * kVec - 1) / (kDequantizeThreads * kVec));
+    const dim3 grid((unsigned)std::min<int64_t>((int64_t)rows * pieces, kMostBlocks)), block(kDequantizeThreads);
+    if (stream) {
+        dequantizeKernel<T, true><<<grid, block, 0, s>>>(q, ldq, scale, (T*)out, ldOut, rows, cols, pieces);
+    } else {
+        dequantizeKernel<T, false><<<grid, block, 0, s>>>(q, ldq, scale, (T*)out, ldOut, rows, cols, pieces);
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
 extern "C" int ridge_int8_quantize(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale,
                                    int64_t rows, int64_t cols, void* stream) {
     if (rows == 0 && cols > 0 && isType(type)) return hipSuccess;
     if (rows < 0 || !rowsFit(x, ldx, cols, type, q, ldq, scale, rows, cols)) return hipErrorInvalidValue;
-    RowArgs a = {x, q, scale, ldx, ldq, (int)rows, (int)cols, nullptr, nullptr, nullptr, 0, 0, 0.0f};
-    hipStream_t s = (hipStream_t)stream;
-    switch (type) {
-        case RIDGE_F16: return launchByLength<Plain<_Float16>>(a, s);
-        case RIDGE_BF16: return launchByLength<Plain<__bf16>>(a, s);
-        default: return launchByLength<Plain<float>>(a, s);
-    }
+    const RowArgs a = {x, q, scale, ldx, ldq, (int)rows, (int)cols};
+    return launchTyped<Plain>(a, type, streams(rows, cols, type), (hipStream_t)stream);
 }
 
 extern "C" int ridge_int8_silu_mul(const void* x, int64_t ldx, int type, int8_t* q, int64_t ldq, float* scale,
@@ -327,13 +418,8 @@ extern "C" int ridge_int8_silu_mul(const void* x, int64_t ldx, int type, int8_t*
     if (rows == 0 && cols > 0 && isType(type)) return hipSuccess;
     if (rows < 0 || cols > INT32_MAX / 2 || !rowsFit(x, ldx, 2 * cols, type, q, ldq, scale, rows, cols))
         return hipErrorInvalidValue;
-    RowArgs a = {x, q, scale, ldx, ldq, (int)rows, (int)cols, nullptr, nullptr, nullptr, 0, 0, 0.0f};
-    hipStream_t s = (hipStream_t)stream;
-    switch (type) {
-        case RIDGE_F16: return launchByLength<Gated<_Float16>>(a, s);
-        case RIDGE_BF16: return launchByLength<Gated<__bf16>>(a, s);
-        default: return launchByLength<Gated<float>>(a, s);
-    }
+    const RowArgs a = {x, q, scale, ldx, ldq, (int)rows, (int)cols};
+    return launchTyped<Gated>(a, type, streams(rows, 2 * cols, type), (hipStream_t)stream);
 }
 
 extern "C" int ridge_int8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldResidual,
@@ -349,19 +435,16 @@ extern "C" int ridge_int8_rms_norm(const void* x, int64_t ldx, const void* resid
     if (residual && (!aligned(residual, sizeOf(type)) || !aligned(residualOut, sizeOf(type)) || ldResidual < cols ||
                      ldResidualOut < cols))
         return hipErrorInvalidValue;
-    RowArgs a = {x,        q,      scale,       ldx,        ldq,           (int)rows, (int)cols,
-                 residual, weight, residualOut, ldResidual, ldResidualOut, eps};
+    const NormArgs<false> a = {x,         q,         scale, residual, weight, residualOut, (int)rows,
+                               (int)cols, eps,       ldx,   ldq,      ldResidual, ldResidualOut};
+    const bool past = streams(rows, cols, type);
     hipStream_t s = (hipStream_t)stream;
     switch (type) {
         case RIDGE_F16:
-            return weightType == RIDGE_F16
-                       ? launchByLength<Normed<_Float16, _Float16>>(a, s)
-                       : launchByLength<Normed<_Float16, float>>(a, s);
+            return weightType == type ? launchNorm<_Float16, _Float16>(a, past, s) : launchNorm<_Float16, float>(a, past, s);
         case RIDGE_BF16:
-            return weightType == RIDGE_BF16
-                       ? launchByLength<Normed<__bf16, __bf16>>(a, s)
-                       : launchByLength<Normed<__bf16, float>>(a, s);
-        default: return launchByLength<Normed<float, float>>(a, s);
+            return weightType == type ? launchNorm<__bf16, __bf16>(a, past, s) : launchNorm<__bf16, float>(a, past, s);
+        default: return launchNorm<float, float>(a, past, s);
     }
 }
 
@@ -369,18 +452,12 @@ extern "C" int ridge_int8_dequantize(const int8_t* q, int64_t ldq, const float* 
                                      int type, int64_t rows, int64_t cols, void* stream) {
     if (rows == 0 && cols > 0 && isType(type)) return hipSuccess;
     if (rows < 0 || !rowsFit(out, ldOut, cols, type, q, ldq, scale, rows, cols)) return hipErrorInvalidValue;
+    const bool past = streams(rows, cols, type);
+    const int r = (int)rows, c = (int)cols;
     hipStream_t s = (hipStream_t)stream;
-    const int pieces = (int)((cols + kDequantizeThreads * kVec - 1) / (kDequantizeThreads * kVec));
-    const dim3 grid((unsigned)std::min(rows * pieces, kMostBlocks)), block(kDequantizeThreads);
     switch (type) {
-        case RIDGE_F16:
-            dequantizeKernel<<<grid, block, 0, s>>>(q, ldq, scale, (_Float16*)out, ldOut, (int)rows, (int)cols, pieces);
-            break;
-        case RIDGE_BF16:
-            dequantizeKernel<<<grid, block, 0, s>>>(q, ldq, scale, (__bf16*)out, ldOut, (int)rows, (int)cols, pieces);
-            break;
-        default:
-            dequantizeKernel<<<grid, block, 0, s>>>(q, ldq, scale, (float*)out, ldOut, (int)rows, (int)cols, pieces);
+        case RIDGE_F16: return launchDequantize<_Float16>(q, ldq, scale, out, ldOut, r, c, past, s);
+        case RIDGE_BF16: return launchDequantize<__bf16>(q, ldq, scale, out, ldOut, r, c, past, s);
+        default: return launchDequantize<float>(q, ldq, scale, out, ldOut, r, c, past, s);
     }
-    return hipGetLastError();
 }
