@@ -154,9 +154,9 @@ struct RowsOut {
     int64_t ld = 0;
     RowsOut(PyObject* out, int64_t rows, int64_t cols, const at::Device& device) : given(out) {
         if (out == Py_None) {
-            q = at::empty({rows, to16(cols)}, at::TensorOptions(device).dtype(at::kChar)).narrow(1, 0, cols);
+            ld = ridge_int8_row_stride(cols);
+            q = at::empty({rows, ld}, at::TensorOptions(device).dtype(at::kChar)).narrow(1, 0, cols);
             scale = at::empty({rows}, at::TensorOptions(device).dtype(at::kFloat));
-            ld = to16(cols);
             return;
         }
         if (!PyTuple_Check(out) || PyTuple_GET_SIZE(out) != 2) refuse("out must be (q, scale)");

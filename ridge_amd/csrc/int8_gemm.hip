@@ -7,79 +7,117 @@
 
 namespace {
 
-using ridge::Int8Args;
+using ridge::Int8Operands;
+using ridge::Int8Sizes;
 
-constexpr int kCUs = 256;   // of an MI355X
-
-template <typename T, typename Out, bool PINGPONG>
-hipError_t launchTiles(Int8Args args, hipStream_t stream) {
-    const int64_t tilesM = ridge::int8TilesM<T>(args.M), tilesN = ridge::int8TilesN<T>(args.N);
-    if (tilesM * tilesN > (int64_t)UINT32_MAX / T::kThreads) return hipErrorInvalidValue;
-    args.order = ridge::tileOrder<T::BM, T::BN, ridge::kInt8GroupM>((int)tilesM * T::BM, (int)tilesN * T::BN);
-    ridge::int8GemmKernel<T, Out, PINGPONG><<<dim3((unsigned)(tilesM * tilesN)), dim3(T::kThreads), 0, stream>>>(args);
-    return hipGetLastError();
-}
-
-template <typename T, typename Out>
-hipError_t launchFew(const Int8Args& args, hipStream_t stream) {
-    const unsigned blocks = (unsigned)((args.N + 16 * T::TN - 1) / (16 * T::TN));
-    ridge::int8FewKernel<T, Out><<<dim3(blocks), dim3(T::kThreads), 0, stream>>>(ridge::fewArgs(args));
-    return hipGetLastError();
-}
-
-// The tiles, eight wavefronts each, and what a CU takes for one of each with the chip
-// full, in 2.5 ns a 64 k (measured at K = 4096).
+// How a product runs, by number: tiles of C as one workgroup each, or (kFew) small ones
+// whose K a workgroup's waves share.
 using Tile256x256 = ridge::Int8Traits<256, 256, 128, 128, 64, 2>;
-using Tile256x128 = ridge::Int8Traits<256, 128, 128, 64, 64, 3>;   // ping-pong: 5% faster than uniform
+using Tile256x128 = ridge::Int8Traits<256, 128, 128, 64, 64, 3>;   // ping-pong
 using Tile128x128 = ridge::Int8Traits<128, 128, 128, 32, 64, 3>;
+using Pair128x128 = ridge::Int8Traits<128, 128, 128, 32, 64, 2>;   // two workgroups a CU
 using Tile64x128 = ridge::Int8Traits<64, 128, 128, 32, 32, 3>;
 using Tile64x64 = ridge::Int8Traits<64, 64, 128, 16, 32, 4>;
-constexpr int kTiles = 5;
-constexpr int kTileRows[kTiles] = {256, 256, 128, 64, 64};
-constexpr int kTileCols[kTiles] = {256, 128, 128, 128, 64};
-constexpr int64_t kTileCost[kTiles] = {470, 280, 175, 107, 73};
+using Few16x16 = ridge::Int8FewTraits<1, 1, 8, 2>;
+using Few32x16 = ridge::Int8FewTraits<2, 1, 8, 2>;
+using Few32x32 = ridge::Int8FewTraits<2, 2, 8, 2>;
 
-// The tile whose grid keeps the busiest CU shortest, the larger one where two are alike. A
-// smaller tile moves more operand bytes for its products, a larger one leaves CUs idle on
-// a small grid. Measured at K = 4096, us, 256x256 | 256x128 | 128x128 | 64x128 | 64x64:
-// 256 x 4096 40 | 22.6 | 17.5 | 12.1 | 9.0; 512 x 4096 40 | 22.9 | 17.8 | 13.2 | 14.5;
-// 1024 x 4096 40 | 23.5 | 20.1 | 21.8 | 26.8; 2048 x 4096 43 | 30.9 | 40 | 42 | 51;
-// 4096 x 4096 53 | 61 | 77 | 81 | 101.
-int chooseTile(int64_t M, int64_t N) {
+constexpr int kCUs = 256;   // of an MI355X
+constexpr int kForms = 9, kFirstFew = 6;
+struct FormCost {
+    int rows, cols;
+    int call, tile, perK;   // 10 ns: c, a and 1000 b of the time c + n (a + b K)
+};
+// With n the tiles of the busiest CU, the time of a launch is within 10 to 17% (one
+// standard deviation) of c + n (a + b K): the constants are fitted to 68 products of 1 to
+// 8192 rows, 74 to 16384 columns and K of 75 to 15814, of whole and odd sizes, each timed
+// in every form. The form that this makes the fastest was on average 0.9% slower than the
+// fastest one timed, 18% in the worst case (8192 x 8192 x 128). What the forms are for, us
+// 256x256 | 256x128 | 128x128 | its pair | 64x128 | 64x64 | few 16x16 | 32x16 | 32x32:
+//   4096 x 4096 x 4096   52.3 | 58.8 | 75.0 | 61.9 | 80.8 | 98.3 | - | - | -
+//   2319 x 1792 x 6784   64.1 | 33.8 | 49.1 | 37.8 | 45.6 | 48.8 | - | - | -
+//   2048 x 2048 x 2048   25.2 | 16.0 | 11.6 | 13.6 | 13.0 | 15.6 | 86 | 93 | 59
+//   3873 x 4263 x 175    21.5 | 21.8 | 23.6 | 17.2 | 21.5 | 29.6 | - | - | -
+//   149 x 8886 x 6784    64.0 | 30.7 | 23.9 | 32.2 | 18.0 | 20.5 | 54 | 54 | 38
+//   48 x 8192 x 4096     39.9 | 20.1 | 15.7 | 20.6 | 12.0 | 8.3 | 13.3 | 15.9 | 11.2
+//   1 x 4096 x 4096      39.7 | 19.9 | 15.6 | 20.1 | 11.3 | 7.5 | 5.0 | 5.2 | 5.6
+//   300 x 300 x 8192     75.1 | 38.2 | 27.3 | 38.0 | 19.6 | 12.9 | 8.7 | 7.1 | 8.5
+//   792 x 256 x 3468     45.7 | 28.3 | 18.8 | 23.3 | 15.0 | 11.1 | 9.6 | 9.6 | 7.9
+constexpr FormCost kForm[kForms] = {
+    {256, 256, 0, 750, 856},  {256, 128, 0, 680, 455}, {128, 128, 50, 400, 327},
+    {128, 128, 190, 220, 372}, {64, 128, 200, 150, 223}, {64, 64, 210, 120, 136},
+    {16, 16, 170, 70, 31},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
+};
+
+int64_t tilesOf(int form, int64_t M, int64_t N) {
+    const FormCost& f = kForm[form];
+    return ((M + f.rows - 1) / f.rows) * ((N + f.cols - 1) / f.cols);
+}
+
+int chooseForm(const Int8Sizes& z, bool packed) {
     int best = 0;
     int64_t least = INT64_MAX;
-    for (int t = 0; t < kTiles; ++t) {
-        const int64_t tiles = ((M + kTileRows[t] - 1) / kTileRows[t]) * ((N + kTileCols[t] - 1) / kTileCols[t]);
-        const int64_t cost = (tiles + kCUs - 1) / kCUs * kTileCost[t];
-        if (cost < least) best = t, least = cost;
+    // Small tiles of all sizes take the arguments of small ones only.
+    for (int i = 0; i < (packed ? kForms : kFirstFew); ++i) {
+        const FormCost& f = kForm[i];
+        const int64_t n = (tilesOf(i, z.M, z.N) + kCUs - 1) / kCUs;
+        const int64_t cost = f.call + n * (f.tile + (int64_t)f.perK * z.K / 1000);
+        if (cost < least) best = i, least = cost;
     }
     return best;
 }
 
+template <typename T, typename Out, bool PINGPONG, bool PACKED>
+hipError_t launchTiles(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
+    ridge::int8GemmKernel<T, Out, PINGPONG, PACKED>
+        <<<dim3((unsigned)tiles), dim3(T::kThreads), 0, stream>>>(ridge::int8Args<PACKED>(p, z));
+    return hipGetLastError();
+}
+
+template <typename T, typename Out>
+hipError_t launchFew(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
+    ridge::int8FewKernel<T, Out><<<dim3((unsigned)tiles), dim3(T::kThreads), 0, stream>>>(ridge::int8Args<true>(p, z));
+    return hipGetLastError();
+}
+
+template <typename Out, bool PACKED>
+hipError_t launchForm(int form, const Int8Operands& p, const Int8Sizes& z, hipStream_t s) {
+    const int64_t tiles = tilesOf(form, z.M, z.N);
+    // A grid's work-items fit 32 bits, and its tiles the kernels' divisions.
+    if (tiles >= (1 << 23)) return hipErrorInvalidValue;
+    switch (form) {
+        case 0: return launchTiles<Tile256x256, Out, false, PACKED>(p, z, tiles, s);
+        case 1: return launchTiles<Tile256x128, Out, true, PACKED>(p, z, tiles, s);
+        case 2: return launchTiles<Tile128x128, Out, false, PACKED>(p, z, tiles, s);
+        case 3: return launchTiles<Pair128x128, Out, false, PACKED>(p, z, tiles, s);
+        case 4: return launchTiles<Tile64x128, Out, false, PACKED>(p, z, tiles, s);
+        case 5: return launchTiles<Tile64x64, Out, false, PACKED>(p, z, tiles, s);
+    }
+    if constexpr (PACKED) {
+        switch (form) {
+            case 6: return launchFew<Few16x16, Out>(p, z, tiles, s);
+            case 7: return launchFew<Few32x16, Out>(p, z, tiles, s);
+            case 8: return launchFew<Few32x32, Out>(p, z, tiles, s);
+        }
+    }
+    return hipErrorInvalidValue;
+}
+
 template <typename Out>
-hipError_t launchGemm(const Int8Args& args, hipStream_t stream) {
-    // Few tokens and no more channels than one workgroup of 16 a CU takes: a 64 x 64 tile
-    // would leave three CUs in four idle. us, few | 64 x 64 tiles, K = 4096: 1 x 4096 4.9 |
-    // 7.4, 20 x 4096 5.7 | 7.6, 64 x 4096 8.3 | 8.2; 64 x 2000 x 8000 11.5 | 16.8; 1 x 1000
-    // x 16384 7.1 | 20.5. With twice the channels the tiles are as fast: 16 x 8192 8.2 | 7.8.
-    static_assert(ridge::kFewMostN == 16 * kCUs, "a workgroup of 16 channels on each CU");
-    if (args.N <= ridge::kFewMostN && args.ldc <= UINT32_MAX) {
-        if (args.M <= 16) return launchFew<ridge::Int8FewTraits<1, 1, 16, 2>, Out>(args, stream);
-        if (args.M <= 32) return launchFew<ridge::Int8FewTraits<2, 1, 8, 2>, Out>(args, stream);
-        if (args.M <= ridge::kFewMostM) return launchFew<ridge::Int8FewTraits<4, 1, 8, 2>, Out>(args, stream);
-    }
-    switch (chooseTile(args.M, args.N)) {
-        case 0: return launchTiles<Tile256x256, Out, false>(args, stream);
-        case 1: return launchTiles<Tile256x128, Out, true>(args, stream);
-        case 2: return launchTiles<Tile128x128, Out, false>(args, stream);
-        case 3: return launchTiles<Tile64x128, Out, false>(args, stream);
-        default: return launchTiles<Tile64x64, Out, false>(args, stream);
-    }
+hipError_t launchGemm(const Int8Operands& p, const Int8Sizes& z, hipStream_t stream) {
+    const bool packed = ridge::int8ArgsFit(z);
+    const int form = chooseForm(z, packed);
+    return packed ? launchForm<Out, true>(form, p, z, stream) : launchForm<Out, false>(form, p, z, stream);
 }
 
 bool aligned(const void* p, size_t to) { return p != nullptr && ((uintptr_t)p & (to - 1)) == 0; }
 
 }  // namespace
+
+extern "C" int64_t ridge_int8_row_stride(int64_t cols) {
+    const int64_t to = cols > 512 ? 128 : 16;
+    return (cols + to - 1) / to * to;
+}
 
 extern "C" int ridge_int8_gemm(const int8_t* A, int64_t lda, const float* scaleA, const int8_t* B, int64_t ldb,
                                const float* scaleB, const void* bias, void* C, int64_t ldc, int type, int64_t M,
@@ -93,11 +131,11 @@ extern "C" int ridge_int8_gemm(const int8_t* A, int64_t lda, const float* scaleA
         ldb >= (1 << 23) || ldc < N || !aligned(A, 16) || !aligned(B, 16) || !aligned(scaleA, 4) ||
         !aligned(scaleB, 4) || !aligned(C, size) || ((uintptr_t)bias & (size - 1)))
         return hipErrorInvalidValue;
-    const Int8Args args = {A,        B,        scaleA, scaleB, bias,   C, (int)lda, (int)ldb, ldc, (int)M,
-                           (int)N, (int)K, {}};
+    const Int8Operands p = {A, B, scaleA, scaleB, bias, C};
+    const Int8Sizes z = {(int)M, (int)N, (int)K, (int)lda, (int)ldb, ldc};
     switch (type) {
-        case RIDGE_F16: return launchGemm<_Float16>(args, (hipStream_t)stream);
-        case RIDGE_BF16: return launchGemm<__bf16>(args, (hipStream_t)stream);
-        default: return launchGemm<float>(args, (hipStream_t)stream);
+        case RIDGE_F16: return launchGemm<_Float16>(p, z, (hipStream_t)stream);
+        case RIDGE_BF16: return launchGemm<__bf16>(p, z, (hipStream_t)stream);
+        default: return launchGemm<float>(p, z, (hipStream_t)stream);
     }
 }

@@ -25,18 +25,58 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kInt8MfmaK = 64;   // k of one instruction
 
-struct Int8Args {
+// A launch's arguments. They are written to device memory before it, 64 bytes at a time:
+// a second write would cost 0.8 us of the host's time, which is what the shortest products
+// wait for. So where sizes allow (int8ArgsFit) they are packed into one: strides, multiples
+// of 16 below 2^23, in 19 bits each, K in 17, M and N in 16, ldc in 32.
+struct Int8Operands {
     const int8_t* A;
     const int8_t* B;
     const float* scaleA;
     const float* scaleB;
     const void* bias;
     void* C;
-    int lda, ldb;
-    int64_t ldc;
-    int M, N, K;
-    TileOrder order;   // of ceil(M / BM) x ceil(N / BN) tiles
 };
+
+struct Int8Sizes {
+    int M, N, K, lda, ldb;
+    int64_t ldc;
+};
+
+template <bool PACKED>
+struct Int8Args;
+template <>
+struct Int8Args<true> {
+    Int8Operands p;
+    uint64_t stridesAndK, rest;
+    __host__ __device__ __forceinline__ Int8Sizes sizes() const {
+        return {(int)(rest & 0xffff),
+                (int)(rest >> 16 & 0xffff),
+                (int)(stridesAndK >> 38),
+                (int)(stridesAndK & 0x7ffff) * 16,
+                (int)(stridesAndK >> 19 & 0x7ffff) * 16,
+                (int64_t)(rest >> 32)};
+    }
+};
+template <>
+struct Int8Args<false> {
+    Int8Operands p;
+    Int8Sizes s;
+    __host__ __device__ __forceinline__ Int8Sizes sizes() const { return s; }
+};
+static_assert(sizeof(Int8Args<true>) <= 64, "arguments of one write");
+
+inline bool int8ArgsFit(const Int8Sizes& s) { return s.M <= 0xffff && s.N <= 0xffff && s.ldc <= 0xffffffffll; }
+
+template <bool PACKED>
+inline Int8Args<PACKED> int8Args(const Int8Operands& p, const Int8Sizes& s) {
+    if constexpr (PACKED) {
+        return {p, (uint64_t)(s.lda / 16) | (uint64_t)(s.ldb / 16) << 19 | (uint64_t)s.K << 38,
+                (uint64_t)s.M | (uint64_t)s.N << 16 | (uint64_t)s.ldc << 32};
+    } else {
+        return {p, s};
+    }
+}
 
 // Where chunk q = row * CPR + c of a tile lies in LDS (an involution). LDS serves a
 // fragment's read 16 lanes at a time, lanes {0-3, 12-15, 20-27} and {4-11, 16-19, 28-31}
@@ -109,11 +149,13 @@ __device__ __forceinline__ float scaledSum(int sum, float a, float b, float bias
     return fmaf((float)sum * a, b, bias);
 }
 
+// One tile of C: its loads, fragments, products and epilogue.
 template <typename T, typename Out>
 struct Int8Block {
     static constexpr int TM = T::TM, TN = T::TN, KS = T::KS, CPR = T::CPR;
 
-    const Int8Args& args;
+    const Int8Operands p;
+    const Int8Sizes z;
     const char* lds;
     uint32_t ldsBase;
     int lane, wave, waveM, waveN;
@@ -126,7 +168,9 @@ struct Int8Block {
     int4_t acc[TM][TN];
     int numK, numFull;             // K tiles, and those that K fills
 
-    __device__ __forceinline__ Int8Block(const char* ldsArray, const Int8Args& a, int row, int col) : args(a) {
+    __device__ __forceinline__ Int8Block(const char* ldsArray, const Int8Operands& operands, const Int8Sizes& a,
+                                            int row, int col)
+        : p(operands), z(a) {
         lds = ldsArray;
         ldsBase = ldsAddress(ldsArray);
         lane = threadIdx.x % kWaveSize;
@@ -135,8 +179,8 @@ struct Int8Block {
         waveN = wave % T::kWavesN;
         blockRow = row;
         blockCol = col;
-        gA = (const char*)a.A + (int64_t)row * a.lda;
-        gB = (const char*)a.B + (int64_t)col * a.ldb;
+        gA = (const char*)p.A + (int64_t)row * a.lda;
+        gB = (const char*)p.B + (int64_t)col * a.ldb;
         numFull = a.K / T::BK;
         numK = numFull + (a.K % T::BK != 0);
 #pragma unroll
@@ -145,8 +189,9 @@ struct Int8Block {
         for (int i = 0; i < T::kPerWaveB; ++i) offB[i] = offset(chunkOf(i), a.ldb, a.N - 1 - col);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            rdA[ks] = swizzleRows<CPR>((waveM * T::WM + lane % 16) * CPR + 4 * ks + lane / 16) * 16;
-            rdB[ks] = T::kRegionA + swizzleRows<CPR>((waveN * T::WN + lane % 16) * CPR + 4 * ks + lane / 16) * 16;
+            const int c = 4 * ks + lane / 16;
+            rdA[ks] = swizzleRows<CPR>((waveM * T::WM + lane % 16) * CPR + c) * 16;
+            rdB[ks] = T::kRegionA + swizzleRows<CPR>((waveN * T::WN + lane % 16) * CPR + c) * 16;
         }
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm)
@@ -161,9 +206,9 @@ struct Int8Block {
         const uint32_t to = ldsBase + T::kRing + wave * 256;
         const int at = wave * 64 + lane;
         if (wave < T::BM / 64) {
-            globalLoadLds4(args.scaleA + blockRow, 4u * (uint32_t)min(at, args.M - 1 - blockRow), to);
+            globalLoadLds4(p.scaleA + blockRow, 4u * (uint32_t)min(at, z.M - 1 - blockRow), to);
         } else if (wave < (T::BM + T::BN) / 64) {
-            globalLoadLds4(args.scaleB + blockCol, 4u * (uint32_t)min(at - T::BM, args.N - 1 - blockCol), to);
+            globalLoadLds4(p.scaleB + blockCol, 4u * (uint32_t)min(at - T::BM, z.N - 1 - blockCol), to);
         }
     }
 
@@ -172,22 +217,26 @@ struct Int8Block {
         return swizzleRows<CPR>((i * T::kWaves + wave) * 64 + lane);
     }
 
-    // Strides are below 2^23 and tiles have at most 256 rows, so offsets fit 32 bits.
+    // Byte offset of a load's chunk from the tile's first row. Strides are below 2^23 and
+    // tiles have at most 256 rows: offsets fit 32 bits.
     static __device__ __forceinline__ uint32_t offset(int chunk, int ld, int lastRow) {
         return (uint32_t)min(chunk / CPR, lastRow) * (uint32_t)ld + (uint32_t)(chunk % CPR) * 16u;
     }
 
-    // Refills LDS stage `stage` with K tile kTile (this wave's share). `whole`: the tile
-    // is known to be one that K fills.
+    // Refills LDS stage `stage` with K tile kTile (this wave's share). WHOLE: K is known to
+    // fill it; else a chunk behind K's last one is replaced by that.
     template <bool WHOLE>
     __device__ __forceinline__ void issueTile(int kTile, int stage) const {
         const char* srcA = gA + (int64_t)kTile * T::BK;
         const char* srcB = gB + (int64_t)kTile * T::BK;
         const uint32_t dstA = ldsBase + stage * T::kBytesA;
         const uint32_t dstB = ldsBase + T::kRegionA + stage * T::kBytesB;
-        // How far behind the last chunk of K each lane's chunk is.
-        const int last = WHOLE || kTile < numFull ? CPR - 1 : (args.K - 1) / 16 - kTile * CPR;
-        auto past = [&](int i) { return WHOLE ? 0u : (uint32_t)max(chunkOf(i) % CPR - last, 0) * 16u; };
+        const int last = WHOLE || kTile < numFull ? CPR - 1 : (z.K - 1) / 16 - kTile * CPR;
+        auto past = [&](int i) {
+            if constexpr (WHOLE) return 0u;
+            const int chunk = swizzleRows<CPR>((i * T::kWaves + wave) * 64 + laneAgain()) % CPR;
+            return (uint32_t)max(chunk - last, 0) * 16u;
+        };
 #pragma unroll
         for (int i = 0; i < T::kPerWaveA; ++i)
             globalLoadLds16(srcA, offA[i] - past(i), dstA + (i * T::kWaves + wave) * 1024);
@@ -209,7 +258,7 @@ struct Int8Block {
 
     // Clears what A's fragments of K tile kTile hold behind K.
     __device__ __forceinline__ void clearBehind(int kTile, int ks, int4_t (&a)[TM]) const {
-        const int4_t mask = firstBytes(args.K - (kTile * T::BK + ks * kInt8MfmaK + 16 * (lane / 16)));
+        const int4_t mask = firstBytes(z.K - (kTile * T::BK + ks * kInt8MfmaK + 16 * (laneAgain() / 16)));
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) a[tm] &= mask;
     }
@@ -253,12 +302,12 @@ struct Int8Block {
             sb[tn] = *(const RIDGE_LDS_AS float4_t*)(scales + T::BM + waveN * T::WN + tn * 16 + 4 * g);
             add[tn] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        if (args.bias != nullptr) {
-            const Out* bias = (const Out*)args.bias;
+        if (p.bias != nullptr) {
+            const Out* bias = (const Out*)p.bias;
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) add[tn][e] = (float)bias[min(col0 + tn * 16 + 4 * g + e, args.N - 1)];
+                for (int e = 0; e < 4; ++e) add[tn][e] = (float)bias[min(col0 + tn * 16 + 4 * g + e, z.N - 1)];
         }
         Quad quads[TN];
         auto compute = [&](int tm) {
@@ -291,14 +340,14 @@ struct Int8Block {
             for (int j = 0; j < kReads; ++j) {
                 const int q = j * 64 + lane;
                 const int row = row0 + 16 * tm + q / kChunks, col = col0 + q % kChunks * kPer;
-                if (row < args.M && col < args.N) {
-                    Out* dst = (Out*)args.C + (int64_t)row * args.ldc + col;
-                    if (col + kPer <= args.N) {
+                if (row < z.M && col < z.N) {
+                    Out* dst = (Out*)p.C + (int64_t)row * z.ldc + col;
+                    if (col + kPer <= z.N) {
                         *(Placed*)dst = v[j];
                     } else {
 #pragma unroll
                         for (int e = 0; e < kPer; ++e)
-                            if (col + e < args.N) dst[e] = v[j][e];
+                            if (col + e < z.N) dst[e] = v[j][e];
                     }
                 }
             }
@@ -471,15 +520,40 @@ __host__ __device__ inline int int8TilesN(int N) {
     return (N + T::BN - 1) / T::BN;
 }
 
-template <typename T, typename Out, bool PINGPONG>
+// n / d for n below 2^24, by f32's reciprocal and a correction: a uniform value.
+__device__ __forceinline__ DivMod divideSmall(uint32_t n, uint32_t d) {
+    uint32_t q = (uint32_t)__builtin_amdgcn_readfirstlane((int)((float)n * __builtin_amdgcn_rcpf((float)d)));
+    int r = (int)(n - q * d);
+    if (r < 0) {
+        --q;
+        r += (int)d;
+    } else if (r >= (int)d) {
+        ++q;
+        r -= (int)d;
+    }
+    return {q, (uint32_t)r};
+}
+
+// tileOf's order (groups of kInt8GroupM tile rows, column by column) without its
+// arguments: fewer than 2^23 tiles, which the launch sees to.
+template <typename T>
+__device__ __forceinline__ void int8TileOf(int id, int tilesM, int tilesN, int& row, int& col) {
+    const DivMod group = divideSmall((uint32_t)id, (uint32_t)(kInt8GroupM * tilesN));
+    const int first = (int)group.quot * kInt8GroupM;
+    const DivMod in = divideSmall(group.rem, (uint32_t)min(tilesM - first, kInt8GroupM));
+    row = (first + (int)in.rem) * T::BM;
+    col = (int)in.quot * T::BN;
+}
+
+template <typename T, typename Out, bool PINGPONG, bool PACKED>
 __global__ __launch_bounds__(T::kThreads)
-void int8GemmKernel(Int8Args args) {
+void int8GemmKernel(Int8Args<PACKED> args) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLdsBytes];
-    const int tilesM = int8TilesM<T>(args.M), tilesN = int8TilesN<T>(args.N);
+    const Int8Sizes z = args.sizes();
+    const int tilesM = int8TilesM<T>(z.M), tilesN = int8TilesN<T>(z.N);
     int row, col;
-    tileOf<T::BM, T::BN, kInt8GroupM>(xcdRemap(blockIdx.x, tilesM * tilesN), tilesM * T::BM, tilesN * T::BN,
-                                      args.order, row, col);
-    Int8Block<T, Out> blk(lds, args, row, col);
+    int8TileOf<T>(xcdRemap(blockIdx.x, tilesM * tilesN), tilesM, tilesN, row, col);
+    Int8Block<T, Out> blk(lds, args.p, z, row, col);
     if constexpr (PINGPONG) {
         int8PingPongLoop<T>(blk);
     } else {
@@ -489,38 +563,15 @@ void int8GemmKernel(Int8Args args) {
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens: up to 16 TM rows of A, where B's bytes are all there is to move.
+// Few tokens, or few tiles: 16 TM x 16 TN of C a workgroup, whose WAVES wavefronts share K.
 //
-// A workgroup owns 16 TN channels and all tokens, and its WAVES wavefronts share K: wave
-// w takes the 128-byte pieces w, w + WAVES, ... of every row, so that the workgroup reads
-// its rows front to back. A wave streams its pieces through a ring of its own in LDS
+// Wave w takes the 128-byte pieces w, w + WAVES, ... of every row, so that the workgroup
+// reads its rows front to back. A wave streams its pieces through a ring of its own in LDS
 // (eight lanes load a row's 128 bytes, one fragment read takes 16 rows: straight to
 // registers the 16 lanes of a load would be 16 rows apart) and waits for nothing but its
 // own loads: there is no barrier before the end, where the sums meet. They are 32-bit
 // integers, whose order does not matter.
 // ---------------------------------------------------------------------------
-// In 64 bytes: arguments are written to device memory before a launch, and a second line
-// of them would cost 0.8 us of the host's time. Strides are multiples of 16 below 2^23.
-constexpr int kFewMostM = 64, kFewMostN = 4096;
-struct Int8FewArgs {
-    const int8_t* A;
-    const int8_t* B;
-    const float* scaleA;
-    const float* scaleB;
-    const void* bias;
-    void* C;
-    uint32_t strideAndM;   // lda / 16 in 19 bits, M
-    uint32_t strideAndN;   // ldb / 16 in 19 bits, N
-    int K;
-    uint32_t ldc;
-};
-static_assert(sizeof(Int8FewArgs) <= 64 && kFewMostM < (1 << 13) && kFewMostN < (1 << 13), "arguments of one write");
-
-inline Int8FewArgs fewArgs(const Int8Args& a) {
-    return {a.A, a.B, a.scaleA, a.scaleB, a.bias, a.C, (uint32_t)a.lda / 16 | (uint32_t)a.M << 19,
-            (uint32_t)a.ldb / 16 | (uint32_t)a.N << 19, a.K, (uint32_t)a.ldc};
-}
-
 template <int TM_, int TN_, int WAVES_, int STAGES_>
 struct Int8FewTraits {
     static constexpr int TM = TM_, TN = TN_, kWaves = WAVES_, kStages = STAGES_;
@@ -540,35 +591,39 @@ struct Int8FewTraits {
 
 template <typename T, typename Out>
 __global__ __launch_bounds__(T::kThreads)
-void int8FewKernel(Int8FewArgs args) {
-    const int M = (int)(args.strideAndM >> 19), N = (int)(args.strideAndN >> 19);
-    const uint32_t lda = (args.strideAndM & 0x7ffff) * 16, ldb = (args.strideAndN & 0x7ffff) * 16;
+void int8FewKernel(Int8Args<true> args) {
+    const Int8Operands p = args.p;
+    const Int8Sizes z = args.sizes();
     constexpr int TM = T::TM, TN = T::TN, KS = T::KS, CPR = T::CPR, STAGES = T::kStages, L = T::kLoads;
     __shared__ __attribute__((aligned(1024))) char lds[T::kLdsBytes];
     const int lane = threadIdx.x % kWaveSize;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-    const int col0 = blockIdx.x * 16 * TN;
+    // Workgroups of the same channels are neighbours on one XCD: they read the same rows of B.
+    const int rowBlocks = (z.M + 16 * TM - 1) / (16 * TM), colBlocks = (z.N + 16 * TN - 1) / (16 * TN);
+    const DivMod block = divideSmall((uint32_t)xcdRemap(blockIdx.x, rowBlocks * colBlocks), (uint32_t)rowBlocks);
+    const int row0 = (int)block.rem * 16 * TM, col0 = (int)block.quot * 16 * TN;
     const int r16 = lane % 16, g = lane / 16;
 
     // A piece in LDS: 16 TN rows of B, then 16 TM rows of A. Load i fills eight of them.
-    const char* gB = (const char*)args.B + (int64_t)col0 * ldb;
+    const char* gA = (const char*)p.A + (int64_t)row0 * z.lda;
+    const char* gB = (const char*)p.B + (int64_t)col0 * z.ldb;
     uint32_t off[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
         const int q = swizzleRows<CPR>(64 * i + lane), row = q / CPR;
-        off[i] = (uint32_t)(q % CPR) * 16u + (i < 2 * TN ? (uint32_t)min(row, N - 1 - col0) * ldb
-                                                         : (uint32_t)min(row - 16 * TN, M - 1) * lda);
+        off[i] = (uint32_t)(q % CPR) * 16u + (i < 2 * TN ? (uint32_t)min(row, z.N - 1 - col0) * (uint32_t)z.ldb
+                                                         : (uint32_t)min(row - 16 * TN, z.M - 1 - row0) * (uint32_t)z.lda);
     }
     const uint32_t ring = ldsAddress(lds) + wave * T::kWaveBytes;
-    const int pieces = (args.K + T::kPiece - 1) / T::kPiece;
+    const int pieces = (z.K + T::kPiece - 1) / T::kPiece;
     auto issue = [&](int piece, int stage) {
         const int64_t at = (int64_t)piece * T::kPiece;
         // How far behind the last chunk of K this lane's chunk is.
-        const int last = min((args.K - 1) / 16 - piece * CPR, CPR - 1);
+        const int last = min((z.K - 1) / 16 - piece * CPR, CPR - 1);
         auto past = [&](int i) { return (uint32_t)max(swizzleRows<CPR>(64 * i + lane) % CPR - last, 0) * 16u; };
 #pragma unroll
         for (int i = 0; i < L; ++i)
-            globalLoadLds16((i < 2 * TN ? gB : (const char*)args.A) + at, off[i] - past(i),
+            globalLoadLds16((i < 2 * TN ? gB : gA) + at, off[i] - past(i),
                             ring + stage * T::kPieceBytes + i * 1024);
     };
     int4_t acc[TM][TN];
@@ -606,10 +661,10 @@ void int8FewKernel(Int8FewArgs args) {
                 // The stage has been read before it is filled again.
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 if (i + STAGES < mine) issue(piece + STAGES * T::kWaves, s);
-                if (piece * T::kPiece + T::kPiece > args.K) {
+                if (piece * T::kPiece + T::kPiece > z.K) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
-                        const int4_t mask = firstBytes(args.K - (piece * T::kPiece + ks * kInt8MfmaK + 16 * g));
+                        const int4_t mask = firstBytes(z.K - (piece * T::kPiece + ks * kInt8MfmaK + 16 * g));
 #pragma unroll
                         for (int tm = 0; tm < TM; ++tm) a[ks][tm] &= mask;
                     }
@@ -639,15 +694,15 @@ void int8FewKernel(Int8FewArgs args) {
 #pragma unroll
         for (int w = 0; w < T::kWaves; ++w)
             total += *(const int4_t*)(lds + w * T::kWaveBytes + (t * kWaveSize + lane) * 16);
-        const int row = 16 * (t / TN) + r16, col = col0 + 16 * (t % TN) + 4 * g;
-        if (row < M) {
-            const float sa = args.scaleA[row];
-            Out* dst = (Out*)args.C + (int64_t)row * args.ldc + col;
+        const int row = row0 + 16 * (t / TN) + r16, col = col0 + 16 * (t % TN) + 4 * g;
+        if (row < z.M) {
+            const float sa = p.scaleA[row];
+            Out* dst = (Out*)p.C + (int64_t)row * z.ldc + col;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (col + e < N) {
-                    const float add = args.bias ? (float)((const Out*)args.bias)[col + e] : 0.0f;
-                    dst[e] = (Out)scaledSum(total[e], sa, args.scaleB[col + e], add);
+                if (col + e < z.N) {
+                    const float add = p.bias ? (float)((const Out*)p.bias)[col + e] : 0.0f;
+                    dst[e] = (Out)scaledSum(total[e], sa, p.scaleB[col + e], add);
                 }
             }
         }

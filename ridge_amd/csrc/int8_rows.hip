@@ -91,8 +91,8 @@ struct RowArgs {
     __device__ int64_t ldq() const { return strideQ; }
 };
 
-// The norm's, with all its matrices contiguous (the common case, which fits) or with
-// strides.
+// The norm's, with its 16- and 32-bit matrices contiguous (the common case, which fits) or
+// with strides of their own.
 template <bool DENSE>
 struct NormArgs;
 template <>
@@ -105,7 +105,8 @@ struct NormArgs<true> {
     void* residualOut;
     int rows, cols;
     float eps;
-    __device__ int64_t ldq() const { return ((int64_t)cols + 15) / 16 * 16; }
+    uint32_t strideQ16;   // in 16 bytes
+    __device__ int64_t ldq() const { return (int64_t)strideQ16 * 16; }
     __device__ int64_t ldxOf() const { return cols; }
     __device__ int64_t ldResidualOf() const { return cols; }
     __device__ int64_t ldResidualOutOf() const { return cols; }
@@ -384,8 +385,9 @@ hipError_t launchTyped(const RowArgs& a, int type, bool stream, hipStream_t s) {
 template <typename T, typename W>
 hipError_t launchNorm(const NormArgs<false>& a, bool stream, hipStream_t s) {
     if (stream) return launchByLength<Normed<T, W, true, false>>(a, s);
-    const NormArgs<true> d = {a.x, a.q, a.scale, a.residual, a.weight, a.residualOut, a.rows, a.cols, a.eps};
-    const bool dense = a.rows == 1 || (a.ldx == a.cols && a.strideQ == ((int64_t)a.cols + 15) / 16 * 16 &&
+    const NormArgs<true> d = {a.x, a.q, a.scale, a.residual, a.weight, a.residualOut, a.rows, a.cols, a.eps,
+                              (uint32_t)(a.strideQ / 16)};
+    const bool dense = a.rows == 1 || (a.ldx == a.cols && a.strideQ / 16 <= UINT32_MAX &&
                                        (!a.residual || (a.ldResidual == a.cols && a.ldResidualOut == a.cols)));
     return dense ? launchByLength<Normed<T, W, false, true>>(d, s) : launchByLength<Normed<T, W, false, false>>(a, s);
 }

@@ -66,6 +66,7 @@ def lib():
             ("gemm", [p, n, p, p, n, p, p, p, n, i, n, n, n, p])):
         function = getattr(L, "ridge_int8_" + name)
         function.restype, function.argtypes = i, args
+    L.ridge_int8_row_stride.restype, L.ridge_int8_row_stride.argtypes = n, [n]
     _lib = L
     return L
 
@@ -85,11 +86,12 @@ def _load():
 
 
 def empty(rows, cols, device=None):
-    """(q, scale): uninitialised 8-bit rows and their scales. The rows lie a multiple of
-    16 bytes apart; what is behind `cols` is never looked at."""
+    """(q, scale): uninitialised 8-bit rows and their scales, the rows a multiple of 16
+    bytes apart, and of 128 where they are long, which the product reads fastest
+    (ridge_int8_row_stride). What is behind `cols` is never looked at."""
     import torch
     device = "cuda" if device is None else device
-    q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=device)
+    q = torch.empty((rows, lib().ridge_int8_row_stride(cols)), dtype=torch.int8, device=device)
     return q[:, :cols], torch.empty(rows, dtype=torch.float32, device=device)
 
 
