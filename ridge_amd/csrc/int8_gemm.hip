@@ -67,9 +67,22 @@ int chooseForm(const Int8Sizes& z, bool packed) {
     return best;
 }
 
-template <typename T, typename Out, bool PINGPONG, bool PACKED>
+// A C of more than this whose rows are whole cache lines is stored past the caches: it would
+// push the operands out of them. us, cached | past the caches, forms 0, 1 and 3: 8192 x
+// 8192 x 128 51.3 | 45.3, 52.2 | 42.0, 47.1 | 39.3; x 1024 91.1 | 84.0, 115.9 | 88.5, 111.0 |
+// 88.6; x 8192 424 | 420. Lines that two tiles share lose by it (8192 x 8191 x 512 66.8 |
+// 78.8), and so does a smaller C (4096 x 8192 x 1024 40.7 | 44.2).
+constexpr int64_t kStreamBytes = (int64_t)64 << 20;
+
+template <typename Out>
+bool streams(const Int8Operands& p, const Int8Sizes& z) {
+    return (int64_t)z.M * z.N * (int64_t)sizeof(Out) > kStreamBytes && z.ldc * (int64_t)sizeof(Out) % 128 == 0 &&
+           (uintptr_t)p.C % 128 == 0;
+}
+
+template <typename T, typename Out, bool PINGPONG, bool PACKED, bool STREAM = false>
 hipError_t launchTiles(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
-    ridge::int8GemmKernel<T, Out, PINGPONG, PACKED>
+    ridge::int8GemmKernel<T, Out, PINGPONG, PACKED, STREAM>
         <<<dim3((unsigned)tiles), dim3(T::kThreads), 0, stream>>>(ridge::int8Args<PACKED>(p, z));
     return hipGetLastError();
 }
@@ -85,6 +98,13 @@ hipError_t launchForm(int form, const Int8Operands& p, const Int8Sizes& z, hipSt
     const int64_t tiles = tilesOf(form, z.M, z.N);
     // A grid's work-items fit 32 bits, and its tiles the kernels' divisions.
     if (tiles >= (1 << 23)) return hipErrorInvalidValue;
+    if (streams<Out>(p, z)) {   // no other form has a grid of that size
+        switch (form) {
+            case 0: return launchTiles<Tile256x256, Out, false, PACKED, true>(p, z, tiles, s);
+            case 1: return launchTiles<Tile256x128, Out, true, PACKED, true>(p, z, tiles, s);
+            case 3: return launchTiles<Pair128x128, Out, false, PACKED, true>(p, z, tiles, s);
+        }
+    }
     switch (form) {
         case 0: return launchTiles<Tile256x256, Out, false, PACKED>(p, z, tiles, s);
         case 1: return launchTiles<Tile256x128, Out, true, PACKED>(p, z, tiles, s);

@@ -289,6 +289,8 @@ struct Int8Block {
     typedef Out Chunk __attribute__((ext_vector_type(kPer)));
     typedef Out Placed __attribute__((ext_vector_type(kPer), aligned(sizeof(Out))));
 
+    // STREAM: past the caches.
+    template <bool STREAM>
     __device__ __forceinline__ void store() const {
         RIDGE_LDS_AS char* region = (RIDGE_LDS_AS char*)(const_cast<char*>(lds)) + wave * kRegionBytes;
         const RIDGE_LDS_AS float* scales = (const RIDGE_LDS_AS float*)((const RIDGE_LDS_AS char*)(lds) + T::kRing);
@@ -343,7 +345,11 @@ struct Int8Block {
                 if (row < z.M && col < z.N) {
                     Out* dst = (Out*)p.C + (int64_t)row * z.ldc + col;
                     if (col + kPer <= z.N) {
-                        *(Placed*)dst = v[j];
+                        if constexpr (STREAM) {
+                            __builtin_nontemporal_store(*(const Placed*)&v[j], (Placed*)dst);
+                        } else {
+                            *(Placed*)dst = v[j];
+                        }
                     } else {
 #pragma unroll
                         for (int e = 0; e < kPer; ++e)
@@ -545,7 +551,7 @@ __device__ __forceinline__ void int8TileOf(int id, int tilesM, int tilesN, int& 
     col = (int)in.quot * T::BN;
 }
 
-template <typename T, typename Out, bool PINGPONG, bool PACKED>
+template <typename T, typename Out, bool PINGPONG, bool PACKED, bool STREAM>
 __global__ __launch_bounds__(T::kThreads)
 void int8GemmKernel(Int8Args<PACKED> args) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLdsBytes];
@@ -559,7 +565,7 @@ void int8GemmKernel(Int8Args<PACKED> args) {
     } else {
         int8UniformLoop<T>(blk);
     }
-    blk.store();
+    blk.template store<STREAM>();
 }
 
 // ---------------------------------------------------------------------------
