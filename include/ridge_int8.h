@@ -73,6 +73,12 @@ int ridge_int8_gemm(const int8_t* A, int64_t lda, const float* scaleA, const int
                     const float* scaleB, const void* bias, void* C, int64_t ldc, int type, int64_t M, int64_t N,
                     int64_t K, void* stream);
 
+/* Which of its forms a product of contiguous rows runs in: 0 .. 5 tiles of 256x256,
+ * 256x128, 128x128, 128x128 (two on a CU), 64x128 and 64x64; 6 .. 8 tiles of 16x16, 32x16
+ * and 32x32 whose K a workgroup's waves share. -1 for sizes that ridge_int8_gemm refuses or
+ * that hold no element. No device is touched. */
+int ridge_int8_gemm_form(int64_t M, int64_t N, int64_t K);
+
 #ifdef __cplusplus
 }
 #endif

@@ -130,6 +130,8 @@ hipError_t launchGemm(const Int8Operands& p, const Int8Sizes& z, hipStream_t str
     return packed ? launchForm<Out, true>(form, p, z, stream) : launchForm<Out, false>(form, p, z, stream);
 }
 
+constexpr int64_t kMostRows = INT32_MAX - 255;   // whole tiles of them still fit 31 bits
+
 bool aligned(const void* p, size_t to) { return p != nullptr && ((uintptr_t)p & (to - 1)) == 0; }
 
 }  // namespace
@@ -146,7 +148,6 @@ extern "C" int ridge_int8_gemm(const int8_t* A, int64_t lda, const float* scaleA
     if (M < 0 || N < 0 || K < 1 || K > RIDGE_INT8_MAX_K) return hipErrorInvalidValue;
     if (M == 0 || N == 0) return hipSuccess;
     const size_t size = type == RIDGE_F32 ? 4 : 2;
-    constexpr int64_t kMostRows = INT32_MAX - 255;   // whole tiles of them still fit 31 bits
     if (M > kMostRows || N > kMostRows || lda < K || ldb < K || lda % 16 || ldb % 16 || lda >= (1 << 23) ||
         ldb >= (1 << 23) || ldc < N || !aligned(A, 16) || !aligned(B, 16) || !aligned(scaleA, 4) ||
         !aligned(scaleB, 4) || !aligned(C, size) || ((uintptr_t)bias & (size - 1)))
@@ -158,4 +159,11 @@ extern "C" int ridge_int8_gemm(const int8_t* A, int64_t lda, const float* scaleA
         case RIDGE_BF16: return launchGemm<__bf16>(p, z, (hipStream_t)stream);
         default: return launchGemm<float>(p, z, (hipStream_t)stream);
     }
+}
+
+extern "C" int ridge_int8_gemm_form(int64_t M, int64_t N, int64_t K) {
+    if (M < 1 || N < 1 || K < 1 || M > kMostRows || N > kMostRows || K > RIDGE_INT8_MAX_K) return -1;
+    const int ld = (int)ridge_int8_row_stride(K);
+    const Int8Sizes z = {(int)M, (int)N, (int)K, ld, ld, N};
+    return chooseForm(z, ridge::int8ArgsFit(z));
 }

@@ -17,7 +17,7 @@ P = 1 << 20   # an address that is never followed
 
 def test_every_declared_symbol_is_exported():
     names = _declared(os.path.join(ROOT, "include", "ridge_int8.h"))
-    assert len(names) == 6
+    assert len(names) == 7
     L = ctypes.CDLL(I.LIB_PATH)
     assert [n for n in names if not hasattr(L, n)] == []
 
@@ -82,3 +82,30 @@ def test_host_tensors_are_refused():
                  lambda: I.dequantize(q, s), lambda: I.gemm(q, s, q, s)):
         with pytest.raises(I.RidgeInt8Error, match="device tensor"):
             call()
+
+
+# What the GPU tests run the forms with, and the products that each is for.
+FORMS = [(0, 4001, 4093, 2065), (1, 4001, 4103, 2065), (1, 2301, 1805, 2049), (2, 2031, 2031, 1031), (3, 3873, 4263, 175), (4, 149, 8887, 4111),
+         (5, 49, 8195, 1029), (6, 3, 4001, 1027), (7, 299, 301, 4099), (8, 791, 257, 3469)]
+
+
+@pytest.mark.parametrize("form,M,N,K", FORMS)
+def test_every_form_of_the_product_is_chosen_somewhere(form, M, N, K):
+    L = ctypes.CDLL(I.LIB_PATH)
+    L.ridge_int8_gemm_form.argtypes = [ctypes.c_int64] * 3
+    assert L.ridge_int8_gemm_form(M, N, K) == form
+
+
+def test_form_of_sizes_without_a_product():
+    L = ctypes.CDLL(I.LIB_PATH)
+    L.ridge_int8_gemm_form.argtypes = [ctypes.c_int64] * 3
+    for sizes in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, I.MAX_K + 1), (1 << 31, 1, 1), (1, -4, 1)):
+        assert L.ridge_int8_gemm_form(*sizes) == -1
+    # Sizes past 16 bits take no form of small tiles, whose arguments hold 16.
+    assert 0 <= L.ridge_int8_gemm_form(1, 70000, 64) < 6 and 0 <= L.ridge_int8_gemm_form(70000, 1, 131071) < 6
+
+
+@pytest.mark.parametrize("cols,stride", [(1, 16), (16, 16), (17, 32), (512, 512), (513, 640), (4096, 4096), (4097, 4224)])
+def test_row_stride(cols, stride):
+    assert I.lib().ridge_int8_row_stride(cols) == stride
+    assert I.empty(2, cols, device="cpu")[0].stride(0) == stride

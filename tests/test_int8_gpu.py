@@ -18,6 +18,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from ridge_amd import int8 as I  # noqa: E402
+from test_int8 import FORMS  # noqa: E402
 
 DEV = "cuda:0"
 U = 2.0 ** -24
@@ -420,3 +421,77 @@ def test_refusals():
         I.quantize(y)
     with torch.no_grad():
         assert torch.equal(I.quantize(y)[0], q)
+
+
+# ---------------------------------------------------------------------------
+# the operators together
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [1, 7, 65, 300])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_feed_forward_block(tokens, dtype):
+    from ridge_amd.int8_mlp import Int8Mlp, plain_block, random_block
+    hidden, inner = 1000, 2100
+    weights = random_block(hidden, inner, dtype, tokens)
+    mlp = Int8Mlp(*weights)
+    x, r = _randn(tokens, hidden, dtype, 1) * 0.5, _randn(tokens, hidden, dtype, 2)
+    y, s = mlp(x, r)
+    space = mlp.workspace(tokens, dtype)
+    y2, s2 = mlp(x, r, space)
+    assert y2 is space["y"] and s2 is space["residual"]
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+    want, sums = plain_block(x.double(), r.double(), *(w.double() for w in weights))
+    assert torch.equal(s, (x.float() + r.float()).to(dtype))
+    # Rounding to steps of max / 127 leaves an error of 0.29 steps. Normal rows of 1000 to
+    # 2100 reach 3.5 of their standard deviations: 0.8% for each of the four operands, but
+    # the norm's rows have channels nine times as wide (27 of a deviation of 2.4: 2.6%)
+    # and silu(gate) * up reaches about 15 of its deviations (3.4%). Together 4.6%, of
+    # which the gate's share counts about 1.4 times: under 7%.
+    assert float((y.double() - want).norm() / want.norm()) < 0.07
+
+
+def test_feed_forward_block_refuses_weights_of_another_shape():
+    from ridge_amd.int8_mlp import Int8Mlp, random_block
+    norm_weight, gate_up, down = random_block(64, 96, torch.float16, 1)
+    for w in ((norm_weight, gate_up[:-2], down), (norm_weight[:-1], gate_up, down), (norm_weight, gate_up, down.t())):
+        with pytest.raises(I.RidgeInt8Error):
+            Int8Mlp(*w)
+
+
+def test_feed_forward_command_in_a_graph():
+    from ridge_amd import int8_mlp
+    assert int8_mlp.main(["--hidden", "256", "--inner", "512", "--tokens", "1,33", "--steps", "5", "--graph"]) == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 70000, 33), (70000, 3, 33), (66000, 70, 200)])
+def test_products_whose_sizes_do_not_pack(M, N, K):
+    _product(M, N, K, torch.float16, True, seed=M)
+
+
+def test_product_past_the_caches():
+    # A C of more than 64 MiB whose rows are whole cache lines, and one a row too narrow.
+    for M, N in ((4200, 8192), (4200, 8190), (9000, 4096)):
+        a, sa = _int8(M, 200, 1)
+        b, sb = _int8(N, 200, 2)
+        _check_product(I.gemm(a, sa, b, sb), a, sa, b, sb)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form,M,N,K", FORMS)
+def test_every_form_of_the_product(form, M, N, K, dtype):
+    _product(M, N, K, dtype, True, seed=K)
+
+
+@pytest.mark.parametrize("cols", [5003, 16384])
+def test_rows_past_the_caches(cols):
+    # More than 64 MiB: read and written non-temporally; the same results as a part of it.
+    rows = (64 << 20) // (2 * cols) + 5
+    x, r = _randn(rows, cols, torch.float16, 1), _randn(rows, cols, torch.float16, 2)
+    w = torch.ones(cols, dtype=torch.float16, device=DEV)
+    part = slice(rows - 40, rows)
+    for make in (lambda t, s: I.quantize(t), lambda t, s: I.silu_mul(t[:, :cols // 2 * 2]),
+                 lambda t, s: I.rms_norm(t, w, residual=s)):
+        for got, want in zip(make(x, r), make(x[part], r[part])):
+            assert torch.equal(got[part], want)
+    q, scale = I.quantize(x)
+    assert torch.equal(I.dequantize(q, scale)[part], I.dequantize(q[part], scale[part]))
