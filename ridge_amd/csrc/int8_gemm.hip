@@ -12,9 +12,9 @@ using ridge::Int8Sizes;
 
 // How a product runs, by number: tiles of C as one workgroup each, or (kFew) small ones
 // whose K a workgroup's waves share.
-using Tile256x256 = ridge::Int8Traits<256, 256, 128, 128, 64, 2>;
-using Tile256x128 = ridge::Int8Traits<256, 128, 128, 64, 64, 3>;   // ping-pong
-using Tile128x128 = ridge::Int8Traits<128, 128, 128, 32, 64, 3>;
+using ridge::Tile128x128;
+using ridge::Tile256x128;
+using ridge::Tile256x256;
 using Pair128x128 = ridge::Int8Traits<128, 128, 128, 32, 64, 2>;   // two workgroups a CU
 using Tile64x128 = ridge::Int8Traits<64, 128, 128, 32, 32, 3>;
 using Tile64x64 = ridge::Int8Traits<64, 64, 128, 16, 32, 4>;
@@ -22,7 +22,7 @@ using Few16x16 = ridge::Int8FewTraits<1, 1, 8, 2>;
 using Few32x16 = ridge::Int8FewTraits<2, 1, 8, 2>;
 using Few32x32 = ridge::Int8FewTraits<2, 2, 8, 2>;
 
-constexpr int kCUs = 256;   // of an MI355X
+constexpr int kCUs = ridge::kInt8CUs;
 constexpr int kForms = 9, kFirstFew = 6;
 struct FormCost {
     int rows, cols;
@@ -49,6 +49,9 @@ constexpr FormCost kForm[kForms] = {
     {16, 16, 170, 70, 31},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
 };
 
+// A grid's work-items fit 32 bits, and its tiles the kernels' divisions.
+constexpr int64_t kMostTiles = 1 << 22;
+
 int64_t tilesOf(int form, int64_t M, int64_t N) {
     const FormCost& f = kForm[form];
     return ((M + f.rows - 1) / f.rows) * ((N + f.cols - 1) / f.cols);
@@ -60,8 +63,13 @@ int chooseForm(const Int8Sizes& z, bool packed) {
     // Small tiles of all sizes take the arguments of small ones only.
     for (int i = 0; i < (packed ? kForms : kFirstFew); ++i) {
         const FormCost& f = kForm[i];
-        const int64_t n = (tilesOf(i, z.M, z.N) + kCUs - 1) / kCUs;
-        const int64_t cost = f.call + n * (f.tile + (int64_t)f.perK * z.K / 1000);
+        const int64_t tiles = tilesOf(i, z.M, z.N);
+        auto rounds = [&](const FormCost& of, int64_t n) { return n * (of.tile + (int64_t)of.perK * z.K / 1000); };
+        int64_t cost = f.call + rounds(f, (tiles + kCUs - 1) / kCUs);
+        if (i == 0 && tiles < kMostTiles) {
+            const ridge::Int8Rounds r = ridge::int8Rounds((int)tiles);
+            if (r.parts > 1) cost = rounds(f, r.whole / kCUs) + rounds(kForm[r.parts == 2 ? 1 : 2], 1);
+        }
         if (cost < least) best = i, least = cost;
     }
     return best;
@@ -87,6 +95,14 @@ hipError_t launchTiles(const Int8Operands& p, const Int8Sizes& z, int64_t tiles,
     return hipGetLastError();
 }
 
+template <typename Out, bool PACKED, bool STREAM>
+hipError_t launchRounds(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
+    ridge::int8RoundsKernel<Out, PACKED, STREAM>
+        <<<dim3((unsigned)ridge::int8Rounds((int)tiles).blocks), dim3(Tile256x256::kThreads), 0, stream>>>(
+            ridge::int8Args<PACKED>(p, z));
+    return hipGetLastError();
+}
+
 template <typename T, typename Out>
 hipError_t launchFew(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
     ridge::int8FewKernel<T, Out><<<dim3((unsigned)tiles), dim3(T::kThreads), 0, stream>>>(ridge::int8Args<true>(p, z));
@@ -96,17 +112,16 @@ hipError_t launchFew(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, h
 template <typename Out, bool PACKED>
 hipError_t launchForm(int form, const Int8Operands& p, const Int8Sizes& z, hipStream_t s) {
     const int64_t tiles = tilesOf(form, z.M, z.N);
-    // A grid's work-items fit 32 bits, and its tiles the kernels' divisions.
-    if (tiles >= (1 << 23)) return hipErrorInvalidValue;
+    if (tiles >= kMostTiles) return hipErrorInvalidValue;
     if (streams<Out>(p, z)) {   // no other form has a grid of that size
         switch (form) {
-            case 0: return launchTiles<Tile256x256, Out, false, PACKED, true>(p, z, tiles, s);
+            case 0: return launchRounds<Out, PACKED, true>(p, z, tiles, s);
             case 1: return launchTiles<Tile256x128, Out, true, PACKED, true>(p, z, tiles, s);
             case 3: return launchTiles<Pair128x128, Out, false, PACKED, true>(p, z, tiles, s);
         }
     }
     switch (form) {
-        case 0: return launchTiles<Tile256x256, Out, false, PACKED>(p, z, tiles, s);
+        case 0: return launchRounds<Out, PACKED, false>(p, z, tiles, s);
         case 1: return launchTiles<Tile256x128, Out, true, PACKED>(p, z, tiles, s);
         case 2: return launchTiles<Tile128x128, Out, false, PACKED>(p, z, tiles, s);
         case 3: return launchTiles<Pair128x128, Out, false, PACKED>(p, z, tiles, s);

@@ -568,6 +568,63 @@ void int8GemmKernel(Int8Args<PACKED> args) {
     blk.template store<STREAM>();
 }
 
+using Tile256x256 = Int8Traits<256, 256, 128, 128, 64, 2>;
+using Tile256x128 = Int8Traits<256, 128, 128, 64, 64, 3>;   // ping-pong
+using Tile128x128 = Int8Traits<128, 128, 128, 32, 64, 3>;
+
+// Grids of 256 x 256 tiles: whole rounds of them on the chip's CUs, and what is left of
+// more than a round cut into as many parts as still fit one: a last round of few tiles
+// would leave most CUs idle. us, the fastest form without parts | with them: 4001 x 4103 x
+// 2065 (272 tiles) 55.6 | 41.5, 5888 x 5888 x 1664 (529) 70.6 | 59.4, 6144 x 4096 x 2048
+// (384) 58.2 | 51.4, 7663 x 5248 x 3712 (630) 129.6 | 121.4.
+constexpr int kInt8CUs = 256;
+struct Int8Rounds {
+    int whole, parts, blocks;   // tiles in whole rounds; parts of each other tile; workgroups
+};
+__host__ __device__ inline Int8Rounds int8Rounds(int tiles) {
+    const int left = tiles > kInt8CUs ? tiles % kInt8CUs : 0;
+    const int parts = left == 0 || left > kInt8CUs / 2 ? 1 : left > kInt8CUs / 4 ? 2 : 4;
+    const int whole = parts == 1 ? tiles : tiles - left;
+    return {whole, parts, whole + (tiles - whole) * parts};
+}
+
+template <typename Out, bool PACKED, bool STREAM>
+__global__ __launch_bounds__(Tile256x256::kThreads)
+void int8RoundsKernel(Int8Args<PACKED> args) {
+    using T = Tile256x256;
+    static_assert(T::kThreads == Tile256x128::kThreads && T::kThreads == Tile128x128::kThreads, "parts of one launch");
+    constexpr int kLds = T::kLdsBytes > Tile256x128::kLdsBytes ? T::kLdsBytes : Tile256x128::kLdsBytes;
+    static_assert(kLds >= Tile128x128::kLdsBytes, "the parts share the tile's LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[kLds];
+    const Int8Sizes z = args.sizes();
+    const int tilesM = int8TilesM<T>(z.M), tilesN = int8TilesN<T>(z.N);
+    const Int8Rounds r = int8Rounds(tilesM * tilesN);
+    int row, col;
+    if ((int)blockIdx.x < r.whole) {
+        int8TileOf<T>(xcdRemap(blockIdx.x, r.whole), tilesM, tilesN, row, col);
+        Int8Block<T, Out> blk(lds, args.p, z, row, col);
+        int8UniformLoop<T>(blk);
+        blk.template store<STREAM>();
+        return;
+    }
+    const int id = xcdRemap(blockIdx.x - r.whole, r.blocks - r.whole);
+    int8TileOf<T>(r.whole + id / r.parts, tilesM, tilesN, row, col);
+    if (r.parts == 4) {
+        row += id % 4 / 2 * 128;
+        col += id % 2 * 128;
+        if (row >= z.M || col >= z.N) return;   // a part of an edge tile that has nothing of C
+        Int8Block<Tile128x128, Out> blk(lds, args.p, z, row, col);
+        int8UniformLoop<Tile128x128>(blk);
+        blk.template store<STREAM>();
+    } else {
+        col += id % 2 * 128;
+        if (col >= z.N) return;
+        Int8Block<Tile256x128, Out> blk(lds, args.p, z, row, col);
+        int8PingPongLoop<Tile256x128>(blk);
+        blk.template store<STREAM>();
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Few tokens, or few tiles: 16 TM x 16 TN of C a workgroup, whose WAVES wavefronts share K.
 //

@@ -85,7 +85,8 @@ def test_host_tensors_are_refused():
 
 
 # What the GPU tests run the forms with, and the products that each is for.
-FORMS = [(0, 4001, 4093, 2065), (1, 4001, 4103, 2065), (1, 2301, 1805, 2049), (2, 2031, 2031, 1031), (3, 3873, 4263, 175), (4, 149, 8887, 4111),
+# Form 0 without parts, and with its last round's tiles in quarters and in halves.
+FORMS = [(0, 4001, 4093, 2065), (0, 4001, 4103, 2065), (0, 6001, 4100, 1040), (1, 2301, 1805, 2049), (2, 2031, 2031, 1031), (3, 829, 3583, 159), (4, 149, 8887, 4111),
          (5, 49, 8195, 1029), (6, 3, 4001, 1027), (7, 299, 301, 4099), (8, 791, 257, 3469)]
 
 
