@@ -31,8 +31,10 @@ struct FormCost {
 // With n the tiles of the busiest CU, the time of a launch is within 10 to 17% (one
 // standard deviation) of c + n (a + b K): the constants are fitted to 68 products of 1 to
 // 8192 rows, 74 to 16384 columns and K of 75 to 15814, of whole and odd sizes, each timed
-// in every form. The form that this makes the fastest was on average 0.9% slower than the
-// fastest one timed, 18% in the worst case (8192 x 8192 x 128). What the forms are for, us
+// in every form, and then moved to where the choice loses least: the form that they make
+// the fastest was 0.8% slower on average than the fastest one timed, 18% in the worst case
+// (8192 x 8192 x 128). 256 x 256 tiles count their last round by its parts (int8Rounds,
+// which those times are without). What the forms are for, us
 // 256x256 | 256x128 | 128x128 | its pair | 64x128 | 64x64 | few 16x16 | 32x16 | 32x32:
 //   4096 x 4096 x 4096   52.3 | 58.8 | 75.0 | 61.9 | 80.8 | 98.3 | - | - | -
 //   2319 x 1792 x 6784   64.1 | 33.8 | 49.1 | 37.8 | 45.6 | 48.8 | - | - | -
@@ -46,7 +48,7 @@ struct FormCost {
 constexpr FormCost kForm[kForms] = {
     {256, 256, 0, 750, 856},  {256, 128, 0, 680, 455}, {128, 128, 50, 400, 327},
     {128, 128, 190, 220, 372}, {64, 128, 200, 150, 223}, {64, 64, 210, 120, 136},
-    {16, 16, 170, 70, 31},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
+    {16, 16, 170, 70, 43},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
 };
 
 // A grid's work-items fit 32 bits, and its tiles the kernels' divisions.

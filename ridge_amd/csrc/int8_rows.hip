@@ -146,7 +146,7 @@ __device__ __forceinline__ float quotient(float v, float d) {
 template <typename T, bool STREAM>
 struct Plain {
     typedef RowArgs Args;
-    static constexpr bool kNorm = false;
+    static constexpr bool kNorm = false, kStream = STREAM;
     const T* x;
     __device__ Plain(const Args& a, int64_t row) : x((const T*)a.x + row * a.ldx) {}
     template <int n>
@@ -158,7 +158,7 @@ struct Plain {
 template <typename T, bool STREAM>
 struct Gated {
     typedef RowArgs Args;
-    static constexpr bool kNorm = false;
+    static constexpr bool kNorm = false, kStream = STREAM;
     const T* x;
     int cols;
     __device__ Gated(const Args& a, int64_t row) : x((const T*)a.x + row * a.ldx), cols(a.cols) {}
@@ -177,7 +177,7 @@ struct Gated {
 template <typename T, typename W, bool STREAM, bool DENSE>
 struct Normed {
     typedef NormArgs<DENSE> Args;
-    static constexpr bool kNorm = true;
+    static constexpr bool kNorm = true, kStream = STREAM;
     const T* x;
     const T* residual;
     const W* weight;
@@ -339,10 +339,19 @@ hipError_t launchRows(const typename Source::Args& a, hipStream_t stream) {
 
 // The threads of a row, by its length: as many as hold it in at most four vectors each. A
 // norm's 1024 threads have not got the registers for that: it reads rows of more than
-// 16384 columns twice.
+// 16384 columns twice. Few rows leave CUs to spare and take more threads and fewer vectors
+// each, which also is less code to run through once: us in a graph, silu as for many rows
+// | so: 13 x 2048 4.2 | 2.7, 4 x 8192 4.5 | 4.0, 500 x 8192 7.2 | 6.8; 16000 x 2048 39.4 |
+// 41.8. Not the norm, whose sum would be added up in another order: a row's result must
+// not depend on how many rows there are.
+constexpr int kFewRows = 512;
 template <typename Source>
 hipError_t launchByLength(const typename Source::Args& a, hipStream_t stream) {
     if (a.cols <= 64 * kVec) return launchRows<Source, 64, 1>(a, stream);
+    if constexpr (!Source::kNorm && !Source::kStream) {   // no few rows of these lengths are that large
+        if (a.rows <= kFewRows && a.cols <= 256 * kVec) return launchRows<Source, 256, 1>(a, stream);
+        if (a.rows <= kFewRows && a.cols <= 512 * kVec * 2) return launchRows<Source, 512, 2>(a, stream);
+    }
     if (a.cols <= 64 * kVec * 4) return launchRows<Source, 64, 4>(a, stream);
     if (a.cols <= 256 * kVec * 4) return launchRows<Source, 256, 4>(a, stream);
     if (a.cols <= 512 * kVec * 4) return launchRows<Source, 512, 4>(a, stream);

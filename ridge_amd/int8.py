@@ -11,10 +11,11 @@ held in 8 bits with one scale each, what makes them, and their matrix product.
     dequantize(q, scale)       -> the values q * scale
 
 q is int8 and scale float32; the 16- and 32-bit tensors are float16, bfloat16 or
-float32. Sums, norms and scales are held in 32 bits, and a product's sum is exact. A
-weight [channels, K] goes through quantize() once and is b from then on. Rows may be
-views: of any stride and offset in 16 and 32 bits, in 8 bits ones that start at multiples
-of 16 bytes, which empty() sees to for every number of columns.
+float32. Sums, norms and scales are held in 32 bits, and a product's sum is exact: a
+row's result is the same, bit for bit, whatever rows are beside it. A weight
+[channels, K] goes through quantize() once and is b from then on. Rows may be views: of
+any stride and offset in 16 and 32 bits, in 8 bits ones that start at multiples of 16
+bytes, which empty() sees to for every number of columns.
 
 Every call is asynchronous on `stream` (the current one by default) and writes into
 `out` where that is given: as everywhere, a tensor that another stream made or will free

@@ -495,3 +495,19 @@ def test_rows_past_the_caches(cols):
             assert torch.equal(got[part], want)
     q, scale = I.quantize(x)
     assert torch.equal(I.dequantize(q, scale)[part], I.dequantize(q[part], scale[part]))
+
+
+@pytest.mark.parametrize("cols", [600, 2048, 2049, 8192, 11007])
+def test_a_row_does_not_depend_on_the_rows_beside_it(cols):
+    x, r = _randn(700, cols, torch.bfloat16, 1), _randn(700, cols, torch.bfloat16, 2)
+    w, b = torch.ones(cols, dtype=torch.bfloat16, device=DEV), _int8(300, cols, 3)
+    for make in (lambda t, s: I.quantize(t), lambda t, s: I.silu_mul(t[:, :cols // 2 * 2]),
+                 lambda t, s: I.rms_norm(t, w, residual=s)):
+        whole = make(x, r)
+        for rows in (slice(0, 1), slice(3, 20), slice(100, 612)):
+            for got, want in zip(make(x[rows], r[rows]), whole):
+                assert torch.equal(got, want[rows])
+    q, scale = I.quantize(x)
+    y = I.gemm(q, scale, *b)
+    for rows in (slice(0, 1), slice(3, 20), slice(100, 612)):
+        assert torch.equal(I.gemm(q[rows], scale[rows], *b), y[rows])
