@@ -68,7 +68,8 @@ int ridge_int8_dequantize(const int8_t* q, int64_t ldq, const float* scale, void
                           int64_t rows, int64_t cols, void* stream);
 
 /* C [M, N] of `type` <- the product above; bias [N] of `type`, or null. K is at most
- * RIDGE_INT8_MAX_K, and an 8-bit stride below 2^23. */
+ * RIDGE_INT8_MAX_K, an 8-bit stride below 2^23, and C at most 2^23 - 1024 tiles of 256 x
+ * 256. */
 int ridge_int8_gemm(const int8_t* A, int64_t lda, const float* scaleA, const int8_t* B, int64_t ldb,
                     const float* scaleB, const void* bias, void* C, int64_t ldc, int type, int64_t M, int64_t N,
                     int64_t K, void* stream);

@@ -51,8 +51,9 @@ constexpr FormCost kForm[kForms] = {
     {16, 16, 170, 70, 43},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
 };
 
-// A grid's work-items fit 32 bits, and its tiles the kernels' divisions.
-constexpr int64_t kMostTiles = 1 << 22;
+// A grid's work-items fit 32 bits, its tiles the kernels' divisions, and neither gains more
+// than a round by parts.
+constexpr int64_t kMostTiles = (1 << 23) - 1024;
 
 int64_t tilesOf(int form, int64_t M, int64_t N) {
     const FormCost& f = kForm[form];
@@ -66,6 +67,7 @@ int chooseForm(const Int8Sizes& z, bool packed) {
     for (int i = 0; i < (packed ? kForms : kFirstFew); ++i) {
         const FormCost& f = kForm[i];
         const int64_t tiles = tilesOf(i, z.M, z.N);
+        if (i > 0 && tiles >= kMostTiles) continue;
         auto rounds = [&](const FormCost& of, int64_t n) { return n * (of.tile + (int64_t)of.perK * z.K / 1000); };
         int64_t cost = f.call + rounds(f, (tiles + kCUs - 1) / kCUs);
         if (i == 0 && tiles < kMostTiles) {

@@ -129,16 +129,20 @@ struct NormArgs<false> {
     __device__ int64_t ldResidualOutOf() const { return ldResidualOut; }
 };
 
-// v / d for d of 1 and more, rounded correctly but where d comes near the range's end and
-// the quotient is nothing beside it: Newton's step on the reciprocal, the product, and
-// its exact remainder's correction. Six instructions where a division of any two numbers
-// takes ten.
+// v / d for d from 1 to kFarDivisor, rounded correctly: Newton's step on the reciprocal, the
+// product, and its exact remainder's correction. Six instructions, where a division of any
+// two numbers takes ten and bounded the gated activation.
+constexpr float kFarDivisor = 1e37f;
 __device__ __forceinline__ float quotient(float v, float d) {
     float r = __builtin_amdgcn_rcpf(d);
     r = fmaf(fmaf(-d, r, 1.0f), r, r);
-    float q = v * r;
-    q = fmaf(fmaf(-d, q, v), r, q);
-    return d > 1e37f ? v * 0.0f : q;
+    const float q = v * r;
+    return fmaf(fmaf(-d, q, v), r, q);
+}
+
+// And for larger ones, whose reciprocal leaves the normal numbers: within a unit.
+__device__ __forceinline__ float farQuotient(float v, float d) {
+    return v * __builtin_amdgcn_rcpf(d * 0x1p-64f) * 0x1p-64f;
 }
 
 // Sources of a row's values: load() gives n of them from column col on, and adds what the
@@ -167,8 +171,21 @@ struct Gated {
         float u[n];
         loadRow<STREAM>(x + col, v);
         loadRow<STREAM>(x + cols + col, u);
+        float d[n], g[n], most = 0.0f;
 #pragma unroll
-        for (int e = 0; e < n; ++e) v[e] = quotient(v[e], 1.0f + expf(-v[e])) * u[e];
+        for (int e = 0; e < n; ++e) {
+            d[e] = 1.0f + expf(-v[e]);
+            most = fmaxf(most, d[e]);
+            g[e] = v[e];
+            v[e] = quotient(g[e], d[e]);
+        }
+        if (most > kFarDivisor) {   // gates under -85: few waves have one
+#pragma unroll
+            for (int e = 0; e < n; ++e)
+                if (d[e] > kFarDivisor) v[e] = farQuotient(g[e], d[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < n; ++e) v[e] *= u[e];
     }
 };
 

@@ -511,3 +511,20 @@ def test_a_row_does_not_depend_on_the_rows_beside_it(cols):
     y = I.gemm(q, scale, *b)
     for rows in (slice(0, 1), slice(3, 20), slice(100, 612)):
         assert torch.equal(I.gemm(q[rows], scale[rows], *b), y[rows])
+
+
+def test_silu_of_values_whose_exponential_comes_near_the_ranges_end():
+    g = torch.tensor([[-87.5, -86.0, -85.0, -80.0]], device=DEV)
+    u = torch.tensor([[1e36, 1e36, -1e36, 1e34]], device=DEV)
+    q, scale = I.silu_mul(torch.cat([g, u], dim=1))
+    _check_rows(q, scale, g.double() * torch.sigmoid(g.double()) * u.double())
+
+
+def test_a_product_of_more_rows_than_the_smallest_tiles_count():
+    # 64 x 64 tiles, which few columns ask for, would be more than a launch has.
+    M, K = 600_000_000, 16
+    a = torch.zeros((M, K), dtype=torch.int8, device=DEV)
+    a[-3:] = 5
+    sa, b, sb = torch.ones(M, device=DEV), torch.full((1, K), 2, dtype=torch.int8, device=DEV), torch.ones(1, device=DEV)
+    out = I.gemm(a, sa, b, sb)
+    assert torch.all(out[-3:] == 160) and not out[:-3].any()
