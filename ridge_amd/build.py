@@ -26,6 +26,7 @@ import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -199,18 +200,20 @@ def build_int8(gate=True):
     """libridge_int8.so. No kernel of it may use scratch memory."""
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIB, exist_ok=True)
-    objs, spilling = [], 0
-    for src in INT8_SRCS:
-        o = os.path.join(BUILD, src.replace(".hip", ".o"))
-        remarks = _run([HIPCC] + LIB_HIP_FLAGS + ["-Rpass-analysis=kernel-resource-usage", "-x", "hip", "-c",
-                                                  os.path.join(CSRC, src), "-o", o], capture=True)
-        kernels = kernel_remarks(remarks)
+    objs, spilling = [os.path.join(BUILD, src.replace(".hip", ".o")) for src in INT8_SRCS], 0
+
+    def compiled(src, o):
+        return _run([HIPCC] + LIB_HIP_FLAGS + ["-Rpass-analysis=kernel-resource-usage", "-x", "hip", "-c",
+                                               os.path.join(CSRC, src), "-o", o], capture=True)
+    with ThreadPoolExecutor(len(INT8_SRCS)) as pool:
+        remarks = list(pool.map(compiled, INT8_SRCS, objs))
+    for src, text in zip(INT8_SRCS, remarks):
+        kernels = kernel_remarks(text)
         bad = {k: r for k, r in kernels.items() if r["scratch"] or r["vgpr_spill"] or r["sgpr_spill"]}
         print("  %s: %d kernels, %d spilling" % (src, len(kernels), len(bad)))
         for k, r in bad.items():
             print("    SPILL %s: %s" % (k, r))
         spilling += len(bad)
-        objs.append(o)
     if spilling and gate:
         raise SystemExit("spill gate: %d 8-bit kernel(s) use scratch" % spilling)
     so = os.path.join(LIB, "libridge_int8.so")

@@ -117,7 +117,7 @@ template <typename Out, bool PACKED>
 hipError_t launchForm(int form, const Int8Operands& p, const Int8Sizes& z, hipStream_t s) {
     const int64_t tiles = tilesOf(form, z.M, z.N);
     if (tiles >= kMostTiles) return hipErrorInvalidValue;
-    if (streams<Out>(p, z)) {   // no other form has a grid of that size
+    if (streams<Out>(p, z)) {   // the other forms hardly ever have a C of that size
         switch (form) {
             case 0: return launchRounds<Out, PACKED, true>(p, z, tiles, s);
             case 1: return launchTiles<Tile256x128, Out, true, PACKED, true>(p, z, tiles, s);
@@ -184,5 +184,6 @@ extern "C" int ridge_int8_gemm_form(int64_t M, int64_t N, int64_t K) {
     if (M < 1 || N < 1 || K < 1 || M > kMostRows || N > kMostRows || K > RIDGE_INT8_MAX_K) return -1;
     const int ld = (int)ridge_int8_row_stride(K);
     const Int8Sizes z = {(int)M, (int)N, (int)K, ld, ld, N};
-    return chooseForm(z, ridge::int8ArgsFit(z));
+    const int form = chooseForm(z, ridge::int8ArgsFit(z));
+    return tilesOf(form, M, N) < kMostTiles ? form : -1;
 }

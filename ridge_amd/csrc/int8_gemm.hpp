@@ -6,10 +6,9 @@
 // A (M x K) and B (N x K) both have k along memory. v_mfma_i32_16x16x64_i8 takes 16
 // consecutive k of one row a lane (16 bytes, lane group g = lane / 16 holding k = 16 g ..
 // 16 g + 15), which is byte for byte the operand layout of the FP16 instruction of half
-// the K: a tile's rows are loaded straight into LDS in 16-byte chunks, swizzled (swizzleRows), and
-// both fragments are single ds_read_b128s. With B's
-// fragment in the first operand lane l holds C[m0 + l % 16][n0 + 4 (l / 16) + r] in
-// element r.
+// the K: a tile's rows are loaded straight into LDS in 16-byte chunks, swizzled
+// (swizzleRows), and both fragments are single ds_read_b128s. With B's fragment in the
+// first operand lane l holds C[m0 + l % 16][n0 + 4 (l / 16) + r] in element r.
 //
 // Any M, N and K: a row past the end of A or B is replaced by the last one (its products
 // are not stored), and of the last K tile's chunks those past the end by the last chunk;

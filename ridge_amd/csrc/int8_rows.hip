@@ -129,6 +129,22 @@ struct NormArgs<false> {
     __device__ int64_t ldResidualOutOf() const { return ldResidualOut; }
 };
 
+// e^x as 2^n 2^f: x log2(e) in two f32 parts, n the whole number next to it and f what is
+// left, which the exponential's instruction takes. Within a unit, as expf is, of fewer
+// instructions: the ends of the range are one clamp, behind which 2^n makes infinities and
+// zeros by itself, and a NaN need not come out of it (it comes out of the gate's product).
+// Its steps are not to be contracted: high - n in one step with its product would hold the
+// part that low adds. (Bit for bit expf for every x below 1e30.)
+__device__ __forceinline__ float exponential(float x) {
+#pragma clang fp contract(off)
+    constexpr float kLog2e = 1.44269504088896341f, kRest = (float)(1.44269504088896341 - (double)kLog2e);
+    x = __builtin_amdgcn_fmed3f(x, -128.0f, 128.0f);
+    const float high = x * kLog2e;
+    const float low = fmaf(x, kRest, fmaf(x, kLog2e, -high));
+    const float n = rintf(high);
+    return ldexpf(__builtin_amdgcn_exp2f((high - n) + low), (int)n);
+}
+
 // v / d for d from 1 to kFarDivisor, rounded correctly: Newton's step on the reciprocal, the
 // product, and its exact remainder's correction. Six instructions, where a division of any
 // two numbers takes ten and bounded the gated activation.
@@ -174,7 +190,7 @@ struct Gated {
         float d[n], g[n], most = 0.0f;
 #pragma unroll
         for (int e = 0; e < n; ++e) {
-            d[e] = 1.0f + expf(-v[e]);
+            d[e] = 1.0f + exponential(-v[e]);
             most = fmaxf(most, d[e]);
             g[e] = v[e];
             v[e] = quotient(g[e], d[e]);

@@ -100,7 +100,8 @@ def test_every_form_of_the_product_is_chosen_somewhere(form, M, N, K):
 def test_form_of_sizes_without_a_product():
     L = ctypes.CDLL(I.LIB_PATH)
     L.ridge_int8_gemm_form.argtypes = [ctypes.c_int64] * 3
-    for sizes in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, I.MAX_K + 1), (1 << 31, 1, 1), (1, -4, 1)):
+    for sizes in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, I.MAX_K + 1), (1 << 31, 1, 1), (1, -4, 1),
+                  (1 << 30, 1 << 30, 16)):
         assert L.ridge_int8_gemm_form(*sizes) == -1
     # Sizes past 16 bits take no form of small tiles, whose arguments hold 16.
     assert 0 <= L.ridge_int8_gemm_form(1, 70000, 64) < 6 and 0 <= L.ridge_int8_gemm_form(70000, 1, 131071) < 6
