@@ -166,6 +166,7 @@ struct RowsOut {
         if (r.rows != rows || r.cols != cols)
             refuse("out holds %lld x %lld, not %lld x %lld", (long long)r.rows, (long long)r.cols, (long long)rows,
                    (long long)cols);
+        noGradient(&scale);
         ld = r.ld;
     }
     int8_t* at8() const { return (int8_t*)q.data_ptr(); }
@@ -196,6 +197,7 @@ struct MatrixOut {
                            : tensor(out, "out");
         r = matrix(t, "out", &device);
         code = typeOf(t, "out");
+        noGradient(&t);
         if (r.rows != rows || r.cols != cols || (type && t.scalar_type() != *type))
             refuse("out must be %lld x %lld%s%s", (long long)rows, (long long)cols, type ? " of " : "",
                    type ? c10::toString(*type) : "");
@@ -255,6 +257,7 @@ PyObject* rmsNormImpl(PyObject* const* args, Py_ssize_t n) {
             refuse("residual must be like x");
         if (residualOut.scalar_type() != x.scalar_type() || to.rows != r.rows || to.cols != r.cols)
             refuse("residual_out must be like x");
+        noGradient(&residualOut);
     }
     const RowsOut out(args[5], r.rows, r.cols, device);
     enqueued("ridge_int8_rms_norm",
@@ -272,6 +275,7 @@ PyObject* dequantizeImpl(PyObject* const* args, Py_ssize_t n) {
     const at::Tensor &q = tensor(args[0], "q"), &scale = tensor(args[1], "scale");
     const Rows r = rows8(q, scale, "q");
     if (r.cols < 1) refuse("q has no columns");
+    noGradient(&scale);
     const On on(q.device(), args[4]);
     const MatrixOut out(args[3], args[2], r.rows, r.cols, q.device());
     enqueued("ridge_int8_dequantize",
@@ -291,9 +295,11 @@ PyObject* gemmImpl(PyObject* const* args, Py_ssize_t n) {
         refuse("K must be 1 to %d and strides below %lld, not %lld, %lld and %lld", (int)RIDGE_INT8_MAX_K,
                (long long)kMostStride, (long long)ra.cols, (long long)ra.ld, (long long)rb.ld);
     const at::Tensor* bias = optionalTensor(args[4], "bias");
+    noGradient(&aScale);
+    noGradient(&bScale);
+    noGradient(bias);
     const On on(device, args[7]);
     const MatrixOut out(args[6], args[5], ra.rows, rb.rows, device);
-    noGradient(bias);
     if (bias) vector(*bias, rb.rows, out.t.scalar_type(), device, "bias");
     enqueued("ridge_int8_gemm",
              ridge_int8_gemm((const int8_t*)a.data_ptr(), ra.ld, (const float*)aScale.data_ptr(),

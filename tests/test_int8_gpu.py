@@ -528,3 +528,26 @@ def test_a_product_of_more_rows_than_the_smallest_tiles_count():
     sa, b, sb = torch.ones(M, device=DEV), torch.full((1, K), 2, dtype=torch.int8, device=DEV), torch.ones(1, device=DEV)
     out = I.gemm(a, sa, b, sb)
     assert torch.all(out[-3:] == 160) and not out[:-3].any()
+
+
+def test_no_call_drops_a_gradient():
+    x = _randn(4, 64, torch.float16, 1)
+    w = torch.ones(64, dtype=torch.float16, device=DEV)
+    q, s = I.quantize(x)
+    bias = torch.zeros(4, dtype=torch.float16, device=DEV)
+
+    def leaf(t):
+        return t.clone().requires_grad_()
+    calls = [
+        lambda: I.quantize(leaf(x)), lambda: I.silu_mul(leaf(x)), lambda: I.quantize(x, out=(q, leaf(s))),
+        lambda: I.rms_norm(leaf(x), w), lambda: I.rms_norm(x, leaf(w)), lambda: I.rms_norm(x, w, residual=leaf(x)),
+        lambda: I.rms_norm(x, w, residual=x, residual_out=leaf(x)),
+        lambda: I.dequantize(q, leaf(s)), lambda: I.dequantize(q, s, out=leaf(x)),
+        lambda: I.gemm(q, leaf(s), q, s), lambda: I.gemm(q, s, q, leaf(s)), lambda: I.gemm(q, s, q, s, bias=leaf(bias)),
+        lambda: I.gemm(q, s, q, s, out=leaf(torch.empty((4, 4), dtype=torch.float16, device=DEV))),
+    ]
+    for call in calls:
+        with pytest.raises(I.RidgeInt8Error, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
