@@ -4,7 +4,9 @@
  *
  * An 8-bit row stands for the values q[j] * scale: q is a whole number in -127 .. 127
  * and scale the row's largest magnitude over 127 (the smallest normal float, where it
- * would be less). The rows that are rounded are f32, and halves round to even:
+ * would be less). The rows that are rounded are f32, and halves round to even: q is the
+ * whole number next to 127 value / largest, not to the quotient by the scale's f32, which
+ * is off by its own rounding (half of the largest value, 63.5, is 64 in every row):
  *   quantize:  the rows as they are;
  *   silu_mul:  g / (1 + exp(-g)) * u of a row that holds g and then u;
  *   rms_norm:  s / sqrt(mean(s^2) + eps) * weight of s = x + residual.

@@ -9,7 +9,7 @@
 //
 // A norm needs one reduction, not two: the sum of squares and the largest |s w| are taken
 // together, because the reciprocal root that multiplies a whole row moves out of the
-// maximum.
+// maximum, and out of the quotients that are rounded.
 
 #include "ridge_int8.h"
 
@@ -61,18 +61,30 @@ __device__ __forceinline__ void storeRow(T* at, const float (&v)[n]) {
     }
 }
 
-// Nearest whole numbers (halves to even) of v / scale, which is at most 127 and a rounding.
-// The quotient is the correctly rounded one, by one correction of v * (1 / scale) with its
-// exact remainder: a product alone rounds values near a half the other way. Adding 1.5 *
-// 2^23 leaves the whole number in the low bits. A row whose scale is not finite gets bytes
-// that mean nothing.
+// A value that all lanes of the wave have, in a scalar register (a wave is never of two rows).
+// It saves the norm, and rows read twice, a wave a SIMD (16384 x 8192 with dequantize 242 us
+// without it, 226 with it); the gated kernels of 4 vectors lose one by it.
+__device__ __forceinline__ float uniform(float v) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
+// A row's 127th: the largest magnitude over 127 is whole + rest to about 46 bits.
+struct Step {
+    float whole, rest, inverse;   // and 1 / whole
+};
+
+// Nearest whole numbers (halves to even) of v / step. The quotient is v * (1 / step) corrected
+// once by its remainder, which is exact but for what `rest` lacks, so that a quotient of n + 1/2
+// comes out as that: by the step's f32 alone, half of a row's largest value (63.5) went to 63
+// or to 64 as the step was rounded. Adding 1.5 * 2^23 leaves the whole number in the low bits.
+// A row whose scale is not finite gets bytes that mean nothing.
 template <int n>
-__device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], float scale, float inverse) {
+__device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], const Step& step) {
     typename Memory<signed char, n>::Vec b;
 #pragma unroll
     for (int e = 0; e < n; ++e) {
-        float t = v[e] * inverse;
-        t = fmaf(fmaf(-t, scale, v[e]), inverse, t);
+        float t = v[e] * step.inverse;
+        t = fmaf(fmaf(-t, step.rest, fmaf(-t, step.whole, v[e])), step.inverse, t);
         b[e] = (signed char)__float_as_uint(t + 12582912.0f);
     }
     *(typename Memory<signed char, n>::Vec*)at = b;
@@ -273,6 +285,8 @@ __device__ __forceinline__ void reduceRow(float& sum, uint32_t& top) {
 
 constexpr int64_t kMostBlocks = 1 << 20;  // of a grid: its blocks walk the rows behind them
 
+constexpr float kLift = 0x1p64f, kSmallRow = 0x1p-60f;
+
 // One row a kThreads threads. kVecs vectors a thread hold the row; with kVecs = 0 a row
 // of any length is read twice.
 template <typename Source, int kThreads, int kVecs>
@@ -281,6 +295,7 @@ void makeRowsKernel(typename Source::Args a) {
     constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
     constexpr int kRowsPerBlock = kBlock / kThreads;
     constexpr bool kHeld = kVecs > 0;
+    constexpr bool kScalar = Source::kNorm || !kHeld;   // a row's results in scalar registers
     const int lane = threadIdx.x % kThreads;
     const int whole = a.cols / kVec * kVec;    // columns of whole vectors
     const int single = whole + lane;           // and this lane's behind them
@@ -313,17 +328,34 @@ void makeRowsKernel(typename Source::Args a) {
             // A sum past the range of f32 would make the root 0 and the row silently so.
             root = squares <= FLT_MAX ? 1.0f / sqrtf(squares / (float)a.cols + a.eps) : NAN;
         }
-        float scale = __uint_as_float(top) * root / 127.0f;
-        scale = scale < FLT_MIN ? FLT_MIN : scale;  // a NaN stays one
-        const float inverse = 1.0f / scale;
+        const float most = kScalar ? uniform(__uint_as_float(top)) : __uint_as_float(top);
+        float scale = most * root / 127.0f;
+        // q is value / (most / 127): the root is in both and cancels. Rows of small values are
+        // lifted by a power of two, so that the step's rest stays a normal number.
+        const bool small = most < kSmallRow;
+        const float lifted = small ? most * kLift : most;
+        Step step;
+        step.whole = lifted / 127.0f;
+        step.rest = fmaf(-127.0f, step.whole, lifted) / 127.0f;
+        if (scale < FLT_MIN) {  // a NaN stays one
+            scale = FLT_MIN;
+            step.whole = (small ? FLT_MIN * kLift : FLT_MIN) / root;
+            step.rest = 0.0f;
+        }
+        step.inverse = 1.0f / step.whole;
+        if constexpr (kScalar) step = {uniform(step.whole), uniform(step.rest), uniform(step.inverse)};
         if (lane == 0) a.scale[row] = scale;
         int8_t* const q = a.q + row * a.ldq();
+        auto lift = [&](int, auto& values) {
+            for (float& value : values) value *= kLift;
+        };
+        if (kHeld && small) parts(lift);
         parts([&](int col, auto& values) {
-            if constexpr (!kHeld) source.load(col, values, squares, true);
-            if constexpr (Source::kNorm) {
-                for (float& value : values) value *= root;
+            if constexpr (!kHeld) {
+                source.load(col, values, squares, true);
+                if (small) lift(col, values);
             }
-            storeRounded(q + col, values, scale, inverse);
+            storeRounded(q + col, values, step);
         });
     }
 }

@@ -551,3 +551,24 @@ def test_no_call_drops_a_gradient():
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("dtype,exponents", [(torch.float16, (-10, 0, 15)), (torch.bfloat16, (-118, -60, 0, 55)),
+                                             (torch.float32, (-118, -60, 0, 55))])
+@pytest.mark.parametrize("cols", [3, 700, 20000, 33000])
+def test_half_of_a_rows_largest_value_is_a_half_and_goes_to_even(cols, dtype, exponents):
+    # 127 (top / 2) / top is 63.5 whatever f32 makes of top / 127.
+    bits = {torch.float16: 10, torch.bfloat16: 7, torch.float32: 23}[dtype]
+    mantissas = torch.arange(0, 1 << bits, max(1, (1 << bits) // 128 - (bits > 7)), device=DEV)
+    for exponent in exponents:
+        print("2^%d" % exponent, flush=True)
+        top = ((1 + mantissas.double() / 2 ** bits) * 2.0 ** exponent).to(dtype)
+        x = torch.zeros((len(top), cols), dtype=dtype, device=DEV)
+        x[:, 0], x[:, 1], x[:, -1] = -top, top / 2, -top / 2
+        one = torch.ones(cols, dtype=dtype, device=DEV)
+        # silu(32) is 32 in f32.
+        makers = {"quantize": I.quantize(x), "silu_mul": I.silu_mul(torch.cat([torch.full_like(x, 32), x], dim=1)),
+                  "rms_norm": I.rms_norm(x, one)[:2]}
+        for name, (q, scale) in makers.items():
+            assert torch.all(q[:, 0] == -127) and torch.all(q[:, 1] == 64) and torch.all(q[:, -1] == -64), name
+            assert not q[:, 2:-1].any()
