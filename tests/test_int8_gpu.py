@@ -572,3 +572,22 @@ def test_half_of_a_rows_largest_value_is_a_half_and_goes_to_even(cols, dtype, ex
         for name, (q, scale) in makers.items():
             assert torch.all(q[:, 0] == -127) and torch.all(q[:, 1] == 64) and torch.all(q[:, -1] == -64), name
             assert not q[:, 2:-1].any()
+
+
+# silu(g) u of gates whose e^-g is past f32, where a large u brings the product back. Rows of
+# 16 bits as far as their u goes.
+FAR = [(torch.float32, [-89.0, -89.5, -90.0, -92.0], 3e38), (torch.float32, [-100.0, -101.0, -102.5, -104.0], 1e35),
+       (torch.float32, [-160.0, -165.0, -168.0, -170.0], 3e38), (torch.bfloat16, [-89.0, -90.0, -91.0, -95.0], 1e38),
+       (torch.bfloat16, [-120.0, -121.0, -124.0, -130.0], -2e38), (torch.float16, [-88.75, -89.0, -90.0, -92.0], 6e4),
+       (torch.float32, [-86.0, -88.0, -88.5, -89.0], 1e30)]
+
+
+@pytest.mark.parametrize("dtype,gates,up", FAR)
+def test_silu_of_gates_whose_exponential_is_past_the_range(dtype, gates, up):
+    # e^g to 2 u, the products with g and u one each, the last scaling one: within the 8 u
+    # that _check_rows allows.
+    for n in (4, 500):
+        g = torch.tensor([gates], device=DEV).to(dtype).repeat(3, n // 4)
+        u = torch.full_like(g, up)
+        q, scale = I.silu_mul(torch.cat([g, u], dim=1))
+        _check_rows(q, scale, g.double() * torch.exp(g.double()) / (1 + torch.exp(g.double())) * u.double())
