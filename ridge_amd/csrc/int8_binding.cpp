@@ -71,6 +71,12 @@ void noGradient(const at::Tensor* t) {
         refuse("the 8-bit operators have no gradient: call them under torch.no_grad()");
 }
 
+// A tensor of the caller's that a call has written through its address: a graph that saved it
+// notices by its version, as for torch's own writes. (Tensors of inference mode have none.)
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct Rows {
     int64_t rows, cols, ld;
 };
@@ -171,6 +177,11 @@ struct RowsOut {
     }
     int8_t* at8() const { return (int8_t*)q.data_ptr(); }
     float* atScale() const { return (float*)scale.data_ptr(); }
+    void wrote() const {
+        if (given == Py_None) return;
+        written(q);
+        written(scale);
+    }
     PyObject* result() const {
         if (given != Py_None) return Py_NewRef(given);
         return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(scale));
@@ -202,6 +213,9 @@ struct MatrixOut {
             refuse("out must be %lld x %lld%s%s", (long long)rows, (long long)cols, type ? " of " : "",
                    type ? c10::toString(*type) : "");
     }
+    void wrote() const {
+        if (given != Py_None) written(t);
+    }
     PyObject* result() const { return given != Py_None ? Py_NewRef(given) : THPVariable_Wrap(t); }
     PyObject* given;
 };
@@ -221,6 +235,7 @@ PyObject* rowsOf(PyObject* const* args, Py_ssize_t n, bool gated) {
     const auto call = gated ? ridge_int8_silu_mul : ridge_int8_quantize;
     enqueued(gated ? "ridge_int8_silu_mul" : "ridge_int8_quantize",
              call(x.data_ptr(), r.ld, code, out.at8(), out.ld, out.atScale(), r.rows, cols, on.stream()));
+    out.wrote();
     return out.result();
 }
 
@@ -264,6 +279,8 @@ PyObject* rmsNormImpl(PyObject* const* args, Py_ssize_t n) {
              ridge_int8_rms_norm(x.data_ptr(), r.ld, residual ? residual->data_ptr() : nullptr, in.ld, weight.data_ptr(),
                                  weightCode, (float)eps, code, residual ? residualOut.data_ptr() : nullptr, to.ld,
                                  out.at8(), out.ld, out.atScale(), r.rows, r.cols, on.stream()));
+    out.wrote();
+    if (residual && args[4] != Py_None) written(residualOut);
     PyObject* sum = !residual ? Py_NewRef(Py_None) : args[4] != Py_None ? Py_NewRef(args[4]) : THPVariable_Wrap(residualOut);
     if (args[5] != Py_None)
         return Py_BuildValue("(OON)", PyTuple_GET_ITEM(args[5], 0), PyTuple_GET_ITEM(args[5], 1), sum);
@@ -281,6 +298,7 @@ PyObject* dequantizeImpl(PyObject* const* args, Py_ssize_t n) {
     enqueued("ridge_int8_dequantize",
              ridge_int8_dequantize((const int8_t*)q.data_ptr(), r.ld, (const float*)scale.data_ptr(), out.t.data_ptr(),
                                    out.r.ld, out.code, r.rows, r.cols, on.stream()));
+    out.wrote();
     return out.result();
 }
 
@@ -306,6 +324,7 @@ PyObject* gemmImpl(PyObject* const* args, Py_ssize_t n) {
                              (const int8_t*)b.data_ptr(), rb.ld, (const float*)bScale.data_ptr(),
                              bias ? bias->data_ptr() : nullptr, out.t.data_ptr(), out.r.ld, out.code, ra.rows, rb.rows,
                              ra.cols, on.stream()));
+    out.wrote();
     return out.result();
 }
 
