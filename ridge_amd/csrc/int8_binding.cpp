@@ -69,6 +69,9 @@ int typeOf(const at::Tensor& t, const char* what) {
 void noGradient(const at::Tensor* t) {
     if (t && t->requires_grad() && at::GradMode::is_enabled())
         refuse("the 8-bit operators have no gradient: call them under torch.no_grad()");
+    // Level 0 is the only one. Undefined too where forward mode is off; no_grad leaves it on.
+    if (t && t->_fw_grad(0).defined())
+        refuse("the 8-bit operators have no gradient in forward mode either: take the primal of dual tensors");
 }
 
 // A tensor of the caller's that a call has written through its address: a graph that saved it

@@ -21,8 +21,9 @@ Every call is asynchronous on `stream` (the current one by default) and writes i
 `out` where that is given: as everywhere, a tensor that another stream made or will free
 is the caller's to order. Outputs that a call allocates itself belong to the stream that
 it runs on. Nothing here has a gradient: inputs that need one are refused where gradients
-are on, and a graph that saved a tensor which a call then writes raises in its backward, as
-after torch's own in-place operations. There is no fallback: without the native library every entry point raises.
+are on, and so are forward mode's dual tensors; a graph that saved a tensor which a call then
+writes raises in its backward, as after torch's own in-place operations. There is no
+fallback: without the native library every entry point raises.
 """
 
 import ctypes

@@ -83,3 +83,37 @@ def test_a_blocks_workspace_is_not_overwritten_under_a_graph_in_silence():
     for loss in losses:
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.backward()
+
+
+def test_a_tangent_is_refused():
+    from torch.autograd import forward_ad
+    x, w, q, s, bias = _operands()
+    calls = [
+        lambda dual: I.quantize(dual(x)), lambda dual: I.silu_mul(dual(x)), lambda dual: I.quantize(x, out=(q, dual(s))),
+        lambda dual: I.rms_norm(dual(x), w), lambda dual: I.rms_norm(x, dual(w)),
+        lambda dual: I.rms_norm(x, w, residual=dual(x)), lambda dual: I.rms_norm(x, w, residual=x, residual_out=dual(x)),
+        lambda dual: I.dequantize(q, dual(s)), lambda dual: I.dequantize(q, s, out=dual(x)),
+        lambda dual: I.gemm(q, dual(s), q, s), lambda dual: I.gemm(q, s, q, dual(s)),
+        lambda dual: I.gemm(q, s, q, s, bias=dual(bias)),
+        lambda dual: I.gemm(q, s, q, s, out=dual(torch.empty((4, 4), dtype=torch.float16, device=DEV))),
+    ]
+
+    def dual(t):
+        return forward_ad.make_dual(t.clone(), torch.ones_like(t))
+    for i, call in enumerate(calls):
+        print("call", i, flush=True)
+        # Forward mode goes on under no_grad: it is refused there too.
+        for mode in (torch.enable_grad(), torch.no_grad()):
+            with mode, forward_ad.dual_level(), pytest.raises(I.RidgeInt8Error, match="gradient"):
+                call(dual)
+        with forward_ad.dual_level(), forward_ad._set_fwd_grad_enabled(False):
+            call(dual)
+
+
+def test_functional_transforms_are_refused():
+    x, w, q, s, bias = _operands()
+    for transform in (lambda: torch.func.jvp(lambda t: I.quantize(t)[1], (x,), (torch.ones_like(x),)),
+                      lambda: torch.func.vjp(lambda t: I.quantize(t)[1], x),
+                      lambda: torch.func.vmap(lambda t: I.quantize(t)[1])(x.reshape(2, 2, 64))):
+        with pytest.raises(RuntimeError):
+            transform()
