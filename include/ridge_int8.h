@@ -25,6 +25,8 @@
  * length; strides and pointers of 16- and 32-bit matrices need the alignment of their
  * type only. 8-bit rows start at multiples of 16 bytes (pointer and stride), and their
  * last 16 bytes are readable: what they hold behind the row's length does not matter.
+ * What a call writes shares no byte with anything else of the call, residualOut excepted
+ * where its comment says so: workgroups run in any order, and this is not checked here.
  * No rows is a call that does nothing; a row of no columns is refused.
  *
  * No HIP header is needed to use this file: streams are passed as void*.

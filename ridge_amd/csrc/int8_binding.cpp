@@ -14,10 +14,12 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <optional>
+#include <utility>
 
 #include "ridge_int8.h"
 
@@ -120,6 +122,52 @@ Rows rows8(const at::Tensor& q, const at::Tensor& scale, const char* what, const
     return r;
 }
 
+// The bytes of a matrix: rows of `bytes`, `stride` apart.
+struct Span {
+    const char* what;
+    int64_t at, rows, bytes, stride;
+};
+
+Span span(const at::Tensor& t, const Rows& r, const char* what) {
+    const int64_t size = t.element_size();
+    return {what, (int64_t)t.data_ptr(), r.rows, r.cols * size, r.ld * size};
+}
+
+Span span(const at::Tensor& vector, const char* what) {
+    return span(vector, {1, vector.size(0), vector.size(0)}, what);
+}
+
+int64_t floorDivide(int64_t n, int64_t d) { return n / d - (n % d < 0); }
+
+// Whether any row of a shares a byte with one of b: column slices of one buffer do not, whose
+// rows lie between each other's.
+bool meet(Span a, Span b) {
+    if (a.rows < 1 || b.rows < 1 || a.bytes < 1 || b.bytes < 1) return false;
+    if (a.at >= b.at + (b.rows - 1) * b.stride + b.bytes || b.at >= a.at + (a.rows - 1) * a.stride + a.bytes) return false;
+    if (a.rows > b.rows) std::swap(a, b);
+    if (b.rows == 1) return true;
+    if (a.rows == 1) a.stride = b.stride;
+    // The last row of b that begins before the end of a's row i ends behind all others.
+    auto row = [&](int64_t i, int64_t least) {
+        const int64_t begin = a.at + i * a.stride;
+        const int64_t j = std::min(floorDivide(begin + a.bytes - 1 - b.at, b.stride), least + b.rows - 1);
+        return j >= least && b.at + j * b.stride + b.bytes > begin;
+    };
+    // Of equal strides only j - i counts, from 1 - a.rows on.
+    if (a.stride == b.stride) {
+        b.rows += a.rows - 1;
+        return row(0, 1 - a.rows);
+    }
+    for (int64_t i = 0; i < a.rows; ++i)
+        if (row(i, 0)) return true;
+    return false;
+}
+
+// A call's workgroups read and write in no order: what it writes may be nothing else of it.
+void apart(const Span& written, const Span& other) {
+    if (meet(written, other)) refuse("%s overlaps %s", written.what, other.what);
+}
+
 // Makes the operands' device current, and the stream: the current one for None, else one
 // of torch's streams or a handle. Memory that a call allocates is then that stream's.
 class On {
@@ -177,6 +225,14 @@ struct RowsOut {
                    (long long)cols);
         noGradient(&scale);
         ld = r.ld;
+        apart(span(scale, "out's scales"), span8());
+    }
+    Span span8() const { return span(q, {q.size(0), q.size(1), ld}, "out's q"); }
+    // An operand of the call that writes the rows.
+    void apartFrom(const Span& other) const {
+        if (given == Py_None) return;
+        apart(span8(), other);
+        apart(span(scale, "out's scales"), other);
     }
     int8_t* at8() const { return (int8_t*)q.data_ptr(); }
     float* atScale() const { return (float*)scale.data_ptr(); }
@@ -216,6 +272,9 @@ struct MatrixOut {
             refuse("out must be %lld x %lld%s%s", (long long)rows, (long long)cols, type ? " of " : "",
                    type ? c10::toString(*type) : "");
     }
+    void apartFrom(const Span& other) const {
+        if (given != Py_None) apart(span(t, r, "out"), other);
+    }
     void wrote() const {
         if (given != Py_None) written(t);
     }
@@ -235,6 +294,7 @@ PyObject* rowsOf(PyObject* const* args, Py_ssize_t n, bool gated) {
     const int64_t cols = gated ? r.cols / 2 : r.cols;
     const On on(x.device(), args[2]);
     const RowsOut out(args[1], r.rows, cols, x.device());
+    out.apartFrom(span(x, r, what));
     const auto call = gated ? ridge_int8_silu_mul : ridge_int8_quantize;
     enqueued(gated ? "ridge_int8_silu_mul" : "ridge_int8_quantize",
              call(x.data_ptr(), r.ld, code, out.at8(), out.ld, out.atScale(), r.rows, cols, on.stream()));
@@ -278,6 +338,20 @@ PyObject* rmsNormImpl(PyObject* const* args, Py_ssize_t n) {
         noGradient(&residualOut);
     }
     const RowsOut out(args[5], r.rows, r.cols, device);
+    const Span spanX = span(x, r, "x"), spanWeight = span(weight, "weight");
+    out.apartFrom(spanX);
+    out.apartFrom(spanWeight);
+    if (residual) {
+        const Span spanResidual = span(*residual, in, "residual"), spanSum = span(residualOut, to, "residual_out");
+        out.apartFrom(spanResidual);
+        if (args[4] != Py_None) {
+            out.apartFrom(spanSum);
+            apart(spanSum, spanWeight);
+            // x or residual itself: a thread reads what it then writes.
+            for (const Span& from : {spanX, spanResidual})
+                if (spanSum.at != from.at || spanSum.stride != from.stride) apart(spanSum, from);
+        }
+    }
     enqueued("ridge_int8_rms_norm",
              ridge_int8_rms_norm(x.data_ptr(), r.ld, residual ? residual->data_ptr() : nullptr, in.ld, weight.data_ptr(),
                                  weightCode, (float)eps, code, residual ? residualOut.data_ptr() : nullptr, to.ld,
@@ -298,6 +372,8 @@ PyObject* dequantizeImpl(PyObject* const* args, Py_ssize_t n) {
     noGradient(&scale);
     const On on(q.device(), args[4]);
     const MatrixOut out(args[3], args[2], r.rows, r.cols, q.device());
+    out.apartFrom(span(q, r, "q"));
+    out.apartFrom(span(scale, "scale"));
     enqueued("ridge_int8_dequantize",
              ridge_int8_dequantize((const int8_t*)q.data_ptr(), r.ld, (const float*)scale.data_ptr(), out.t.data_ptr(),
                                    out.r.ld, out.code, r.rows, r.cols, on.stream()));
@@ -322,6 +398,11 @@ PyObject* gemmImpl(PyObject* const* args, Py_ssize_t n) {
     const On on(device, args[7]);
     const MatrixOut out(args[6], args[5], ra.rows, rb.rows, device);
     if (bias) vector(*bias, rb.rows, out.t.scalar_type(), device, "bias");
+    out.apartFrom(span(a, ra, "a"));
+    out.apartFrom(span(b, rb, "b"));
+    out.apartFrom(span(aScale, "a_scale"));
+    out.apartFrom(span(bScale, "b_scale"));
+    if (bias) out.apartFrom(span(*bias, "bias"));
     enqueued("ridge_int8_gemm",
              ridge_int8_gemm((const int8_t*)a.data_ptr(), ra.ld, (const float*)aScale.data_ptr(),
                              (const int8_t*)b.data_ptr(), rb.ld, (const float*)bScale.data_ptr(),

@@ -15,7 +15,9 @@ float32. Sums, norms and scales are held in 32 bits, and a product's sum is exac
 row's result is the same, bit for bit, whatever rows are beside it. A weight
 [channels, K] goes through quantize() once and is b from then on. Rows may be views: of
 any stride and offset in 16 and 32 bits, in 8 bits ones that start at multiples of 16
-bytes, which empty() sees to for every number of columns.
+bytes, which empty() sees to for every number of columns. What a call writes may be nothing
+else of the call (rms_norm's residual_out excepted): an output that shares a byte with an
+operand is refused, column slices of one buffer are not.
 
 Every call is asynchronous on `stream` (the current one by default) and writes into
 `out` where that is given: as everywhere, a tensor that another stream made or will free

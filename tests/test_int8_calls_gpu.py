@@ -117,3 +117,91 @@ def test_functional_transforms_are_refused():
                       lambda: torch.func.vmap(lambda t: I.quantize(t)[1])(x.reshape(2, 2, 64))):
         with pytest.raises(RuntimeError):
             transform()
+
+
+def test_outputs_over_operands_are_refused():
+    x, w, q, s, bias = _operands()
+    flat = torch.zeros(1024, dtype=torch.float16, device=DEV)
+    bytes_ = flat.view(torch.int8)
+    f32 = flat.view(torch.float32)
+    view = flat[:256].view(4, 64)
+    out8 = I.empty(4, 64)
+    rows8 = bytes_[:256].view(4, 64)
+    C = flat[:16].view(4, 4)
+    refused = {
+        "shifted by a row": lambda: I.rms_norm(view, w, residual=x, residual_out=flat[64:320].view(4, 64)),
+        "shifted by an element": lambda: I.rms_norm(view, w, residual=x, residual_out=flat[1:257].view(4, 64)),
+        "another stride": lambda: I.rms_norm(view, w, residual=x, residual_out=flat.as_strided((4, 64), (65, 1))),
+        "over the residual": lambda: I.rms_norm(x, w, residual=view, residual_out=flat[64:320].view(4, 64)),
+        "x itself, over the residual": lambda: I.rms_norm(view, w, residual=flat[64:320].view(4, 64), residual_out=view),
+        "over the weight": lambda: I.rms_norm(x, flat[:64], residual=x, residual_out=view),
+        "rows over x": lambda: I.rms_norm(view, w, out=(rows8, s)),
+        "rows over the residual": lambda: I.rms_norm(x, w, residual=view, out=(rows8, s)),
+        "rows over the sum": lambda: I.rms_norm(x, w, residual=x, residual_out=view, out=(rows8, s)),
+        "scales over x": lambda: I.rms_norm(view, w, out=(out8[0], f32[126:130])),
+        "scales in the rows": lambda: I.quantize(x, out=(rows8, f32[60:64])),
+        "quantize over x": lambda: I.quantize(view, out=(rows8, s)),
+        "quantize's scales": lambda: I.quantize(view, out=(out8[0], f32[:4])),
+        "silu_mul over its rows": lambda: I.silu_mul(view, out=(rows8[:, :32], s)),
+        "dequantize over q": lambda: I.dequantize(rows8, s, out=view),
+        "dequantize over its scales": lambda: I.dequantize(q, f32[100:104], out=view),
+        "C over a": lambda: I.gemm(rows8, s, q, s, out=C),
+        "C over b": lambda: I.gemm(q, s, rows8, s, out=C),
+        "C over a_scale": lambda: I.gemm(q, f32[:4], q, s, out=C),
+        "C over b_scale": lambda: I.gemm(q, s, q, f32[4:8], out=C),
+        "C over the bias": lambda: I.gemm(q, s, q, s, bias=flat[12:16], out=C),
+    }
+    for name, call in refused.items():
+        print(name, flush=True)
+        with pytest.raises(I.RidgeInt8Error, match="overlaps"):
+            call()
+
+
+def test_outputs_beside_operands_in_one_buffer():
+    x, w, q, s, bias = _operands()
+    want = I.quantize(x)
+    # x, the residual and the sum as columns of one buffer, the 8-bit rows behind them.
+    memory = torch.zeros((4, 64 * 3 + 32), dtype=torch.float16, device=DEV)
+    view, residual, total = (memory[:, 64 * i:64 * i + 64] for i in range(3))
+    rows8 = memory.view(torch.int8)[:, 384:448]
+    view.copy_(x)
+    assert torch.equal(I.quantize(view, out=(rows8, s))[0], want[0])
+    got = I.rms_norm(view, w, residual=residual, residual_out=total, out=(rows8, s))
+    assert torch.equal(got[0], I.rms_norm(x, w)[0]) and torch.equal(total, x)
+    # In place, where x and the residual are the same too.
+    for into in (view, residual):
+        into.copy_(x)
+        assert torch.equal(I.rms_norm(into, w, residual=into, residual_out=into)[2], x + x)
+    # Halves of one buffer.
+    both = torch.zeros((8, 64), dtype=torch.float16, device=DEV)
+    both[:4] = x
+    assert torch.equal(I.rms_norm(both[:4], w, residual=both[:4], residual_out=both[4:])[2], x + x)
+
+
+def test_overlap_of_rows_at_any_stride():
+    # Random views of one buffer against the bytes that they consist of.
+    import random
+    rng = random.Random(3)
+    memory = torch.zeros(1 << 12, dtype=torch.int8, device=DEV)
+    s = torch.ones(9, device=DEV)
+    met = 0
+    for case in range(600):
+        rows, cols = rng.randint(1, 9), rng.randint(1, 40)
+        ld8 = 16 * rng.randint((cols + 15) // 16, 8)
+        at8 = 16 * rng.randint(0, 40)
+        ld16 = ld8 // 2 if rng.random() < 0.5 and ld8 // 2 >= cols else rng.randint(cols, 90)
+        at16 = rng.randint(0, 400)
+        q = memory.as_strided((rows, cols), (ld8, 1), at8)
+        out = memory.view(torch.float16).as_strided((rows, cols), (ld16, 1), at16)
+        read = {at8 + i * ld8 + j for i in range(rows) for j in range(cols)}
+        written = {2 * (at16 + i * ld16 + j) + e for i in range(rows) for j in range(cols) for e in (0, 1)}
+        overlap = bool(read & written)
+        met += overlap
+        try:
+            I.dequantize(q, s[:rows], out=out)
+            refused = False
+        except I.RidgeInt8Error as e:
+            assert "overlaps" in str(e)
+            refused = True
+        assert refused == overlap, (case, rows, cols, ld8, at8, ld16, at16)
+    assert 100 < met < 500
