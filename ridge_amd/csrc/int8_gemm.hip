@@ -1,6 +1,7 @@
 // int8_gemm.hip -- the launches of the 8-bit product, for the C ABI in include/ridge_int8.h.
 
 #include "int8_gemm.hpp"
+#include "int8_launch.hpp"
 #include "ridge_int8.h"
 
 #include <hip/hip_runtime.h>
@@ -94,23 +95,21 @@ bool streams(const Int8Operands& p, const Int8Sizes& z) {
 
 template <typename T, typename Out, bool PINGPONG, bool PACKED, bool STREAM = false>
 hipError_t launchTiles(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
-    ridge::int8GemmKernel<T, Out, PINGPONG, PACKED, STREAM>
-        <<<dim3((unsigned)tiles), dim3(T::kThreads), 0, stream>>>(ridge::int8Args<PACKED>(p, z));
-    return hipGetLastError();
+    return ridge::launchKernel(ridge::int8GemmKernel<T, Out, PINGPONG, PACKED, STREAM>, (unsigned)tiles, T::kThreads,
+                               stream, ridge::int8Args<PACKED>(p, z));
 }
 
 template <typename Out, bool PACKED, bool STREAM>
 hipError_t launchRounds(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
-    ridge::int8RoundsKernel<Out, PACKED, STREAM>
-        <<<dim3((unsigned)ridge::int8Rounds((int)tiles).blocks), dim3(Tile256x256::kThreads), 0, stream>>>(
-            ridge::int8Args<PACKED>(p, z));
-    return hipGetLastError();
+    return ridge::launchKernel(ridge::int8RoundsKernel<Out, PACKED, STREAM>,
+                               (unsigned)ridge::int8Rounds((int)tiles).blocks, Tile256x256::kThreads, stream,
+                               ridge::int8Args<PACKED>(p, z));
 }
 
 template <typename T, typename Out>
 hipError_t launchFew(const Int8Operands& p, const Int8Sizes& z, int64_t tiles, hipStream_t stream) {
-    ridge::int8FewKernel<T, Out><<<dim3((unsigned)tiles), dim3(T::kThreads), 0, stream>>>(ridge::int8Args<true>(p, z));
-    return hipGetLastError();
+    return ridge::launchKernel(ridge::int8FewKernel<T, Out>, (unsigned)tiles, T::kThreads, stream,
+                               ridge::int8Args<true>(p, z));
 }
 
 template <typename Out, bool PACKED>

@@ -11,6 +11,7 @@
 // together, because the reciprocal root that multiplies a whole row moves out of the
 // maximum, and out of the quotients that are rounded.
 
+#include "int8_launch.hpp"
 #include "ridge_int8.h"
 
 #include <hip/hip_runtime.h>
@@ -414,8 +415,7 @@ hipError_t launchRows(const typename Source::Args& a, hipStream_t stream) {
     constexpr int kBlock = kThreads < 256 ? 256 : kThreads;
     constexpr int kRowsPerBlock = kBlock / kThreads;
     const int64_t blocks = std::min<int64_t>((a.rows + (int64_t)kRowsPerBlock - 1) / kRowsPerBlock, kMostBlocks);
-    makeRowsKernel<Source, kThreads, kVecs><<<dim3((unsigned)blocks), dim3(kBlock), 0, stream>>>(a);
-    return hipGetLastError();
+    return ridge::launchKernel(makeRowsKernel<Source, kThreads, kVecs>, (unsigned)blocks, kBlock, stream, a);
 }
 
 // The threads of a row, by its length: as many as hold it in at most four vectors each. A
@@ -486,13 +486,9 @@ template <typename T>
 hipError_t launchDequantize(const int8_t* q, int64_t ldq, const float* scale, void* out, int64_t ldOut, int rows,
                             int cols, bool stream, hipStream_t s) {
     const int pieces = (int)(((int64_t)cols + kDequantizeThreads * kVec - 1) / (kDequantizeThreads * kVec));
-    const dim3 grid((unsigned)std::min<int64_t>((int64_t)rows * pieces, kMostBlocks)), block(kDequantizeThreads);
-    if (stream) {
-        dequantizeKernel<T, true><<<grid, block, 0, s>>>(q, ldq, scale, (T*)out, ldOut, rows, cols, pieces);
-    } else {
-        dequantizeKernel<T, false><<<grid, block, 0, s>>>(q, ldq, scale, (T*)out, ldOut, rows, cols, pieces);
-    }
-    return hipGetLastError();
+    const unsigned blocks = (unsigned)std::min<int64_t>((int64_t)rows * pieces, kMostBlocks);
+    return ridge::launchKernel(stream ? dequantizeKernel<T, true> : dequantizeKernel<T, false>, blocks,
+                               kDequantizeThreads, s, q, ldq, scale, (T*)out, ldOut, rows, cols, pieces);
 }
 
 }  // namespace

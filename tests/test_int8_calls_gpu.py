@@ -1,4 +1,6 @@
 """What the 8-bit operators' calls do with the tensors and streams that they are given."""
+import ctypes
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -205,3 +207,17 @@ def test_overlap_of_rows_at_any_stride():
             refused = True
         assert refused == overlap, (case, rows, cols, ld8, at8, ld16, at16)
     assert 100 < met < 500
+
+
+def test_an_earlier_failed_call_is_not_this_ones():
+    x, w, q, s, bias = _operands()
+    hip = ctypes.CDLL(I.LIB_PATH)   # its runtime, found through it
+    calls = [lambda: I.quantize(x), lambda: I.silu_mul(x), lambda: I.rms_norm(x, w), lambda: I.dequantize(q, s),
+             lambda: I.gemm(q, s, q, s)]
+    for call in calls:
+        call()
+        assert hip.hipSetDevice(1 << 20) != 0   # a refusal by the runtime, which it also keeps as the last error
+        try:
+            call()
+        finally:
+            hip.hipGetLastError()
