@@ -168,35 +168,51 @@ void apart(const Span& written, const Span& other) {
     if (meet(written, other)) refuse("%s overlaps %s", written.what, other.what);
 }
 
+// An attribute that is a whole number, or a whole number itself.
+void* numberOf(PyObject* o, const char* attribute) {
+    PyObject* number = PyLong_Check(o) ? Py_NewRef(o) : PyObject_GetAttrString(o, attribute);
+    void* value = number ? PyLong_AsVoidPtr(number) : nullptr;
+    Py_XDECREF(number);
+    if (PyErr_Occurred()) throw python_error();
+    return value;
+}
+
+// The handle of one of torch's streams, or the handle itself, on the operands' device.
+hipStream_t streamOf(PyObject* stream, c10::DeviceIndex device) {
+    const hipStream_t handle = (hipStream_t)numberOf(stream, "cuda_stream");
+    int64_t on = device;
+    hipDevice_t found;
+    if (PyObject_HasAttrString(stream, "device_index")) {   // a default stream's handle is null on every device
+        on = (int64_t)(intptr_t)numberOf(stream, "device_index");
+    } else if (handle && hipStreamGetDevice(handle, &found) == hipSuccess) {
+        on = found;
+    }
+    if (on != device) refuse("the stream is on device %lld, not on the operands' %d", (long long)on, (int)device);
+    return handle;
+}
+
 // Makes the operands' device current, and the stream: the current one for None, else one
 // of torch's streams or a handle. Memory that a call allocates is then that stream's.
 class On {
   public:
     On(const at::Device& device, PyObject* stream) : device_(device.index()), before_(c10::hip::current_device()) {
+        const hipStream_t p = stream != Py_None ? streamOf(stream, device_) : nullptr;
         if (device_ != before_) c10::hip::set_device(device_);
         if (stream != Py_None) {
-            PyObject* handle = PyLong_Check(stream) ? Py_NewRef(stream) : PyObject_GetAttrString(stream, "cuda_stream");
-            void* p = handle ? PyLong_AsVoidPtr(handle) : nullptr;
-            Py_XDECREF(handle);
-            if (PyErr_Occurred()) {
-                leave();
-                throw python_error();
-            }
             current_ = c10::hip::getCurrentHIPStream(device_);
-            c10::hip::setCurrentHIPStream(p ? c10::hip::getStreamFromExternal((hipStream_t)p, device_)
+            c10::hip::setCurrentHIPStream(p ? c10::hip::getStreamFromExternal(p, device_)
                                             : c10::hip::getDefaultHIPStream(device_));
         }
     }
-    ~On() { leave(); }
+    ~On() {
+        if (current_) c10::hip::setCurrentHIPStream(*current_);
+        if (device_ != before_) c10::hip::set_device(before_);
+    }
     On(const On&) = delete;
     On& operator=(const On&) = delete;
     void* stream() const { return c10::hip::getCurrentHIPStream(device_).stream(); }
 
   private:
-    void leave() {
-        if (current_) c10::hip::setCurrentHIPStream(*current_);
-        if (device_ != before_) c10::hip::set_device(before_);
-    }
     c10::DeviceIndex device_, before_;
     std::optional<c10::hip::HIPStream> current_;
 };

@@ -221,3 +221,28 @@ def test_an_earlier_failed_call_is_not_this_ones():
             call()
         finally:
             hip.hipGetLastError()
+
+
+def test_a_stream_of_another_device_is_refused():
+    class Elsewhere:
+        cuda_stream, device_index = 0, 1
+    x, w, q, s, bias = _operands()
+    for call in (lambda t: I.quantize(x, stream=t), lambda t: I.rms_norm(x, w, stream=t),
+                 lambda t: I.dequantize(q, s, stream=t), lambda t: I.gemm(q, s, q, s, stream=t)):
+        with pytest.raises(I.RidgeInt8Error, match="stream"):
+            call(Elsewhere())
+
+
+def test_streams_by_object_and_by_handle():
+    x = _operands()[0]
+    want = I.quantize(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (None, side, side.cuda_stream, torch.cuda.default_stream(), 0, torch.cuda.ExternalStream(side.cuda_stream)):
+        q, scale = I.quantize(x, stream=stream)
+        torch.cuda.synchronize()
+        assert torch.equal(q, want[0]) and torch.equal(scale, want[1])
+        assert torch.cuda.current_stream() == torch.cuda.default_stream()
+    for stream in ("stream", 1.5, object()):
+        with pytest.raises((AttributeError, TypeError)):
+            I.quantize(x, stream=stream)
