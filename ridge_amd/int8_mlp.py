@@ -42,14 +42,15 @@ class Int8Mlp:
                 "y": torch.empty((tokens, self.hidden), dtype=dtype, device=device),
                 "residual": torch.empty((tokens, self.hidden), dtype=dtype, device=device)}
 
-    def __call__(self, x, residual, workspace=None):
-        """(y, x + residual), on the current stream; both in the workspace where one is given."""
+    def __call__(self, x, residual=None, workspace=None):
+        """(y, x + residual), on the current stream; both in the workspace where one is given.
+        Without a residual, as before a model's first block, the sum is x itself."""
         w = workspace or self.workspace(x.shape[0], x.dtype)
-        h, h_scale, residual = int8.rms_norm(x, self.norm_weight, self.eps, residual=residual,
-                                             residual_out=w["residual"], out=w["h"])
+        h, h_scale, total = int8.rms_norm(x, self.norm_weight, self.eps, residual=residual,
+                                          residual_out=None if residual is None else w["residual"], out=w["h"])
         gate_up = int8.gemm(h, h_scale, *self.gate_up, out=w["gate_up"])
         a, a_scale = int8.silu_mul(gate_up, out=w["a"])
-        return int8.gemm(a, a_scale, *self.down, out=w["y"]), residual
+        return int8.gemm(a, a_scale, *self.down, out=w["y"]), x if residual is None else total
 
 
 def plain_block(x, residual, norm_weight, gate_up, down, eps=1e-6):

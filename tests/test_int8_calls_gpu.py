@@ -246,3 +246,18 @@ def test_streams_by_object_and_by_handle():
     for stream in ("stream", 1.5, object()):
         with pytest.raises((AttributeError, TypeError)):
             I.quantize(x, stream=stream)
+
+
+@pytest.mark.parametrize("tokens", [1, 33])
+def test_feed_forward_block_without_a_residual(tokens):
+    from ridge_amd.int8_mlp import Int8Mlp, plain_block, random_block
+    mlp = Int8Mlp(*random_block(256, 512, torch.float16, 1))
+    x = _randn(tokens, 256, torch.float16, 2)
+    y, residual = mlp(x, None)
+    assert residual is x
+    space = mlp.workspace(tokens, torch.float16)
+    y2, residual = mlp(x, None, space)
+    assert y2 is space["y"] and residual is x and torch.equal(y, y2)
+    # x + 0 is x: the same block.
+    y3, s = mlp(x, torch.zeros_like(x))
+    assert torch.equal(y, y3) and torch.equal(s, x)
