@@ -1,5 +1,6 @@
 """What the 8-bit operators' calls do with the tensors and streams that they are given."""
 import ctypes
+import math
 
 import pytest
 
@@ -261,3 +262,17 @@ def test_feed_forward_block_without_a_residual(tokens):
     # x + 0 is x: the same block.
     y3, s = mlp(x, torch.zeros_like(x))
     assert torch.equal(y, y3) and torch.equal(s, x)
+
+
+def test_feed_forward_command_fails_on_results_that_are_not_numbers(monkeypatch):
+    from ridge_amd import int8_mlp
+    plain = int8_mlp.random_block
+
+    def broken(*args):
+        norm_weight, gate_up, down = plain(*args)
+        down[0, 0] = math.nan
+        return norm_weight, gate_up, down
+    args = ["--hidden", "64", "--inner", "64", "--tokens", "1,2", "--steps", "2"]
+    assert int8_mlp.main(args) == 0
+    monkeypatch.setattr(int8_mlp, "random_block", broken)
+    assert int8_mlp.main(args) == 1
