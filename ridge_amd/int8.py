@@ -68,7 +68,8 @@ def lib():
             ("silu_mul", [p, n, i, p, n, p, n, n, p]),
             ("rms_norm", [p, n, p, n, p, i, f, i, p, n, p, n, p, n, n, p]),
             ("dequantize", [p, n, p, p, n, i, n, n, p]),
-            ("gemm", [p, n, p, p, n, p, p, p, n, i, n, n, n, p])):
+            ("gemm", [p, n, p, p, n, p, p, p, n, i, n, n, n, p]),
+            ("gemm_form", [n, n, n])):
         function = getattr(L, "ridge_int8_" + name)
         function.restype, function.argtypes = i, args
     L.ridge_int8_row_stride.restype, L.ridge_int8_row_stride.argtypes = n, [n]

@@ -591,3 +591,69 @@ def test_silu_of_gates_whose_exponential_is_past_the_range(dtype, gates, up):
         u = torch.full_like(g, up)
         q, scale = I.silu_mul(torch.cat([g, u], dim=1))
         _check_rows(q, scale, g.double() * torch.exp(g.double()) / (1 + torch.exp(g.double())) * u.double())
+
+
+H, B, F = torch.float16, torch.bfloat16, torch.float32
+# (form, type, M, N, K) of products whose C goes past the caches: rows of whole cache lines,
+# more than 64 MiB. Sizes of up to 65535 rows and more (the two forms of a launch's
+# arguments); form 0 with its last round in quarters, halves and whole.
+PAST = [(0, H, 4200, 8181, 200), (0, B, 5000, 8180, 100), (0, F, 6100, 8171, 100), (0, H, 174416, 193, 32),
+        (0, B, 174416, 193, 32), (0, F, 130662, 129, 33), (1, H, 35553, 1029, 4020), (1, B, 11584, 3443, 4096),
+        (1, F, 1542, 13871, 2048), (1, H, 325436, 104, 785), (1, B, 325436, 104, 785), (1, F, 255113, 68, 668),
+        (3, H, 56363, 610, 33), (3, B, 56363, 610, 33), (3, F, 1303, 13581, 64), (3, H, 600000, 61, 64),
+        (3, B, 600000, 61, 64), (3, F, 261876, 65, 32)]
+
+
+@pytest.mark.parametrize("form,dtype,M,N,K", PAST)
+def test_every_form_past_the_caches_stays_inside_its_rows(form, dtype, M, N, K):
+    assert I.lib().ridge_int8_gemm_form(M, N, K) == form
+    size = torch.empty((), dtype=dtype).element_size()
+    assert M * N * size > 64 << 20
+    line = 128 // size
+    memory = torch.full((M + 2, (N + line) // line * line), 7.0, dtype=dtype, device=DEV)
+    out = memory[1:-1, :N]
+    assert out.data_ptr() % 128 == 0 and out.stride(0) * size % 128 == 0 and out.stride(0) > N
+    a, sa = _int8(M, K, 1, least=-128)
+    b, sb = _int8(N, K, 2, least=-128)
+    sb = sb / math.sqrt(K)
+    bias = _randn(1, N, dtype, 3)[0]
+    I.gemm(a, sa, b, sb, bias=bias, out=out)
+    for rows in torch.arange(M, device=DEV).split(1 << 16):
+        part = slice(int(rows[0]), int(rows[-1]) + 1)
+        _check_product(out[part], a[part], sa[part], b, sb, bias)
+    out.fill_(7.0)
+    assert torch.all(memory == 7.0), "wrote outside C"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1003, 5002, 16384])
+def test_rows_past_the_caches_of_every_type(cols, dtype):
+    # Rows of wider buffers: the same bits as a part of them gives, and nothing beside them.
+    size = torch.empty((), dtype=dtype).element_size()
+    rows = (64 << 20) // (size * cols) + 5
+    x, r = _randn(rows, cols, dtype, 1, 5, 3), _randn(rows, cols, dtype, 2, 3, 1)
+    w = _randn(1, cols, dtype, 3)[0]
+    part = slice(rows - 40, rows)
+    ld = I.lib().ridge_int8_row_stride(cols) + 128
+    memory = torch.full((rows + 2, ld), 99, dtype=torch.int8, device=DEV)
+    total = torch.full((rows + 2, cols + 9), 7.0, dtype=dtype, device=DEV)
+    inside = memory[1:-1, 16:16 + cols]
+    half = cols // 2
+    makers = [lambda t, s, sum_, q, scale: I.quantize(t, out=(q, scale)),
+              lambda t, s, sum_, q, scale: I.silu_mul(t[:, :2 * half], out=(q[:, :half], scale)),
+              lambda t, s, sum_, q, scale: I.rms_norm(t, w, residual=s, residual_out=sum_, out=(q, scale))]
+    for i, make in enumerate(makers):
+        width = half if i == 1 else cols
+        got = make(x, r, total[1:-1, 4:-5], inside, torch.empty(rows, device=DEV))
+        want = make(x[part], r[part], torch.empty((40, cols), dtype=dtype, device=DEV), *I.empty(40, cols))
+        for g, t in zip(got, want):
+            assert torch.equal(g[part], t)
+        inside[:, :width] = 99
+        assert torch.all(memory == 99)
+        total[1:-1, 4:-5] = 7.0
+        assert torch.all(total == 7.0)
+    q, scale = I.quantize(x)
+    I.dequantize(q, scale, out=total[1:-1, 4:-5])
+    assert torch.equal(total[1:-1, 4:-5][part], I.dequantize(q[part], scale[part], dtype))
+    total[1:-1, 4:-5] = 7.0
+    assert torch.all(total == 7.0)
