@@ -29,14 +29,15 @@ struct FormCost {
     int rows, cols;
     int call, tile, perK;   // 10 ns: c, a and 1000 b of the time c + n (a + b K)
 };
-// With n the tiles of the busiest CU, the time of a launch is within 10 to 17% (one
-// standard deviation) of c + n (a + b K): the constants are fitted to 68 products of 1 to
-// 8192 rows, 74 to 16384 columns and K of 75 to 15814, of whole and odd sizes, each timed
-// in every form, and then moved to where the choice loses least: the form that they make
-// the fastest was 0.8% slower on average than the fastest one timed, 18% in the worst case
-// (8192 x 8192 x 128). 256 x 256 tiles count their last round by its parts (int8Rounds,
-// which those times are without). What the forms are for, us
-// 256x256 | 256x128 | 128x128 | its pair | 64x128 | 64x64 | few 16x16 | 32x16 | 32x32:
+// With n the tiles of the busiest CU, the time of a launch is about c + n (a + b K): within 8
+// to 14% by form (one standard deviation, the larger forms up to 13% too long on average) of
+// 620 products of 1 to 8192 rows, 74 to 16384 columns and K of 75 to 16384, of whole and odd
+// sizes, each timed in every form. By it the choice was 0.6% slower on average than the
+// fastest form timed, 16% in the worst case (2216 x 4158 x 256). For 16 x 16 tiles b = 0.43
+// instead of 0.31 changes 42 of those choices, 31 of them for the worse, by 4% on average (2 x
+// 8576 x 2520 7.3 us instead of 5.6), though some gain (8 x 12288 x 4096 9.6 instead of 10.2).
+// 256 x 256 tiles count their last round by its parts (int8Rounds). What the forms are for,
+// us 256x256 | 256x128 | 128x128 | its pair | 64x128 | 64x64 | few 16x16 | 32x16 | 32x32:
 //   4096 x 4096 x 4096   52.3 | 58.8 | 75.0 | 61.9 | 80.8 | 98.3 | - | - | -
 //   2319 x 1792 x 6784   64.1 | 33.8 | 49.1 | 37.8 | 45.6 | 48.8 | - | - | -
 //   2048 x 2048 x 2048   25.2 | 16.0 | 11.6 | 13.6 | 13.0 | 15.6 | 86 | 93 | 59
@@ -49,7 +50,7 @@ struct FormCost {
 constexpr FormCost kForm[kForms] = {
     {256, 256, 0, 750, 856},  {256, 128, 0, 680, 455}, {128, 128, 50, 400, 327},
     {128, 128, 190, 220, 372}, {64, 128, 200, 150, 223}, {64, 64, 210, 120, 136},
-    {16, 16, 170, 70, 43},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
+    {16, 16, 170, 70, 31},    {32, 16, 100, 170, 52},  {32, 32, 80, 200, 73},
 };
 
 // A grid's work-items fit 32 bits, its tiles the kernels' divisions, and neither gains more

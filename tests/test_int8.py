@@ -111,3 +111,14 @@ def test_form_of_sizes_without_a_product():
 def test_row_stride(cols, stride):
     assert I.lib().ridge_int8_row_stride(cols) == stride
     assert I.empty(2, cols, device="cpu")[0].stride(0) == stride
+
+
+# A few tokens against wide weights, us in tiles of 16x16 | 64x64 whose workgroups have K alone.
+@pytest.mark.parametrize("M,N,K", [
+    (2, 8576, 2520),    # 5.6 | 7.3
+    (2, 8960, 3412),    # 6.5 | 7.9
+    (3, 9728, 3467),    # 7.1 | 8.6
+    (3, 11008, 1408),   # 5.1 | 5.6
+])
+def test_few_tokens_take_the_tiles_that_share_k(M, N, K):
+    assert I.lib().ridge_int8_gemm_form(M, N, K) == 6
