@@ -77,18 +77,14 @@ inline Int8Args<PACKED> int8Args(const Int8Operands& p, const Int8Sizes& s) {
     }
 }
 
-// Where chunk q = row * CPR + c of a tile lies in LDS (an involution). LDS serves a
-// fragment's read 16 lanes at a time, lanes {0-3, 12-15, 20-27} and {4-11, 16-19, 28-31}
-// of each half of the wave: 16 rows of the tile, half of them at one chunk and half at the
-// next, which have to lie in 16 different 16-byte slots of a 256-byte line. The mask
-// repeats every 16 rows, so fragments 16 rows apart are a constant distance apart.
-// (Counted conflicts: none. The mask that would serve lanes 0-15 at once, (row / 4) % 4 at
-// 4 chunks a row, made every read take two turns: 256 x 256 x 64 tiles of K = 4096 on an
-// uncrowded chip 45.1 us against 40.2.)
-template <int CPR>
-__device__ __forceinline__ int swizzleRows(int q) {
-    return q ^ (CPR == 4 ? (q / 8) % 8 : (q / 16) % CPR);
-}
+// Where chunk q = 8 row + c of a tile whose rows are 8 chunks lies in LDS (an involution). LDS
+// serves a fragment's read 16 lanes at a time, lanes {0-3, 12-15, 20-27} and {4-11, 16-19,
+// 28-31} of each half of the wave: 16 rows of the tile, half of them at one chunk and half at
+// the next, which have to lie in 16 different 16-byte slots of a 256-byte line. The mask
+// repeats every 16 rows, so fragments 16 rows apart are a constant distance apart. (Counted
+// conflicts: none.)
+constexpr int kChunksPerRow = 8;
+__device__ __forceinline__ int swizzleRows(int q) { return q ^ (q / 16) % kChunksPerRow; }
 
 // BK counts bytes, which are elements.
 template <int BM_, int BN_, int BK_, int WM_, int WN_, int STAGES_>
@@ -111,7 +107,7 @@ struct Int8Traits {
     static constexpr int kLoadsPerTile = kPerWaveA + kPerWaveB;
 
     static_assert(BM % WM == 0 && BN % WN == 0 && WM % kMfmaM == 0 && WN % kMfmaN == 0, "tiles must nest");
-    static_assert(BK == 64 || BK == 128 || BK == 256, "the swizzle is derived for rows of 4, 8 and 16 chunks");
+    static_assert(CPR == kChunksPerRow, "the swizzle is derived for rows of 8 chunks");
     static_assert(kBytesA % (1024 * kWaves) == 0 && kBytesB % (1024 * kWaves) == 0, "loads must split over the waves");
     static_assert((kStages - 1) * kLoadsPerTile < 64, "in-flight loads exceed the vmcnt counter");
     static_assert(kLdsBytes <= 163840, "LDS is 160 KiB per workgroup on gfx950");
@@ -189,8 +185,8 @@ struct Int8Block {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int c = 4 * ks + lane / 16;
-            rdA[ks] = swizzleRows<CPR>((waveM * T::WM + lane % 16) * CPR + c) * 16;
-            rdB[ks] = T::kRegionA + swizzleRows<CPR>((waveN * T::WN + lane % 16) * CPR + c) * 16;
+            rdA[ks] = swizzleRows((waveM * T::WM + lane % 16) * CPR + c) * 16;
+            rdB[ks] = T::kRegionA + swizzleRows((waveN * T::WN + lane % 16) * CPR + c) * 16;
         }
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm)
@@ -213,7 +209,7 @@ struct Int8Block {
 
     // The chunk of a tile that this lane's share of the wave's load i fetches.
     __device__ __forceinline__ int chunkOf(int i) const {
-        return swizzleRows<CPR>((i * T::kWaves + wave) * 64 + lane);
+        return swizzleRows((i * T::kWaves + wave) * 64 + lane);
     }
 
     // Byte offset of a load's chunk from the tile's first row. Strides are below 2^23 and
@@ -233,7 +229,7 @@ struct Int8Block {
         const int last = WHOLE || kTile < numFull ? CPR - 1 : (z.K - 1) / 16 - kTile * CPR;
         auto past = [&](int i) {
             if constexpr (WHOLE) return 0u;
-            const int chunk = swizzleRows<CPR>((i * T::kWaves + wave) * 64 + laneAgain()) % CPR;
+            const int chunk = swizzleRows((i * T::kWaves + wave) * 64 + laneAgain()) % CPR;
             return (uint32_t)max(chunk - last, 0) * 16u;
         };
 #pragma unroll
@@ -640,6 +636,7 @@ struct Int8FewTraits {
     static constexpr int kThreads = kWaves * kWaveSize;
     static constexpr int kPiece = 128;                       // bytes of a row a wave takes at once
     static constexpr int CPR = kPiece / 16;
+    static_assert(CPR == kChunksPerRow, "the swizzle is derived for rows of 8 chunks");
     static constexpr int KS = kPiece / kInt8MfmaK;
     static constexpr int kTiles = TM * TN;                   // 16 x 16 tiles of C
     static constexpr int kPieceBytes = 16 * (TM + TN) * kPiece;
@@ -672,7 +669,7 @@ void int8FewKernel(Int8Args<true> args) {
     uint32_t off[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-        const int q = swizzleRows<CPR>(64 * i + lane), row = q / CPR;
+        const int q = swizzleRows(64 * i + lane), row = q / CPR;
         off[i] = (uint32_t)(q % CPR) * 16u + (i < 2 * TN ? (uint32_t)min(row, z.N - 1 - col0) * (uint32_t)z.ldb
                                                          : (uint32_t)min(row - 16 * TN, z.M - 1 - row0) * (uint32_t)z.lda);
     }
@@ -682,7 +679,7 @@ void int8FewKernel(Int8Args<true> args) {
         const int64_t at = (int64_t)piece * T::kPiece;
         // How far behind the last chunk of K this lane's chunk is.
         const int last = min((z.K - 1) / 16 - piece * CPR, CPR - 1);
-        auto past = [&](int i) { return (uint32_t)max(swizzleRows<CPR>(64 * i + lane) % CPR - last, 0) * 16u; };
+        auto past = [&](int i) { return (uint32_t)max(swizzleRows(64 * i + lane) % CPR - last, 0) * 16u; };
 #pragma unroll
         for (int i = 0; i < L; ++i)
             globalLoadLds16((i < 2 * TN ? gB : gA) + at, off[i] - past(i),
@@ -696,7 +693,7 @@ void int8FewKernel(Int8Args<true> args) {
 
     const int mine = (pieces - wave + T::kWaves - 1) / T::kWaves;   // this wave's pieces; none or less: 0
     const RIDGE_LDS_AS char* const own = (const RIDGE_LDS_AS char*)(lds) + wave * T::kWaveBytes;
-    const int rd = swizzleRows<CPR>(r16 * CPR + g) * 16;             // k-step 0; step ks flips chunk bit 2
+    const int rd = swizzleRows(r16 * CPR + g) * 16;             // k-step 0; step ks flips chunk bit 2
     staticFor<STAGES>([&](auto sC) {
         if (sC.value < mine) issue(wave + sC.value * T::kWaves, sC.value);
     });

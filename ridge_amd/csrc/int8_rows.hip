@@ -142,10 +142,10 @@ struct NormArgs<false> {
     __device__ int64_t ldResidualOutOf() const { return ldResidualOut; }
 };
 
-// e^x as 2^power times what is returned, by the usual reduction of the argument: x log2(e) in
-// two f32 parts, the power the whole number next to it, and what is left for the exponential's
-// instruction. Its steps are not to be contracted: high - n in one step with its product would
-// hold the part that low adds.
+// e^x as 2^power times what is returned, the argument reduced as Cody and Waite do: x log2(e)
+// in two f32 parts, the power the whole number next to it, and what is left for the
+// exponential's instruction. Its steps are not to be contracted: high - n in one step with its
+// product would hold the part that low adds.
 __device__ __forceinline__ float exponentialParts(float x, int& power) {
 #pragma clang fp contract(off)
     constexpr float kLog2e = 1.44269504088896341f, kRest = (float)(1.44269504088896341 - (double)kLog2e);

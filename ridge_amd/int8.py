@@ -129,6 +129,7 @@ def dequantize(q, scale, dtype=None, out=None, stream=None):
 
 def gemm(a, a_scale, b, b_scale, bias=None, dtype=None, out=None, stream=None):
     """out[m, n] = (sum over k of a[m, k] b[n, k]) * a_scale[m] * b_scale[n] + bias[n].
-    The sum is exact (K at most MAX_K), the rest is computed in 32 bits and rounded once
-    to `dtype` (out's, or float16), which is bias's type too."""
+    The sum is exact (K at most MAX_K, rows of a and b less than MAX_STRIDE apart), the
+    rest is computed in 32 bits and rounded once to `dtype` (out's, or float16), which is
+    bias's type too."""
     return (_native or _load()).gemm(a, a_scale, b, b_scale, bias, dtype, out, stream)
