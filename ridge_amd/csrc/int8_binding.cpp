@@ -2,7 +2,7 @@
 // arguments, the allocation of results and the current stream behind ridge_amd.int8.
 //
 // Native because the calls are short: a decoding step's norm runs 3 us on the GPU, and
-// checking its six tensors in Python took 6 us on the host (9.3 us a call, 3.6 so).
+// checking its six tensors in Python took 6 us on the host (9.3 us a call, 3.2 so).
 
 #include <Python.h>
 

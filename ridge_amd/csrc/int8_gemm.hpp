@@ -25,8 +25,8 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 constexpr int kInt8MfmaK = 64;   // k of one instruction
 
 // A launch's arguments. They are written to device memory before it, 64 bytes at a time:
-// a second write would cost 0.8 us of the host's time, which is what the shortest products
-// wait for. So where sizes allow (int8ArgsFit) they are packed into one: strides, multiples
+// a second write would cost up to 0.5 us of the host's time, which is what the shortest
+// products wait for. So where sizes allow (int8ArgsFit) they are packed into one: strides, multiples
 // of 16 below 2^23, in 19 bits each, K in 17, M and N in 16, ldc in 32.
 struct Int8Operands {
     const int8_t* A;

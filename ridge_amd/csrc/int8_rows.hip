@@ -3,9 +3,10 @@
 //
 // All three makers are one kernel around a different source of a row's f32 values: read
 // the row once, hold its values in registers, reduce the largest magnitude (and, for the
-// norm, the sum of squares) over the row's threads, round and write. Memory bounds them:
-// every input byte is read once and every output byte written once, in 16-byte and
-// 8-byte pieces a lane.
+// norm, the sum of squares) over the row's threads, round and write. Memory bounds them
+// (16384 x 8192: the norm 5.4 TB/s, quantize 5.9): every input byte is read once and every
+// output byte written once, in 16-byte and 8-byte pieces a lane. The gated activation is
+// bound by its arithmetic, 33 vector instructions an element (4096 x 16384 77 us).
 //
 // A norm needs one reduction, not two: the sum of squares and the largest |s w| are taken
 // together, because the reciprocal root that multiplies a whole row moves out of the
@@ -92,8 +93,8 @@ __device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], co
 }
 
 // A launch's arguments. They are written to device memory before it, 64 bytes at a time:
-// a kernel that takes more waits for a second write, 3.5 us of the host's time a call
-// instead of 2.7. What a kernel takes beyond these counts too: it must not ask for its
+// a kernel that takes more waits for a second write, up to 0.5 us a call (a norm of 2 x 4096
+// in a sequence 3.5 us, of rows apart 3.8 to 3.9). What a kernel takes beyond these counts too: it must not ask for its
 // grid's size.
 struct RowArgs {
     const void* x;
@@ -406,8 +407,8 @@ void dequantizeKernel(const int8_t* q, int64_t ldq, const float* scale, T* out, 
 
 // 16- and 32-bit matrices of this size and more are read and written past the caches: who
 // comes next would not find them there, and the 8-bit rows, which the next product reads,
-// stay. us, cached | past the caches, the norm and a reader of its rows: 16384 x 8192 249 |
-// 225, 4096 x 16384 137 | 123, 2048 x 4096 18.7 | 21.0.
+// stay. us, cached | past the caches, the norm of bfloat16 and a reader of its rows: 16384 x
+// 8192 249 | 220, 4096 x 16384 137 | 123, 2048 x 4096 18.5 | 22.3.
 constexpr int64_t kStreamBytes = (int64_t)64 << 20;
 
 template <typename Source, int kThreads, int kVecs>
@@ -421,9 +422,9 @@ hipError_t launchRows(const typename Source::Args& a, hipStream_t stream) {
 // The threads of a row, by its length: as many as hold it in at most four vectors each. A
 // norm's 1024 threads have not got the registers for that: it reads rows of more than
 // 16384 columns twice. Few rows leave CUs to spare and take more threads and fewer vectors
-// each, which also is less code to run through once: us in a graph, silu as for many rows
-// | so: 13 x 2048 4.2 | 2.7, 4 x 8192 4.5 | 4.0, 500 x 8192 7.2 | 6.8; 16000 x 2048 39.4 |
-// 41.8. Not the norm, whose sum would be added up in another order: a row's result must
+// each, which also is less code to run through once: us in a graph, silu of float16 as for
+// many rows | so: 13 x 2048 4.4 | 3.0, 4 x 8192 4.6 | 4.1, 500 x 8192 7.6 | 7.4; but 600 x 8192
+// 9.3 | 9.7, 4000 x 4096 18.9 | 22.9, 8000 x 600 10.5 | 13.7. Not the norm, whose sum would be added up in another order: a row's result must
 // not depend on how many rows there are.
 constexpr int kFewRows = 512;
 template <typename Source>
