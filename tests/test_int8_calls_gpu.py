@@ -276,3 +276,13 @@ def test_feed_forward_command_fails_on_results_that_are_not_numbers(monkeypatch)
     assert int8_mlp.main(args) == 0
     monkeypatch.setattr(int8_mlp, "random_block", broken)
     assert int8_mlp.main(args) == 1
+
+
+def test_ordinary_buffers_are_written_in_inference_mode():
+    x, w, q, s, bias = _operands()
+    out, rows, total = torch.zeros((4, 4), dtype=torch.float16, device=DEV), I.empty(4, 64), torch.zeros_like(x)
+    with torch.inference_mode():
+        I.gemm(q, s, q, s, out=out)
+        I.rms_norm(x, w, residual=x, residual_out=total, out=rows)
+        new = I.gemm(q, s, q, s)
+    assert new.is_inference() and torch.equal(out, new) and torch.equal(total, x + x)
