@@ -13,6 +13,7 @@
 // maximum, and out of the quotients that are rounded.
 
 #include "int8_launch.hpp"
+#include "int8_values.hpp"
 #include "ridge_int8.h"
 
 #include <hip/hip_runtime.h>
@@ -26,70 +27,22 @@ namespace {
 constexpr int kWave = 64;
 constexpr int kVec = 8;  // elements a lane loads at once: 16 bytes of a 16-bit type
 
-// n elements of a row at once, with the alignment of one: rows may start anywhere, and
-// global accesses of any alignment are one instruction here. What a row has behind its
-// last whole vector goes one element a lane.
-template <typename T, int n>
-struct Memory {
-    typedef T Vec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
-};
+using ridge::kLift;
+using ridge::kSmallRow;
+using ridge::loadRow;
+using ridge::magnitude;
+using ridge::Step;
+using ridge::stepOf;
+using ridge::storeRounded;
+using ridge::storeRow;
+
 typedef signed char Bytes8 __attribute__((ext_vector_type(kVec), aligned(8)));
-
-// STREAM: past the caches. A template argument, because the compiler merges the two
-// accesses of a run-time choice and drops the hint.
-template <bool STREAM, int n, typename T>
-__device__ __forceinline__ void loadRow(const T* at, float (&v)[n]) {
-    typedef typename Memory<T, n>::Vec Vec;
-    Vec m;
-    if constexpr (STREAM && n > 1) {
-        m = __builtin_nontemporal_load((const Vec*)at);
-    } else {
-        m = *(const Vec*)at;
-    }
-#pragma unroll
-    for (int e = 0; e < n; ++e) v[e] = (float)m[e];
-}
-
-template <bool STREAM, int n, typename T>
-__device__ __forceinline__ void storeRow(T* at, const float (&v)[n]) {
-    typedef typename Memory<T, n>::Vec Vec;
-    Vec m;
-#pragma unroll
-    for (int e = 0; e < n; ++e) m[e] = (T)v[e];
-    if constexpr (STREAM && n > 1) {
-        __builtin_nontemporal_store(m, (Vec*)at);
-    } else {
-        *(Vec*)at = m;
-    }
-}
 
 // A value that all lanes of the wave have, in a scalar register (a wave is never of two rows).
 // It saves the norm, and rows read twice, a wave a SIMD (16384 x 8192 with dequantize 242 us
 // without it, 226 with it); the gated kernels of 4 vectors lose one by it.
 __device__ __forceinline__ float uniform(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
-}
-
-// A row's 127th: the largest magnitude over 127 is whole + rest to about 46 bits.
-struct Step {
-    float whole, rest, inverse;   // and 1 / whole
-};
-
-// Nearest whole numbers (halves to even) of v / step. The quotient is v * (1 / step) corrected
-// once by its remainder, which is exact but for what `rest` lacks, so that a quotient of n + 1/2
-// comes out as that: by the step's f32 alone, half of a row's largest value (63.5) went to 63
-// or to 64 as the step was rounded. Adding 1.5 * 2^23 leaves the whole number in the low bits.
-// A row whose scale is not finite gets bytes that mean nothing.
-template <int n>
-__device__ __forceinline__ void storeRounded(int8_t* at, const float (&v)[n], const Step& step) {
-    typename Memory<signed char, n>::Vec b;
-#pragma unroll
-    for (int e = 0; e < n; ++e) {
-        float t = v[e] * step.inverse;
-        t = fmaf(fmaf(-t, step.rest, fmaf(-t, step.whole, v[e])), step.inverse, t);
-        b[e] = (signed char)__float_as_uint(t + 12582912.0f);
-    }
-    *(typename Memory<signed char, n>::Vec*)at = b;
 }
 
 // A launch's arguments. They are written to device memory before it, 64 bytes at a time:
@@ -270,9 +223,6 @@ struct Normed {
     }
 };
 
-// Magnitudes are compared as integers: that is their order, and a NaN is above all.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 // Sum and maximum over the kThreads threads of a row, in an order that depends on
 // nothing but kThreads.
 template <int kThreads, bool kSum>
@@ -302,8 +252,6 @@ __device__ __forceinline__ void reduceRow(float& sum, uint32_t& top) {
 }
 
 constexpr int64_t kMostBlocks = 1 << 20;  // of a grid: its blocks walk the rows behind them
-
-constexpr float kLift = 0x1p64f, kSmallRow = 0x1p-60f;
 
 // One row a kThreads threads. kVecs vectors a thread hold the row; with kVecs = 0 a row
 // of any length is read twice.
@@ -347,20 +295,9 @@ void makeRowsKernel(typename Source::Args a) {
             root = squares <= FLT_MAX ? 1.0f / sqrtf(squares / (float)a.cols + a.eps) : NAN;
         }
         const float most = kScalar ? uniform(__uint_as_float(top)) : __uint_as_float(top);
-        float scale = most * root / 127.0f;
-        // q is value / (most / 127): the root is in both and cancels. Rows of small values are
-        // lifted by a power of two, so that the step's rest stays a normal number.
         const bool small = most < kSmallRow;
-        const float lifted = small ? most * kLift : most;
-        Step step;
-        step.whole = lifted / 127.0f;
-        step.rest = fmaf(-127.0f, step.whole, lifted) / 127.0f;
-        if (scale < FLT_MIN) {  // a NaN stays one
-            scale = FLT_MIN;
-            step.whole = (small ? FLT_MIN * kLift : FLT_MIN) / root;
-            step.rest = 0.0f;
-        }
-        step.inverse = 1.0f / step.whole;
+        float scale;
+        Step step = stepOf(most, root, scale);
         if constexpr (kScalar) step = {uniform(step.whole), uniform(step.rest), uniform(step.inverse)};
         if (lane == 0) a.scale[row] = scale;
         int8_t* const q = a.q + row * a.ldq();
