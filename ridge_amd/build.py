@@ -7,6 +7,9 @@ Outputs (git-ignored, shipped with the tree):
     ridge_amd/lib/libridge_gemm.so   GEMM kernel table, fills, hipBLASLt comparator
     ridge_amd/lib/libridge_int8.so   the 8-bit operators (include/ridge_int8.h)
     ridge_amd/lib/_ridge_int8.so     their calls on torch's tensors, a Python extension
+    ridge_amd/lib/libridge_attention.so   the operators around an 8-bit cache
+                                     (include/ridge_attention.h)
+    ridge_amd/lib/_ridge_attention.so     their calls on torch's tensors
     ridge_amd/lib/libridge_model.so  the cost model behind a C ABI
     ridge_amd/bin/ridge-predict      the model CLI (reference tools/ridge-predict.cpp)
     ridge_amd/bin/ridge-check        correctness + throughput harness (bench/check-gemm.cu)
@@ -194,20 +197,21 @@ def build_gemm(gate=True):
 
 
 INT8_SRCS = ["int8_rows.hip", "int8_gemm.hip"]
+ATTENTION_SRCS = ["attention_rope.hip", "attention_cache.hip", "attention_attend.hip"]
 
 
-def build_int8(gate=True):
-    """libridge_int8.so. No kernel of it may use scratch memory."""
+def _build_operators(srcs, name, gate):
+    """lib<name>.so of these sources. No kernel of it may use scratch memory."""
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIB, exist_ok=True)
-    objs, spilling = [os.path.join(BUILD, src.replace(".hip", ".o")) for src in INT8_SRCS], 0
+    objs, spilling = [os.path.join(BUILD, src.replace(".hip", ".o")) for src in srcs], 0
 
     def compiled(src, o):
         return _run([HIPCC] + LIB_HIP_FLAGS + ["-Rpass-analysis=kernel-resource-usage", "-x", "hip", "-c",
                                                os.path.join(CSRC, src), "-o", o], capture=True)
-    with ThreadPoolExecutor(len(INT8_SRCS)) as pool:
-        remarks = list(pool.map(compiled, INT8_SRCS, objs))
-    for src, text in zip(INT8_SRCS, remarks):
+    with ThreadPoolExecutor(len(srcs)) as pool:
+        remarks = list(pool.map(compiled, srcs, objs))
+    for src, text in zip(srcs, remarks):
         kernels = kernel_remarks(text)
         bad = {k: r for k, r in kernels.items() if r["scratch"] or r["vgpr_spill"] or r["sgpr_spill"]}
         print("  %s: %d kernels, %d spilling" % (src, len(kernels), len(bad)))
@@ -215,33 +219,46 @@ def build_int8(gate=True):
             print("    SPILL %s: %s" % (k, r))
         spilling += len(bad)
     if spilling and gate:
-        raise SystemExit("spill gate: %d 8-bit kernel(s) use scratch" % spilling)
-    so = os.path.join(LIB, "libridge_int8.so")
+        raise SystemExit("spill gate: %d kernel(s) of lib%s.so use scratch" % (spilling, name))
+    so = os.path.join(LIB, "lib%s.so" % name)
     _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", so + ".tmp"] + objs)
     os.replace(so + ".tmp", so)
-    build_int8_binding()
     return so
 
 
-def build_int8_binding():
-    """_ridge_int8.so: host code over libridge_int8.so, torch's tensors and its streams. None
-    where there is no torch: the C ABI and everything else are built without."""
+def _build_binding(src, name):
+    """_<name>.so: host code over lib<name>.so, torch's tensors and its streams. None where
+    there is no torch: the C ABI and everything else are built without."""
     import sysconfig
     try:
         import torch
     except ImportError:
-        print("  no torch: _ridge_int8.so is not built")
+        print("  no torch: _%s.so is not built" % name)
         return None
     torch_dir = os.path.dirname(torch.__file__)
-    so = os.path.join(LIB, "_ridge_int8.so")
+    so = os.path.join(LIB, "_%s.so" % name)
     _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
           "-I" + INCLUDE, "-isystem", os.path.join(torch_dir, "include"), "-isystem",
           os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), "-isystem", "/opt/rocm/include",
-          "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "int8_binding.cpp"), "-o", so + ".tmp",
-          "-L" + LIB, "-lridge_int8", "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+          "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, src), "-o", so + ".tmp",
+          "-L" + LIB, "-l" + name, "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
           "-lc10_hip", "-Wl,-rpath,$ORIGIN"])
     os.replace(so + ".tmp", so)
+    return so
+
+
+def build_int8(gate=True):
+    """libridge_int8.so and its binding."""
+    so = _build_operators(INT8_SRCS, "ridge_int8", gate)
+    _build_binding("int8_binding.cpp", "ridge_int8")
+    return so
+
+
+def build_attention(gate=True):
+    """libridge_attention.so and its binding."""
+    so = _build_operators(ATTENTION_SRCS, "ridge_attention", gate)
+    _build_binding("attention_binding.cpp", "ridge_attention")
     return so
 
 
@@ -303,13 +320,15 @@ def build_oracle():
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--no-gate", action="store_true", help="do not fail on spilling variants")
-    ap.add_argument("--only", default="all", choices=["all", "gemm", "int8", "model", "tools", "oracle"])
+    ap.add_argument("--only", default="all", choices=["all", "gemm", "int8", "attention", "model", "tools", "oracle"])
     args = ap.parse_args(argv)
     print("ridge_amd build (%s)" % ARCH, flush=True)
     if args.only in ("all", "gemm"):
         build_gemm(gate=not args.no_gate)
     if args.only in ("all", "int8"):
         build_int8(gate=not args.no_gate)
+    if args.only in ("all", "attention"):
+        build_attention(gate=not args.no_gate)
     if args.only in ("all", "model"):
         build_model()
     if args.only in ("all", "tools"):

@@ -1,0 +1,171 @@
+// attention_cache.hip -- rows written to the 8-bit cache and read back, for the C ABI in
+// include/ridge_attention.h.
+//
+// A row (a token's key or value of one head) is held by the lanes that its columns fill, 8
+// values each: one read of it, its largest magnitude by exchanges between those lanes, and
+// the rounding that every 8-bit row of the framework has. Memory bounds both directions.
+
+#include "attention_common.hpp"
+
+namespace {
+
+using ridge::kBlock;
+using ridge::kWave;
+
+constexpr int kVec = 8;   // columns of a lane
+
+struct CacheArgs {
+    ridge_attention_cache_t cache;
+    const int32_t* slots;
+    void* k;
+    void* v;
+    int64_t kToken, kHead, vToken, vHead;
+    int32_t tokens, each, chunks;   // a wave's heads at a time and the parts that a token's are cut into
+};
+
+// n values of a head at once, the last few of its columns one at a time.
+template <typename T>
+__device__ __forceinline__ void loadPart(const T* at, int n, float (&x)[kVec]) {
+    if (n >= kVec) return ridge::loadRow<false>(at, x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[e] = e < n ? (float)at[e] : 0.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ void storePart(T* at, int n, const float (&x)[kVec]) {
+    if (n >= kVec) return ridge::storeRow<false>(at, x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e)
+        if (e < n) at[e] = (T)x[e];
+}
+
+// Calls f(token, its slot, head) for each head whose key and value this lane has a part of.
+template <int LANES, typename F>
+__device__ __forceinline__ void walk(const CacheArgs& a, F&& f) {
+    constexpr int kHeads = kWave / LANES;
+    ridge::walkParts(a.tokens, a.chunks, [&](int64_t token, int part) {
+        const int32_t slot = a.slots[token];
+        const int from = part * a.each * kHeads + (int)(threadIdx.x % kWave) / LANES;
+        for (int i = 0; i < a.each; ++i) {
+            const int head = from + i * kHeads;
+            if (head < a.cache.heads) f(token, slot, head);
+        }
+    });
+}
+
+// Where a slot's row of a head and its scale are, from the beginning of k or v.
+struct Place {
+    int64_t row, scale;
+    __device__ Place(const ridge_attention_cache_t& c, int32_t slot, int head) {
+        const int32_t page = slot / c.pageSize, at = slot - page * c.pageSize;
+        row = page * c.pageStride + head * c.headStride + at * c.tokenStride;
+        scale = page * c.scalePage + head * c.scaleHead + at;
+    }
+};
+
+__device__ __forceinline__ bool holds(const ridge_attention_cache_t& c, int32_t slot) {
+    return slot >= 0 && slot / c.pageSize < c.pages;
+}
+
+// A row's 8 bits out of this lane's part of it, and its scale.
+template <int LANES>
+__device__ __forceinline__ void storeRow8(float (&x)[kVec], int n, int8_t* at, float* scaleAt) {
+    uint32_t top = 0;
+#pragma unroll
+    for (float value : x) top = max(top, ridge::magnitude(value));
+    const float most = __uint_as_float(ridge::mostOf<LANES>(top));
+    float scale;
+    const ridge::Step step = ridge::stepOf(most, 1.0f, scale);
+    const float lift = most < ridge::kSmallRow ? ridge::kLift : 1.0f;
+#pragma unroll
+    for (float& value : x) value *= lift;
+    if (n >= kVec) {
+        ridge::storeRounded(at, x, step);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            const float one[1] = {x[e]};
+            if (e < n) ridge::storeRounded(at + e, one, step);
+        }
+    }
+    if (threadIdx.x % LANES == 0) *scaleAt = scale;
+}
+
+template <typename T, int LANES>
+__global__ __launch_bounds__(kBlock) void writeKernel(CacheArgs a) {
+    const int col = threadIdx.x % LANES * kVec, n = a.cache.dim - col;
+    walk<LANES>(a, [&](int64_t token, int32_t slot, int head) {
+        if (!holds(a.cache, slot)) return;
+        float k[kVec] = {}, v[kVec] = {};
+        if (n > 0) {
+            loadPart((const T*)a.k + token * a.kToken + head * a.kHead + col, n, k);
+            loadPart((const T*)a.v + token * a.vToken + head * a.vHead + col, n, v);
+        }
+        const Place to(a.cache, slot, head);
+        storeRow8<LANES>(k, n, a.cache.k + to.row + col, a.cache.kScale + to.scale);
+        storeRow8<LANES>(v, n, a.cache.v + to.row + col, a.cache.vScale + to.scale);
+    });
+}
+
+template <typename T, int LANES>
+__global__ __launch_bounds__(kBlock) void readKernel(CacheArgs a) {
+    typedef signed char Bytes __attribute__((ext_vector_type(kVec), aligned(8)));
+    const int col = threadIdx.x % LANES * kVec, n = a.cache.dim - col;
+    walk<LANES>(a, [&](int64_t token, int32_t slot, int head) {
+        if (n <= 0) return;
+        float k[kVec], v[kVec];
+        if (holds(a.cache, slot)) {
+            const Place from(a.cache, slot, head);
+            const Bytes kb = *(const Bytes*)(a.cache.k + from.row + col);   // rows are readable to 16
+            const Bytes vb = *(const Bytes*)(a.cache.v + from.row + col);
+            const float kScale = a.cache.kScale[from.scale], vScale = a.cache.vScale[from.scale];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) k[e] = (float)kb[e] * kScale, v[e] = (float)vb[e] * vScale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) k[e] = v[e] = slot < 0 ? 0.0f : NAN;
+        }
+        storePart((T*)a.k + token * a.kToken + head * a.kHead + col, n, k);
+        storePart((T*)a.v + token * a.vToken + head * a.vHead + col, n, v);
+    });
+}
+
+template <typename Kernel>
+hipError_t launchRows(Kernel kernel, CacheArgs a, int lanes, hipStream_t stream) {
+    const int rows = kWave / lanes;
+    const ridge::Cut cut(a.tokens, (a.cache.heads + rows - 1) / rows);
+    a.each = cut.each, a.chunks = cut.chunks;
+    return ridge::launchKernel(kernel, cut.blocks, kBlock, stream, a);
+}
+
+template <typename T>
+hipError_t launchTyped(const CacheArgs& a, bool write, hipStream_t s) {
+    if (a.cache.dim <= 8 * kVec) return launchRows(write ? writeKernel<T, 8> : readKernel<T, 8>, a, 8, s);
+    if (a.cache.dim <= 16 * kVec) return launchRows(write ? writeKernel<T, 16> : readKernel<T, 16>, a, 16, s);
+    return launchRows(write ? writeKernel<T, 32> : readKernel<T, 32>, a, 32, s);
+}
+
+hipError_t launchCache(const ridge_attention_cache_t* cache, const int32_t* slots, const ridge_attention_heads_t* k,
+                       const ridge_attention_heads_t* v, int type, int64_t tokens, bool write, void* stream) {
+    if (!ridge::isType(type) || !ridge::cacheFits(cache) || !ridge::headsFit(k, type, tokens) || !ridge::headsFit(v, type, tokens) ||
+        k->heads != cache->heads || v->heads != cache->heads || tokens < 0 || tokens > INT32_MAX)
+        return hipErrorInvalidValue;
+    if (tokens == 0) return hipSuccess;
+    if (!ridge::aligned(slots, 4)) return hipErrorInvalidValue;
+    const CacheArgs a = {*cache, slots, k->at, v->at, k->token, k->head, v->token, v->head, (int32_t)tokens, 0, 0};
+    return ridge::typed(type, [&](auto element) { return launchTyped<decltype(element)>(a, write, (hipStream_t)stream); });
+}
+
+}  // namespace
+
+extern "C" int ridge_attention_write(const ridge_attention_cache_t* cache, const int32_t* slots,
+                                     const ridge_attention_heads_t* k, const ridge_attention_heads_t* v, int type,
+                                     int64_t tokens, void* stream) {
+    return launchCache(cache, slots, k, v, type, tokens, true, stream);
+}
+
+extern "C" int ridge_attention_read(const ridge_attention_cache_t* cache, const int32_t* slots,
+                                    const ridge_attention_heads_t* k, const ridge_attention_heads_t* v, int type,
+                                    int64_t tokens, void* stream) {
+    return launchCache(cache, slots, k, v, type, tokens, false, stream);
+}
