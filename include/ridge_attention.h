@@ -45,7 +45,7 @@ typedef struct {
 
 /* The cache: k's byte (page, h, t, d) is k[page * pageStride + h * headStride + t * tokenStride
  * + d], its scale kScale[page * scalePage + h * scaleHead + t], and v's likewise. Strides of
- * rows are in bytes and multiples of 16, those of scales in elements and multiples of 4, and
+ * rows are in bytes and multiples of 16, tokenStride below 2^27, those of scales in elements and multiples of 4, and
  * all four pointers multiples of 16. A row's last 16 bytes are readable. */
 typedef struct {
     int8_t* k;

@@ -160,6 +160,7 @@ struct Cache {
             if (levels[i].stride % 16) refuse("the cache's rows must start at multiples of 16 bytes (as those of empty_cache() do)");
             bytes += (levels[i].count - 1) * levels[i].stride;
         }
+        if (levels[2].stride >= (int64_t)1 << 27) refuse("the rows of a page lie 2^27 bytes apart or more");
         ref.pageStride = levels[0].stride, ref.headStride = levels[1].stride, ref.tokenStride = levels[2].stride;
         for (const at::Tensor* s : {&kScale, &vScale}) {
             if (s->scalar_type() != at::kFloat || s->device() != device() || s->layout() != at::kStrided || s->dim() != 3 ||

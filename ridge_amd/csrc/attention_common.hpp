@@ -37,7 +37,8 @@ inline bool cacheFits(const ridge_attention_cache_t* c) {
         if (stride < 0 || stride % 16) return false;
     for (int64_t stride : {c->scalePage, c->scaleHead})
         if (stride < 0 || stride % 4) return false;
-    return c->dim >= 1 && c->dim <= RIDGE_ATTENTION_MAX_DIM && c->heads >= 1 && c->heads <= 65535 && c->pageSize >= 16 &&
+    // A block of 16 rows is reached by 32-bit offsets.
+    return c->tokenStride < (int64_t)1 << 27 && c->dim >= 1 && c->dim <= RIDGE_ATTENTION_MAX_DIM && c->heads >= 1 && c->heads <= 65535 && c->pageSize >= 16 &&
            c->pageSize % 16 == 0 && c->pages >= 1 && c->pages <= RIDGE_ATTENTION_MAX_SLOTS / c->pageSize;
 }
 

@@ -110,6 +110,7 @@ def test_no_tokens_and_no_heads_are_calls_that_do_nothing():
 BAD_CACHES = {
     "k": dict(k=None), "v off": dict(v=P + 8), "kScale": dict(kScale=P + 4), "vScale": dict(vScale=None),
     "page stride": dict(pageStride=2056), "head stride": dict(headStride=-1024), "token stride": dict(tokenStride=72),
+    "rows far apart": dict(tokenStride=1 << 27),
     "scale page": dict(scalePage=33), "scale head": dict(scaleHead=-16), "pages": dict(pages=0),
     "many pages": dict(pages=1 << 27), "page size": dict(pageSize=24), "small pages": dict(pageSize=0),
     "heads": dict(heads=0), "many heads": dict(heads=65536), "dim": dict(dim=0), "wide": dict(dim=257),
@@ -143,6 +144,8 @@ def test_rows_are_refused(what, changes):
     ("pages each", dict(each=-1)), ("many pages", dict(each=1 << 27)), ("lengths", dict(lengths=None)),
     ("scale", dict(scale=float("inf"))), ("scale nan", dict(scale=float("nan"))), ("window", dict(window=-1)),
     ("lse off", dict(lse=P + 2)), ("type", dict(type=5)), ("batch", dict(batch=-1)), ("many", dict(batch=1 << 30)),
+    ("no workspace", dict(each=100, workspace=None)), ("a small workspace", dict(each=100, bytes=3 * 4 * 4 * 66 * 4 - 1)),
+    ("a workspace off", dict(each=100, workspace=P + 8)),
 ])
 def test_attend_refuses(what, changes):
     args = dict(dict(q=_heads(), cache=_cache(), pages=P, stride=4, each=4, lengths=P, scale=0.125, window=0, out=_heads(),
@@ -152,7 +155,9 @@ def test_attend_refuses(what, changes):
 
 def test_workspace():
     size = A.lib().ridge_attention_workspace
-    assert size(3, 8, 2, 128, 4, 16) >= 0
+    assert size(3, 8, 2, 128, 32, 16) == 0       # one part of 512 tokens
+    assert size(3, 8, 2, 128, 33, 16) == 3 * 8 * 2 * 130 * 4
+    assert size(3, 8, 2, 128, 1 << 20, 16) == 3 * 8 * 64 * 130 * 4
     for bad in ((-1, 8, 2, 128, 4, 16), (1 << 31, 8, 2, 128, 4, 16), (3, 9, 2, 128, 4, 16), (3, 8, 0, 128, 4, 16),
                 (3, 8, 2, 0, 4, 16), (3, 8, 2, 300, 4, 16), (3, 8, 2, 128, -1, 16), (3, 8, 2, 128, 4, 17),
                 (3, 8, 2, 128, 1 << 27, 16)):
