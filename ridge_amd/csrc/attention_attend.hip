@@ -37,7 +37,6 @@ constexpr int kTile = 32;        // tokens of a wave at a time
 constexpr int kRound = kTile * kWavesPerBlock;
 constexpr int kLeastPart = 512;  // tokens of a part
 constexpr int kMostParts = 64;   // of a sequence: longer ones have longer parts
-constexpr uint32_t kRowOfBlocks = 1 << 20;   // of a grid, whose work-items along one direction fit 32 bits
 
 struct AttendArgs {
     const int8_t* k;
@@ -105,8 +104,9 @@ __device__ __forceinline__ Half2 halves(uint32_t high, uint32_t low, int hi, int
 }
 constexpr int kByteExponent = -9;
 
-// Two values in f16, and what they leave. The pair's instruction and the single value's round halves
-// differently: the empty statement has the compiler take the remainder of what was in fact rounded.
+// Two values in f16, and what they leave. The compiler may convert a product with one rounding at one
+// place and with two at another: the empty statement has the remainder taken of what was in fact
+// rounded (without it a few heads in 1000 had a p off by 2^-11).
 __device__ __forceinline__ void split(float a, float b, Half2& high, float& restA, float& restB) {
     uint32_t both = __builtin_bit_cast(uint32_t, Half2{(_Float16)a, (_Float16)b});
     asm("" : "+v"(both));
@@ -119,12 +119,20 @@ __device__ __forceinline__ Half8 join(Half2 a, Half2 b, Half2 c, Half2 d) {
     return Half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// Where a wave's 32 tokens are: two blocks of 16, each in one page. The same for all its lanes.
+struct Place {
+    int64_t rows[2], scales[2];   // from the beginning of k or v and of their scales
+    bool there[2];                // whether the page is one of the cache's: else it is the first one instead
+};
+
 // 32 tokens' operands of a lane. COLS: a head's columns, padded.
 template <int COLS>
 struct Tile {
-    static constexpr int kKeys = COLS / 64;        // 16-byte chunks of a key that a lane loads, 64 bytes apart
+    static constexpr int kChunks = COLS / 16;      // 16-byte chunks of a key
+    static constexpr int kKeys = COLS / 64;        // of them that a lane's scores take from each token
+    static constexpr int kLoads = kChunks / 2;     // of a lane for 32 keys
     static constexpr int kWords = COLS / 64;       // words of a value that a lane loads
-    Word4 k[2][kKeys];
+    Word4 k[kLoads];
     uint32_t v[2][4][kWords];
     Float4 kScale[2], vScale[2];
 };
@@ -133,9 +141,9 @@ template <int COLS>
 __device__ __forceinline__ void loadWords(uint32_t (&to)[COLS / 64], const int8_t* at) {
     typedef uint32_t Words __attribute__((ext_vector_type(COLS / 64)));
     if constexpr (COLS == 64) {
-        to[0] = *(const uint32_t*)at;
+        to[0] = __builtin_nontemporal_load((const uint32_t*)at);
     } else {
-        const Words w = *(const Words*)at;
+        const Words w = __builtin_nontemporal_load((const Words*)at);
 #pragma unroll
         for (int i = 0; i < COLS / 64; ++i) to[i] = w[i];
     }
@@ -198,46 +206,79 @@ struct Part {
         qScale = ldexpf(a.scale, down - kByteExponent);
     }
 
-    // Loads the 32 tokens from t on (whole blocks of 16, each in one page) of key head `head`; blocks
-    // from `lastBlock` on are that one, which is masked. A page outside the cache is the first one
-    // instead, with scales that make NaNs.
-    __device__ __forceinline__ void load(Tile<COLS>& tile, int32_t t, int32_t lastBlock, const int32_t* pages, int64_t rowsAt,
-                                         int64_t scalesAt) const {
-        const uint32_t dim16 = (a.dim + 15) & ~15;
+    // The 32 tokens from t on; blocks behind `lastBlock` are that one, which is masked.
+    __device__ __forceinline__ Place find(int32_t t, int32_t lastBlock, const int32_t* pages) const {
+        Place place;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const uint32_t block = min(t / 16 + b, lastBlock);
-            const uint32_t page = (uint32_t)((block * a.pageMagic) >> a.pageShift), in = block - page * a.pageBlocks;
+            const uint32_t page = (uint32_t)((block * a.pageMagic) >> a.pageShift), in = (block - page * a.pageBlocks) * 16;
             const uint32_t p = uniformLoad(pages + page);
-            const bool there = p < a.pages_;
-            const int64_t rows = rowsAt + (int64_t)(there ? p : 0) * a.pageStride + (int64_t)(in * 16) * a.tokenStride;
-            const int64_t scales = scalesAt + (int64_t)(there ? p : 0) * a.scalePage + in * 16;
-            const int8_t* const k = a.k + rows;
+            place.there[b] = p < a.pages_;
+            place.rows[b] = (int64_t)(place.there[b] ? p : 0) * a.pageStride + (int64_t)in * a.tokenStride;
+            place.scales[b] = (int64_t)(place.there[b] ? p : 0) * a.scalePage + in;
+        }
+        return place;
+    }
+
+    // Whole keys, a chunk a lane: 64 / kChunks of them at once, which are whole cache lines. Of 64
+    // columns a lane's chunk is the one that its scores take.
+    __device__ __forceinline__ void loadKeys(Tile<COLS>& tile, const Place& place, const int8_t* k, const float* scales) const {
+        constexpr int kChunks = Tile<COLS>::kChunks, kRows = kWave / kChunks;
+        const uint32_t chunk = 16 * (kThroughLds ? lane % kChunks : group);
+        const uint32_t offset = (kThroughLds ? lane / kChunks : at) * a.tokenStride + (chunk < dim16() ? chunk : 0);
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-                const uint32_t col = 64 * i + 16 * group;
-                tile.k[b][i] = *(const Word4*)(k + at * a.tokenStride + (col < dim16 ? col : 0));
-            }
-            const int8_t* const v = a.v + rows;
-            const uint32_t col = kBytes * at;
+        for (int n = 0; n < Tile<COLS>::kLoads; ++n) {
+            const int row = n * kRows;
+            tile.k[n] = __builtin_nontemporal_load((const Word4*)(k + place.rows[row / 16] + row % 16 * (int64_t)a.tokenStride + offset));
+        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                loadWords<COLS>(tile.v[b][r], v + (4 * group + r) * a.tokenStride + (col < dim16 ? col : 0));
-            tile.kScale[b] = *(const Float4*)(a.kScale + scales + 4 * group);
-            tile.vScale[b] = *(const Float4*)(a.vScale + scales + 4 * group);
-            if (!there) tile.kScale[b] = NAN;
+        for (int b = 0; b < 2; ++b) {
+            tile.kScale[b] = *(const Float4*)(scales + place.scales[b] + 4 * group);
+            if (!place.there[b]) tile.kScale[b] = NAN;
         }
     }
 
-    // Adds the tile of tokens t .. t + 31; those outside [begin, end) count nothing.
-    __device__ __forceinline__ void add(Tile<COLS>& tile, int32_t t, int32_t begin, int32_t end) {
-        float s[2][4];
+    __device__ __forceinline__ void loadValues(Tile<COLS>& tile, const Place& place, const int8_t* v, const float* scales) const {
+        const uint32_t col = kBytes * at, offset = 4 * group * a.tokenStride + (col < dim16() ? col : 0);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) loadWords<COLS>(tile.v[b][r], v + place.rows[b] + r * (int64_t)a.tokenStride + offset);
+            tile.vScale[b] = *(const Float4*)(scales + place.scales[b] + 4 * group);
+        }
+    }
+
+    __device__ __forceinline__ uint32_t dim16() const { return (a.dim + 15) & ~15; }
+
+    // Keys go through LDS of the wave's own, from whole rows to the 16 bytes of a token that a lane's
+    // scores take; chunks of a row are swapped so that neither side meets another lane's bank.
+    static constexpr bool kThroughLds = COLS > 64;
+    __device__ static __forceinline__ int swap(int row) { return COLS == 128 ? row / 2 % 8 : row % 16; }
+    __device__ __forceinline__ void putKeys(const Tile<COLS>& tile, Word4* lds) const {
+        constexpr int kChunks = Tile<COLS>::kChunks, kRows = kWave / kChunks;
+#pragma unroll
+        for (int n = 0; n < Tile<COLS>::kLoads; ++n) {
+            const int row = n * kRows + lane / kChunks;
+            lds[row * kChunks + (lane % kChunks ^ swap(row))] = tile.k[n];
+        }
+    }
+    __device__ __forceinline__ void getKeys(Word4 (&k)[2][kKeys], const Word4* lds) const {
+        constexpr int kChunks = Tile<COLS>::kChunks;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) k[b][i] = lds[(16 * b + at) * kChunks + ((4 * i + group) ^ swap(16 * b + at))];
+    }
+
+    // The scores of 32 tokens.
+    __device__ __forceinline__ void score(const Word4 (&k)[2][kKeys], const Float4 (&kScale)[2], float (&s)[2][4]) const {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             Float4 score = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < kKeys; ++i) {
-                const Word4 w = tile.k[b][i] ^ 0x80808080u;
+                const Word4 w = k[b][i] ^ 0x80808080u;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t x = w[2 * j], y = w[2 * j + 1];
@@ -247,8 +288,12 @@ struct Part {
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[b][r] = score[r] * tile.kScale[b][r] * qScale;
+            for (int r = 0; r < 4; ++r) s[b][r] = score[r] * kScale[b][r] * qScale;
         }
+    }
+
+    // Adds the tokens t .. t + 31 with their scores; those outside [begin, end) count nothing.
+    __device__ __forceinline__ void add(Tile<COLS>& tile, float (&s)[2][4], int32_t t, int32_t begin, int32_t end) {
         if (t < begin || t + kTile > end) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -327,20 +372,26 @@ __device__ __forceinline__ float logSum(float top, float total) {
     return (top + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
 }
 
+// Waves of a SIMD, by what their registers leave room for.
+template <typename T>
+constexpr int wavesOf(int cols) {
+    return cols == 64 ? 4 : cols == 128 ? (sizeof(T) == 4 ? 2 : 3) : sizeof(T) == 4 ? 1 : 2;
+}
+
 template <typename T, int COLS>
-__global__ __launch_bounds__(kBlock, COLS == 64 ? 4 : COLS == 128 ? 3 : 2) void attendKernel(AttendArgs a) {
+__global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendArgs a) {
     constexpr int kBytes = COLS / 16;
     __shared__ float tops[kWavesPerBlock][kHeadTile], totals[kWavesPerBlock][kHeadTile];
-    __shared__ float sums[kWavesPerBlock][kHeadTile][COLS + 4];
-    const int wave = uniform(threadIdx.x / kWave), group16 = a.heads / a.kvHeads;
-    const uint32_t i = blockIdx.y * kRowOfBlocks + blockIdx.x;
-    // The tiles of one item read the same rows: they go to one of the 8 caches, one behind the other.
-    const uint32_t item = i / (8 * a.tiles) * 8 + i % 8, tile = i / 8 % a.tiles;
-    if (item >= (uint32_t)a.batch * a.kvHeads * a.mostParts) return;
-    const int part = item % a.mostParts, kvHead = item / a.mostParts % a.kvHeads;
-    const int64_t b = item / a.mostParts / a.kvHeads;
+    __shared__ union {
+        float sums[kWavesPerBlock][kHeadTile][COLS + 4];
+        Word4 keys[kWavesPerBlock][kTile * Tile<COLS>::kChunks];
+    } lds;
+    auto& sums = lds.sums;
+    const int wave = uniform(threadIdx.x / kWave), shared = a.heads / a.kvHeads;
+    const int part = blockIdx.x, kvHead = blockIdx.y / a.tiles, tile16 = blockIdx.y - kvHead * a.tiles;
+    const int64_t b = blockIdx.z;
     const Range range(uniformLoad(a.lengths + b), a.capacity, a.window);
-    const int first = kvHead * group16 + tile * kHeadTile, count = min(kHeadTile, group16 - (int)tile * kHeadTile);
+    const int first = kvHead * shared + tile16 * kHeadTile, count = min(kHeadTile, shared - tile16 * kHeadTile);
     if (range.parts == 0) {   // no tokens, or a length outside the cache
         if (part) return;
         for (int c = threadIdx.x; c < count * a.dim; c += kBlock)
@@ -350,6 +401,19 @@ __global__ __launch_bounds__(kBlock, COLS == 64 ? 4 : COLS == 128 ? 3 : 2) void 
     }
     if (part >= range.parts) return;
     const int32_t from = range.base + part * range.each, to = min(range.end, from + range.each);
+    const int32_t* const pages = a.pages + b * a.pagesStride;
+    const int8_t *const k = a.k + kvHead * a.headStride, *const v = a.v + kvHead * a.headStride;
+    const float *const kScale = a.kScale + kvHead * a.scaleHead, *const vScale = a.vScale + kvHead * a.scaleHead;
+    const int32_t lastBlock = (to - 1) / 16;
+    Part<T, COLS> p(a);
+    Tile<COLS> tile;
+    int32_t t = from + wave * kTile;
+    Place place;
+    if (t < to) {
+        place = p.find(t, lastBlock, pages);
+        p.loadKeys(tile, place, k, kScale);
+        p.loadValues(tile, place, v, vScale);
+    }
     // The heads' queries, in f32, with zeros behind them.
     const T* const q = (const T*)a.q + b * a.qToken + first * a.qHead;
     for (int c = threadIdx.x; c < kHeadTile * COLS; c += kBlock) {
@@ -357,19 +421,32 @@ __global__ __launch_bounds__(kBlock, COLS == 64 ? 4 : COLS == 128 ? 3 : 2) void 
         sums[0][h][col] = h < count && col < a.dim ? (float)q[h * a.qHead + col] : 0.0f;
     }
     __syncthreads();
-    Part<T, COLS> p(a);
     p.loadQuery(sums[0][p.at]);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kBytes; ++j) p.sum[j] = 0.0f;
-    const int32_t* const pages = a.pages + b * a.pagesStride;
-    const int64_t rowsAt = kvHead * a.headStride, scalesAt = kvHead * a.scaleHead;
-    const int32_t lastBlock = (to - 1) / 16;
-    for (int32_t t = from + wave * kTile; t < to; t += kRound) {
-        Tile<COLS> tile;
-        p.load(tile, t, lastBlock, pages, rowsAt, scalesAt);
-        p.add(tile, t, range.begin, to);
+    Word4* const keys = lds.keys[wave];
+    while (t < to) {
+        // The next tokens' keys are on their way while these are weighed, their values behind that.
+        const int32_t next = t + kRound;
+        if (next < to) place = p.find(next, lastBlock, pages);
+        Word4 own[2][Tile<COLS>::kKeys];
+        const Float4 scales[2] = {tile.kScale[0], tile.kScale[1]};
+        if constexpr (Part<T, COLS>::kThroughLds) {
+            p.putKeys(tile, keys);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) own[h][0] = tile.k[h];
+        }
+        if (next < to) p.loadKeys(tile, place, k, kScale);
+        if constexpr (Part<T, COLS>::kThroughLds) p.getKeys(own, keys);
+        float s[2][4];
+        p.score(own, scales, s);
+        p.add(tile, s, t, range.begin, to);
+        if (next < to) p.loadValues(tile, place, v, vScale);
+        t = next;
     }
+    __syncthreads();   // the keys' LDS becomes the sums'
     // The waves' sums, each times what its maximum is below the largest by, are added in their order.
     p.total = sum4(p.total);
     if (p.group == 0) tops[wave][p.at] = p.top, totals[wave][p.at] = p.total;
@@ -465,17 +542,27 @@ int mostPartsOf(int64_t capacity, int64_t window) {
     return (int)std::clamp<int64_t>((most + kLeastPart - 1) / kLeastPart, 1, kMostParts);
 }
 
+// A grid has 65535 blocks at the most along its second and third directions.
+constexpr int64_t kMostBatch = 65535;
+
 template <typename T>
-hipError_t launchTyped(const AttendArgs& a, hipStream_t stream) {
-    const uint64_t items = (uint64_t)a.batch * a.kvHeads * a.mostParts, blocks = (items + 7) / 8 * 8 * a.tiles;
-    const dim3 grid((unsigned)std::min<uint64_t>(blocks, kRowOfBlocks), (unsigned)((blocks + kRowOfBlocks - 1) / kRowOfBlocks));
-    const hipError_t rc =
-        a.dim <= 64    ? ridge::launchKernel(attendKernel<T, 64>, grid, kBlock, stream, a)
-        : a.dim <= 128 ? ridge::launchKernel(attendKernel<T, 128>, grid, kBlock, stream, a)
-                       : ridge::launchKernel(attendKernel<T, 256>, grid, kBlock, stream, a);
-    if (rc != hipSuccess || a.mostParts == 1) return rc;
-    const unsigned rows = (unsigned)std::min<int64_t>((int64_t)a.batch * a.heads, kMostBlocks);
-    return ridge::launchKernel(joinKernel<T>, rows, kBlock, stream, a);
+hipError_t launchTyped(AttendArgs a, hipStream_t stream) {
+    const int64_t batch = a.batch;
+    for (int64_t from = 0; from < batch; from += kMostBatch) {
+        a.batch = (int32_t)std::min(batch - from, kMostBatch);
+        const dim3 grid((unsigned)a.mostParts, (unsigned)(a.kvHeads * a.tiles), (unsigned)a.batch);
+        hipError_t rc = a.dim <= 64    ? ridge::launchKernel(attendKernel<T, 64>, grid, kBlock, stream, a)
+                        : a.dim <= 128 ? ridge::launchKernel(attendKernel<T, 128>, grid, kBlock, stream, a)
+                                       : ridge::launchKernel(attendKernel<T, 256>, grid, kBlock, stream, a);
+        if (rc == hipSuccess && a.mostParts > 1)
+            rc = ridge::launchKernel(joinKernel<T>, (unsigned)std::min<int64_t>((int64_t)a.batch * a.heads, kMostBlocks), kBlock,
+                                     stream, a);
+        if (rc != hipSuccess) return rc;
+        a.q = (const T*)a.q + kMostBatch * a.qToken, a.out = (T*)a.out + kMostBatch * a.outToken;
+        a.pages += kMostBatch * a.pagesStride, a.lengths += kMostBatch;
+        if (a.lse) a.lse += kMostBatch * a.heads;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
