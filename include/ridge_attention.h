@@ -34,7 +34,7 @@ extern "C" {
 #endif
 
 /* Most columns of a head, axes of a rotation, and tokens that a cache holds. */
-enum { RIDGE_ATTENTION_MAX_DIM = 256, RIDGE_ATTENTION_MAX_AXES = 4, RIDGE_ATTENTION_MAX_SLOTS = 0x7fffffff };
+enum { RIDGE_ATTENTION_MAX_DIM = 256, RIDGE_ATTENTION_MAX_AXES = 4, RIDGE_ATTENTION_MAX_SLOTS = 0x7fff0000 };
 
 /* Heads of tokens: element (t, h, d) is at[t * token + h * head + d]. */
 typedef struct {

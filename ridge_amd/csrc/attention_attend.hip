@@ -48,12 +48,12 @@ struct AttendArgs {
     float* lse;
     const int32_t* pages;
     const int32_t* lengths;
-    float* parts;          // sums [batch * heads * mostParts][dim], then maxima and sums of p
+    float* parts;          // sums [batch * heads * mostParts][dim], then what they and the sums of p are relative to, and these
     int64_t pageStride, headStride, scalePage, scaleHead;
     int64_t qToken, qHead, outToken, outHead, pagesStride;
-    uint64_t pageMagic;    // (block * pageMagic) >> pageShift is block / blocks of a page
-    uint32_t tokenStride, pageShift, pageBlocks, pages_;
-    int32_t capacity, window, batch, heads, kvHeads, dim, tiles, mostParts;
+    uint32_t tokenStride, pageCount, pageBlocks;   // blocks: of 16 tokens, of a page
+    uint32_t pageMagic, pageShift;                 // block / pageBlocks is 16 block times pageMagic, shifted by 32 + pageShift
+    int32_t capacity, window, batch, heads, kvHeads, dim, tiles, mostParts, run;   // run: parts of a workgroup
     float scale;           // times log2(e): exponentials are powers of two
 };
 
@@ -81,14 +81,18 @@ __device__ __forceinline__ int32_t uniformLoad(const int32_t* at) {
     return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)at;
 }
 
-// Largest over the four lanes of a head (lane, lane ^ 16, lane ^ 32 and both).
+// Largest and sum over the four lanes of a head: this one, lane ^ 16, lane ^ 32 and both.
 __device__ __forceinline__ float most4(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float sum4(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // 2^n for n in -126 .. 127.
@@ -120,9 +124,8 @@ __device__ __forceinline__ Half8 join(Half2 a, Half2 b, Half2 c, Half2 d) {
 }
 
 // Where a wave's 32 tokens are: two blocks of 16, each in one page. The same for all its lanes.
-struct Place {
-    int64_t rows[2], scales[2];   // from the beginning of k or v and of their scales
-    bool there[2];                // whether the page is one of the cache's: else it is the first one instead
+struct Blocks {
+    uint32_t page[2], in[2];   // the cache's page, and the first token in it
 };
 
 // 32 tokens' operands of a lane. COLS: a head's columns, padded.
@@ -137,57 +140,102 @@ struct Tile {
     Float4 kScale[2], vScale[2];
 };
 
-template <int COLS>
-__device__ __forceinline__ void loadWords(uint32_t (&to)[COLS / 64], const int8_t* at) {
-    typedef uint32_t Words __attribute__((ext_vector_type(COLS / 64)));
-    if constexpr (COLS == 64) {
-        to[0] = __builtin_nontemporal_load((const uint32_t*)at);
+// Loads past the caches (bit 1): a key or value is read once, and its cache line whole by one load.
+constexpr int kStream = 2;
+
+// Memory from `at` on, for offsets of 32 bits: no lane computes an address.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t memory(const void* at) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, 0xffffffff, 0x00027000);
+}
+
+template <int n>
+__device__ __forceinline__ void loadWords(uint32_t (&to)[n], __amdgpu_buffer_rsrc_t from, uint32_t lane, uint32_t all) {
+    if constexpr (n == 1) {
+        to[0] = __builtin_amdgcn_raw_buffer_load_b32(from, lane, all, kStream);
+    } else if constexpr (n == 2) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(from, lane, all, kStream);
+        to[0] = w[0], to[1] = w[1];
     } else {
-        const Words w = __builtin_nontemporal_load((const Words*)at);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(from, lane, all, kStream);
 #pragma unroll
-        for (int i = 0; i < COLS / 64; ++i) to[i] = w[i];
+        for (int i = 0; i < n; ++i) to[i] = w[i];
     }
 }
 
-// One workgroup's part of a sequence: 16 query heads over [from, to) of its tokens.
+// One wave's tokens of a part of a sequence, for 16 query heads. Probabilities are relative:
+// 2^(score - from), which is 2^15 / unit for the largest score, so that times a value's scale they are
+// at most 2^15.
 template <typename T, int COLS>
 struct Part {
     static constexpr int kKeys = Tile<COLS>::kKeys;
     static constexpr int kBytes = COLS / 16;       // of a value that a lane loads, and sums of 16 columns that it holds 4 of
     static constexpr bool kSplitQ = sizeof(T) == 4;
+    static constexpr int kLeastExponent = -90;     // of unit: sums of 2^15 / unit stay in f32's range
+    typedef typename ridge::Memory<T, 8>::Vec Vec;
+
     const AttendArgs& a;
     const int lane = threadIdx.x % kWave, at = lane % 16, group = lane / 16;
     Half8 q[kKeys][2], qLow[kSplitQ ? kKeys : 1][2];
-    float qScale;                                  // of scores, in powers of two
+    float qScale;                                  // of scores, to powers of two
     Float4 sum[kBytes];                            // of value columns kBytes (4 group + r) + i, for head `at`
-    float top = -INFINITY, total = 0.0f;           // the largest score, and this lane's part of the sum of p
-    float unit = 0.0f, lift = 0.0f;                // a power of two above every value's scale so far, and 2^15 / unit
-    int exponent = 0;                              // of unit
+    float top, from, total;                        // the largest score, and this lane's part of the sum of p
+    float unit;                                    // a power of two above every value's scale so far
+    int exponent;                                  // of unit
 
     __device__ Part(const AttendArgs& a) : a(a) {}
 
-    // The query's fragments: 8 columns from 64 i + 16 group + 8 j on, of head `at`, whose columns are in
-    // LDS. Of bf16 and f32 the head is scaled by a power of two so that its largest column is 2^14
-    // to 2^15.
-    __device__ void loadQuery(const float* row) {
-        float x[kKeys][2][8];
-        float most = 0.0f;
+    __device__ __forceinline__ void clear() {
+        top = from = -INFINITY, total = 0.0f, exponent = kLeastExponent, unit = power2(kLeastExponent);
+#pragma unroll
+        for (int j = 0; j < kBytes; ++j) sum[j] = 0.0f;
+    }
+
+    // The query's columns that this lane multiplies: 8 from 64 i + 16 group + 8 j on, of head `at`.
+    struct Query {
+        Vec x[kKeys][2];
+    };
+    __device__ __forceinline__ void loadQuery(Query& query, const T* row) const {
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j) {
+                const int col = 64 * i + 16 * group + 8 * j;
+                if (a.dim % 8 == 0) {
+                    query.x[i][j] = *(const Vec*)(row + (col < a.dim ? col : 0));
+                } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[i][j][e] = row[64 * i + 16 * group + 8 * j + e];
-                    most = fmaxf(most, fabsf(x[i][j][e]));
+                    for (int e = 0; e < 8; ++e) {
+                        const T x = row[min(col + e, a.dim - 1)];
+                        query.x[i][j][e] = col + e < a.dim ? x : (T)0;
+                    }
                 }
-        float up = 1.0f;
+            }
+    }
+
+    // Its fragments. A head of bf16 or f32 is scaled by a power of two so that its largest column is
+    // 2^14 to 2^15. A negative scale turns the query, so that the largest score has the largest p.
+    __device__ __forceinline__ void setQuery(const Query& query) {
+        float x[kKeys][2][8];
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool has = 64 * i + 16 * group + 8 * j < a.dim;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][j][e] = has ? (float)query.x[i][j][e] : 0.0f;
+            }
+        float most = 0.0f;
         int down = 0;
         if constexpr (!std::is_same_v<T, _Float16>) {
-            const int n = max(-96, exponentOf(most4(most)) - 14);
-            up = n < -96 ? 1.0f : power2(-n);
-            down = n;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[i][j][e]));
+            down = max(-96, exponentOf(most4(most)) - 14);
         }
+        const float up = a.scale < 0.0f ? -power2(-down) : power2(-down);
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
 #pragma unroll
@@ -203,53 +251,60 @@ struct Part {
                         if constexpr (kSplitQ) qLow[i][j][e + n] = (_Float16)rest[n];
                     }
                 }
-        qScale = ldexpf(a.scale, down - kByteExponent);
+        // Never 0: a masked score of -inf stays one.
+        qScale = fmaxf(ldexpf(fabsf(a.scale), down - kByteExponent), FLT_MIN);
     }
 
-    // The 32 tokens from t on; blocks behind `lastBlock` are that one, which is masked.
-    __device__ __forceinline__ Place find(int32_t t, int32_t lastBlock, const int32_t* pages) const {
-        Place place;
+    // The blocks of the 32 tokens from t on; those behind `lastBlock` are that one, which is masked.
+    __device__ __forceinline__ Blocks find(int32_t t, uint32_t lastBlock, const int32_t* pages) const {
+        Blocks blocks;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const uint32_t block = min(t / 16 + b, lastBlock);
-            const uint32_t page = (uint32_t)((block * a.pageMagic) >> a.pageShift), in = (block - page * a.pageBlocks) * 16;
-            const uint32_t p = uniformLoad(pages + page);
-            place.there[b] = p < a.pages_;
-            place.rows[b] = (int64_t)(place.there[b] ? p : 0) * a.pageStride + (int64_t)in * a.tokenStride;
-            place.scales[b] = (int64_t)(place.there[b] ? p : 0) * a.scalePage + in;
+            const uint32_t block = min((uint32_t)t / 16 + b, lastBlock);
+            const uint32_t page = __umulhi(block * 16, a.pageMagic) >> a.pageShift;
+            blocks.page[b] = uniformLoad(pages + page);
+            blocks.in[b] = (block - page * a.pageBlocks) * 16;
         }
-        return place;
+        return blocks;
     }
+    // A page outside the cache is read as its first one.
+    __device__ __forceinline__ bool there(const Blocks& blocks, int b) const { return blocks.page[b] < a.pageCount; }
+    __device__ __forceinline__ int64_t rowsOf(const Blocks& blocks, int b) const {
+        return (there(blocks, b) ? blocks.page[b] * a.pageStride : 0) + (int64_t)blocks.in[b] * a.tokenStride;
+    }
+    __device__ __forceinline__ const float* scalesOf(const float* scales, const Blocks& blocks, int b) const {
+        return scales + (there(blocks, b) ? blocks.page[b] * a.scalePage : 0) + blocks.in[b];
+    }
+    __device__ __forceinline__ uint32_t within(uint32_t col) const { return col < (uint32_t)((a.dim + 15) & ~15) ? col : 0; }
 
     // Whole keys, a chunk a lane: 64 / kChunks of them at once, which are whole cache lines. Of 64
-    // columns a lane's chunk is the one that its scores take.
-    __device__ __forceinline__ void loadKeys(Tile<COLS>& tile, const Place& place, const int8_t* k, const float* scales) const {
-        constexpr int kChunks = Tile<COLS>::kChunks, kRows = kWave / kChunks;
-        const uint32_t chunk = 16 * (kThroughLds ? lane % kChunks : group);
-        const uint32_t offset = (kThroughLds ? lane / kChunks : at) * a.tokenStride + (chunk < dim16() ? chunk : 0);
-#pragma unroll
-        for (int n = 0; n < Tile<COLS>::kLoads; ++n) {
-            const int row = n * kRows;
-            tile.k[n] = __builtin_nontemporal_load((const Word4*)(k + place.rows[row / 16] + row % 16 * (int64_t)a.tokenStride + offset));
-        }
+    // columns a lane's chunk is the one that its scores take. A page outside the cache makes NaNs.
+    __device__ __forceinline__ void loadKeys(Tile<COLS>& tile, const Blocks& blocks, const int8_t* k, const float* scales) const {
+        constexpr int kChunks = Tile<COLS>::kChunks, kRows = kWave / kChunks, kEach = Tile<COLS>::kLoads / 2;
+        const uint32_t row = kThroughLds ? lane / kChunks : at, chunk = 16 * (kThroughLds ? lane % kChunks : group);
+        const uint32_t offset = row * a.tokenStride + within(chunk);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            tile.kScale[b] = *(const Float4*)(scales + place.scales[b] + 4 * group);
-            if (!place.there[b]) tile.kScale[b] = NAN;
+            const auto from = memory(k + rowsOf(blocks, b));
+#pragma unroll
+            for (int n = 0; n < kEach; ++n)
+                tile.k[b * kEach + n] = __builtin_bit_cast(
+                    Word4, __builtin_amdgcn_raw_buffer_load_b128(from, offset, n * kRows * a.tokenStride, kStream));
+            tile.kScale[b] = *(const Float4*)(scalesOf(scales, blocks, b) + 4 * group);
+            if (!there(blocks, b)) tile.kScale[b] = NAN;
         }
     }
 
-    __device__ __forceinline__ void loadValues(Tile<COLS>& tile, const Place& place, const int8_t* v, const float* scales) const {
-        const uint32_t col = kBytes * at, offset = 4 * group * a.tokenStride + (col < dim16() ? col : 0);
+    __device__ __forceinline__ void loadValues(Tile<COLS>& tile, const Blocks& blocks, const int8_t* v, const float* scales) const {
+        const uint32_t offset = 4 * group * a.tokenStride + within(kBytes * at);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
+            const auto from = memory(v + rowsOf(blocks, b));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) loadWords<COLS>(tile.v[b][r], v + place.rows[b] + r * (int64_t)a.tokenStride + offset);
-            tile.vScale[b] = *(const Float4*)(scales + place.scales[b] + 4 * group);
+            for (int r = 0; r < 4; ++r) loadWords(tile.v[b][r], from, offset, r * a.tokenStride);
+            tile.vScale[b] = *(const Float4*)(scalesOf(scales, blocks, b) + 4 * group);
         }
     }
-
-    __device__ __forceinline__ uint32_t dim16() const { return (a.dim + 15) & ~15; }
 
     // Keys go through LDS of the wave's own, from whole rows to the 16 bytes of a token that a lane's
     // scores take; chunks of a row are swapped so that neither side meets another lane's bank.
@@ -271,7 +326,7 @@ struct Part {
             for (int i = 0; i < kKeys; ++i) k[b][i] = lds[(16 * b + at) * kChunks + ((4 * i + group) ^ swap(16 * b + at))];
     }
 
-    // The scores of 32 tokens.
+    // The scores of 32 tokens, still to be multiplied by qScale.
     __device__ __forceinline__ void score(const Word4 (&k)[2][kKeys], const Float4 (&kScale)[2], float (&s)[2][4]) const {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -288,7 +343,7 @@ struct Part {
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[b][r] = score[r] * kScale[b][r] * qScale;
+            for (int r = 0; r < 4; ++r) s[b][r] = score[r] * kScale[b][r];
         }
     }
 
@@ -312,23 +367,18 @@ struct Part {
             for (int r = 0; r < 4; ++r) most = fmaxf(most, s[b][r]), scale = fmaxf(scale, fabsf(tile.vScale[b][r]));
         // Few tiles have a new maximum or a new largest scale: the sums are rescaled in a branch.
         if (__builtin_amdgcn_ballot_w64(most > top || scale > unit)) {
-            const float next = fmaxf(top, most4(most));
-            float factor = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - next);
-            top = next;
+            scale = most4(scale);   // the 16 heads' lanes have the same tokens
+            if (scale > unit) exponent = min(127, exponentOf(scale) + 1), unit = power2(exponent);
+            const bool none = top == -INFINITY;
+            top = fmaxf(top, most4(most));
+            const float now = top == -INFINITY ? -INFINITY : fmaf(top, qScale, (float)(exponent - 15));
+            const float factor = none ? 0.0f : __builtin_amdgcn_exp2f(from - now);
+            from = now;
             total *= factor;
-#pragma unroll
-            for (int d = 1; d < kWave; d *= 2) scale = fmaxf(scale, __shfl_xor(scale, d));
-            if (scale > unit) {
-                const int now = min(127, max(-112, exponentOf(scale) + 1));
-                factor = unit == 0.0f ? 0.0f : ldexpf(factor, exponent - now);
-                exponent = now;
-                unit = power2(now);
-                lift = power2(15 - now);
-            }
 #pragma unroll
             for (int i = 0; i < kBytes; ++i) sum[i] *= factor;
         }
-        const float from = top == -INFINITY ? 0.0f : top;
+        const float least = top == -INFINITY ? 0.0f : from;
         Half8 high, low;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -337,9 +387,9 @@ struct Part {
                 float weight[2], rest[2];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    const float p = __builtin_amdgcn_exp2f(s[b][r + n] - from);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[b][r + n], qScale, -least));
                     total += p;
-                    weight[n] = p * (tile.vScale[b][r + n] * lift);
+                    weight[n] = p * tile.vScale[b][r + n];
                 }
                 Half2 both;
                 split(weight[0], weight[1], both, rest[0], rest[1]);
@@ -362,14 +412,22 @@ struct Part {
     }
 };
 
+// The launch's arguments, read again: those that only a part's end uses hold no registers before it.
+__device__ __forceinline__ const AttendArgs& again() {
+    typedef const __attribute__((address_space(4))) AttendArgs Constant;
+    uintptr_t at = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const AttendArgs*)(Constant*)at;
+}
+
 // Result (b, head): 16 bits or f32 of `value` columns.
 template <typename T>
 __device__ __forceinline__ void storeOut(const AttendArgs& a, int64_t b, int head, int col, float value) {
     ((T*)a.out)[b * a.outToken + head * a.outHead + col] = (T)value;
 }
 
-__device__ __forceinline__ float logSum(float top, float total) {
-    return (top + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
+__device__ __forceinline__ float logSum(float from, float total) {
+    return (from + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
 }
 
 // Waves of a SIMD, by what their registers leave room for.
@@ -381,17 +439,20 @@ constexpr int wavesOf(int cols) {
 template <typename T, int COLS>
 __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendArgs a) {
     constexpr int kBytes = COLS / 16;
-    __shared__ float tops[kWavesPerBlock][kHeadTile], totals[kWavesPerBlock][kHeadTile];
+    __shared__ float froms[kWavesPerBlock][kHeadTile], totals[kWavesPerBlock][kHeadTile];
     __shared__ union {
         float sums[kWavesPerBlock][kHeadTile][COLS + 4];
         Word4 keys[kWavesPerBlock][kTile * Tile<COLS>::kChunks];
     } lds;
-    auto& sums = lds.sums;
     const int wave = uniform(threadIdx.x / kWave), shared = a.heads / a.kvHeads;
-    const int part = blockIdx.x, kvHead = blockIdx.y / a.tiles, tile16 = blockIdx.y - kvHead * a.tiles;
-    const int64_t b = blockIdx.z;
-    const Range range(uniformLoad(a.lengths + b), a.capacity, a.window);
+    const int kvHead = blockIdx.y / a.tiles, tile16 = blockIdx.y - kvHead * a.tiles;
     const int first = kvHead * shared + tile16 * kHeadTile, count = min(kHeadTile, shared - tile16 * kHeadTile);
+    const int64_t b = blockIdx.z;
+    Part<T, COLS> p(a);
+    typename Part<T, COLS>::Query query;
+    p.loadQuery(query, (const T*)a.q + b * a.qToken + (first + min(p.at, count - 1)) * a.qHead);
+    const Range range(uniformLoad(a.lengths + b), a.capacity, a.window);
+    int part = blockIdx.x * a.run;
     if (range.parts == 0) {   // no tokens, or a length outside the cache
         if (part) return;
         for (int c = threadIdx.x; c < count * a.dim; c += kBlock)
@@ -400,99 +461,93 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
         return;
     }
     if (part >= range.parts) return;
-    const int32_t from = range.base + part * range.each, to = min(range.end, from + range.each);
+    int32_t from = range.base + part * range.each;
+    const int32_t to = (int32_t)min((int64_t)range.end, from + (int64_t)a.run * range.each);
+    const uint32_t lastBlock = (uint32_t)(to - 1) / 16;
     const int32_t* const pages = a.pages + b * a.pagesStride;
     const int8_t *const k = a.k + kvHead * a.headStride, *const v = a.v + kvHead * a.headStride;
     const float *const kScale = a.kScale + kvHead * a.scaleHead, *const vScale = a.vScale + kvHead * a.scaleHead;
-    const int32_t lastBlock = (to - 1) / 16;
-    Part<T, COLS> p(a);
+    // Pages are looked up two tiles ahead, keys loaded one ahead, and values behind their predecessors'.
     Tile<COLS> tile;
     int32_t t = from + wave * kTile;
-    Place place;
+    Blocks blocks = p.find(t, lastBlock, pages);
     if (t < to) {
-        place = p.find(t, lastBlock, pages);
-        p.loadKeys(tile, place, k, kScale);
-        p.loadValues(tile, place, v, vScale);
+        p.loadKeys(tile, blocks, k, kScale);
+        p.loadValues(tile, blocks, v, vScale);
     }
-    // The heads' queries, in f32, with zeros behind them.
-    const T* const q = (const T*)a.q + b * a.qToken + first * a.qHead;
-    for (int c = threadIdx.x; c < kHeadTile * COLS; c += kBlock) {
-        const int h = c / COLS, col = c % COLS;
-        sums[0][h][col] = h < count && col < a.dim ? (float)q[h * a.qHead + col] : 0.0f;
-    }
-    __syncthreads();
-    p.loadQuery(sums[0][p.at]);
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kBytes; ++j) p.sum[j] = 0.0f;
+    blocks = p.find(t + kRound, lastBlock, pages);
+    p.setQuery(query);
     Word4* const keys = lds.keys[wave];
-    while (t < to) {
-        // The next tokens' keys are on their way while these are weighed, their values behind that.
-        const int32_t next = t + kRound;
-        if (next < to) place = p.find(next, lastBlock, pages);
-        Word4 own[2][Tile<COLS>::kKeys];
-        const Float4 scales[2] = {tile.kScale[0], tile.kScale[1]};
-        if constexpr (Part<T, COLS>::kThroughLds) {
-            p.putKeys(tile, keys);
-        } else {
+    for (;; ++part) {
+        p.clear();
+        const int32_t end = min(to, from + range.each);
+        while (t < end) {
+            const int32_t next = t + kRound;
+            Word4 own[2][Tile<COLS>::kKeys];
+            const Float4 scales[2] = {tile.kScale[0], tile.kScale[1]};
+            if constexpr (Part<T, COLS>::kThroughLds) {
+                p.putKeys(tile, keys);
+            } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) own[h][0] = tile.k[h];
+                for (int h = 0; h < 2; ++h) own[h][0] = tile.k[h];
+            }
+            const Blocks ahead = p.find(next + kRound, lastBlock, pages);
+            if (next < to) p.loadKeys(tile, blocks, k, kScale);
+            if constexpr (Part<T, COLS>::kThroughLds) p.getKeys(own, keys);
+            float s[2][4];
+            p.score(own, scales, s);
+            p.add(tile, s, t, range.begin, to);
+            if (next < to) p.loadValues(tile, blocks, v, vScale);
+            blocks = ahead;
+            t = next;
         }
-        if (next < to) p.loadKeys(tile, place, k, kScale);
-        if constexpr (Part<T, COLS>::kThroughLds) p.getKeys(own, keys);
-        float s[2][4];
-        p.score(own, scales, s);
-        p.add(tile, s, t, range.begin, to);
-        if (next < to) p.loadValues(tile, place, v, vScale);
-        t = next;
-    }
-    __syncthreads();   // the keys' LDS becomes the sums'
-    // The waves' sums, each times what its maximum is below the largest by, are added in their order.
-    p.total = sum4(p.total);
-    if (p.group == 0) tops[wave][p.at] = p.top, totals[wave][p.at] = p.total;
-    __syncthreads();
-    float top = tops[0][p.at];
+        // The waves' sums, from the largest `from` on, are added in their order.
+        p.total = sum4(p.total);
+        if (p.group == 0) froms[wave][p.at] = p.from, totals[wave][p.at] = p.total;
+        __syncthreads();   // and the keys' LDS becomes the sums'
+        float most = froms[0][p.at];
 #pragma unroll
-    for (int w = 1; w < kWavesPerBlock; ++w) top = fmaxf(top, tops[w][p.at]);
-    const float below = top == -INFINITY ? 0.0f : top;
-    const float factor = __builtin_amdgcn_exp2f(p.top - below) * (p.unit == 0.0f ? 0.0f : 1.0f);
-    if (p.at < count) {
+        for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, froms[w][p.at]);
+        const float factor = __builtin_amdgcn_exp2f(p.from - (most == -INFINITY ? 0.0f : most) - kByteExponent);
+        if (p.at < count) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < kBytes; ++j)
-                sums[wave][p.at][kBytes * (4 * p.group + r) + j] =
-                    ldexpf(p.sum[j][r] * factor, p.exponent - 15 - kByteExponent);
-    }
-    __syncthreads();
-    const bool alone = range.parts == 1;
-    for (int c = threadIdx.x; c < count * COLS; c += kBlock) {
-        const int h = c / COLS, col = c % COLS;
-        float most = tops[0][h], value = 0.0f, total = 0.0f;
-#pragma unroll
-        for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, tops[w][h]);
-        const float least = most == -INFINITY ? 0.0f : most;
-#pragma unroll
-        for (int w = 0; w < kWavesPerBlock; ++w) {
-            value += sums[w][h][col];
-            total = fmaf(totals[w][h], __builtin_amdgcn_exp2f(tops[w][h] - least), total);
+                for (int j = 0; j < kBytes; ++j) lds.sums[wave][p.at][kBytes * (4 * p.group + r) + j] = p.sum[j][r] * factor;
         }
-        const int64_t row = b * a.heads + first + h;
-        if (alone) {
-            if (col < a.dim) storeOut<T>(a, b, first + h, col, value / total);
-            if (col == 0 && a.lse) a.lse[row] = logSum(most, total);
-        } else {
-            const int64_t place = row * a.mostParts + part, places = (int64_t)a.batch * a.heads * a.mostParts;
-            if (col < a.dim) a.parts[place * a.dim + col] = value;
-            if (col == 0) {
-                a.parts[places * a.dim + 2 * place] = most;
-                a.parts[places * a.dim + 2 * place + 1] = total;
+        __syncthreads();
+        const AttendArgs& e = again();
+        const bool alone = range.parts == 1;
+        for (int c = threadIdx.x; c < count * COLS; c += kBlock) {
+            const int h = c / COLS, col = c % COLS;
+            float most = froms[0][h], value = 0.0f, total = 0.0f;
+#pragma unroll
+            for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, froms[w][h]);
+#pragma unroll
+            for (int w = 0; w < kWavesPerBlock; ++w) {
+                value += lds.sums[w][h][col];
+                total = fmaf(totals[w][h], __builtin_amdgcn_exp2f(froms[w][h] - (most == -INFINITY ? 0.0f : most)), total);
+            }
+            const int64_t row = b * e.heads + first + h;
+            if (alone) {
+                if (col < e.dim) storeOut<T>(e, b, first + h, col, value / total);
+                if (col == 0 && e.lse) e.lse[row] = logSum(most, total);
+            } else {
+                const int64_t place = row * e.mostParts + part, places = (int64_t)e.batch * e.heads * e.mostParts;
+                if (col < e.dim) e.parts[place * e.dim + col] = value;
+                if (col == 0) {
+                    e.parts[places * e.dim + 2 * place] = most;
+                    e.parts[places * e.dim + 2 * place + 1] = total;
+                }
             }
         }
+        from = end;
+        if (from >= to) return;
+        __syncthreads();
     }
 }
 
-// One workgroup a result: its parts' sums, each times what its maximum is below the largest by. The
+// One workgroup a result: its parts' sums, from the largest `from` on. The
 // waves take the parts in turn.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void joinKernel(AttendArgs a) {
@@ -515,13 +570,25 @@ __global__ __launch_bounds__(kBlock) void joinKernel(AttendArgs a) {
         const float weight = lane < range.parts ? __builtin_amdgcn_exp2f(top - least) : 0.0f;
         const float total = ridge::sumOf<kWave>(lane < range.parts ? weight * ends[2 * lane + 1] : 0.0f);
         float x[kMost] = {};
-        for (int p = wave; p < range.parts; p += kWavesPerBlock) {
-            const float w = __shfl(weight, p);
+        // Four parts at a time: their loads are on their way together.
+        constexpr int kAtOnce = 4;
+        for (int from = wave; from < range.parts; from += kWavesPerBlock * kAtOnce) {
+            float part[kAtOnce][kMost], w[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kMost; ++i) {
-                const int col = lane + i * kWave;
-                if (col < a.dim) x[i] = fmaf(w, a.parts[(place + p) * a.dim + col], x[i]);
+            for (int n = 0; n < kAtOnce; ++n) {
+                const int p = from + n * kWavesPerBlock;
+                w[n] = __shfl(weight, min(p, kMostParts - 1));
+                if (p >= range.parts) w[n] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kMost; ++i) {
+                    const int col = lane + i * kWave;
+                    part[n][i] = p < range.parts && col < a.dim ? a.parts[(place + p) * a.dim + col] : 0.0f;
+                }
             }
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n)
+#pragma unroll
+                for (int i = 0; i < kMost; ++i) x[i] = fmaf(w[n], part[n][i], x[i]);
         }
 #pragma unroll
         for (int i = 0; i < kMost; ++i) sums[wave][lane + i * kWave] = x[i];
@@ -542,6 +609,12 @@ int mostPartsOf(int64_t capacity, int64_t window) {
     return (int)std::clamp<int64_t>((most + kLeastPart - 1) / kLeastPart, 1, kMostParts);
 }
 
+// A workgroup goes on to the next parts of its sequence where there are more than fill the card.
+#ifndef WANTED
+#define WANTED 3072
+#endif
+constexpr int64_t kWantedBlocks = WANTED;
+
 // A grid has 65535 blocks at the most along its second and third directions.
 constexpr int64_t kMostBatch = 65535;
 
@@ -550,7 +623,8 @@ hipError_t launchTyped(AttendArgs a, hipStream_t stream) {
     const int64_t batch = a.batch;
     for (int64_t from = 0; from < batch; from += kMostBatch) {
         a.batch = (int32_t)std::min(batch - from, kMostBatch);
-        const dim3 grid((unsigned)a.mostParts, (unsigned)(a.kvHeads * a.tiles), (unsigned)a.batch);
+        a.run = (int32_t)std::clamp<int64_t>((int64_t)a.batch * a.kvHeads * a.tiles * a.mostParts / kWantedBlocks, 1, a.mostParts);
+        const dim3 grid((unsigned)((a.mostParts + a.run - 1) / a.run), (unsigned)(a.kvHeads * a.tiles), (unsigned)a.batch);
         hipError_t rc = a.dim <= 64    ? ridge::launchKernel(attendKernel<T, 64>, grid, kBlock, stream, a)
                         : a.dim <= 128 ? ridge::launchKernel(attendKernel<T, 128>, grid, kBlock, stream, a)
                                        : ridge::launchKernel(attendKernel<T, 256>, grid, kBlock, stream, a);
@@ -601,12 +675,11 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     a.pageStride = cache->pageStride, a.headStride = cache->headStride, a.tokenStride = (uint32_t)cache->tokenStride;
     a.scalePage = cache->scalePage, a.scaleHead = cache->scaleHead;
     a.qToken = q->token, a.qHead = q->head, a.outToken = out->token, a.outHead = out->head, a.pagesStride = pagesStride;
-    // Blocks are fewer than 2^27: with as many bits and the divisor's the quotient is exact.
+    // Blocks are fewer than 2^27: with 28 bits more than the divisor's the quotient is exact.
     a.pageBlocks = (uint32_t)cache->pageSize / 16;
-    a.pageShift = 27;
-    while ((1u << (a.pageShift - 27)) < a.pageBlocks) ++a.pageShift;
-    a.pageMagic = ((1ull << a.pageShift) + a.pageBlocks - 1) / a.pageBlocks;
-    a.pages_ = (uint32_t)cache->pages, a.capacity = (int32_t)capacity;
+    while ((1u << a.pageShift) < a.pageBlocks) ++a.pageShift;
+    a.pageMagic = (uint32_t)(((1ull << (28 + a.pageShift)) + a.pageBlocks - 1) / a.pageBlocks);
+    a.pageCount = (uint32_t)cache->pages, a.capacity = (int32_t)capacity;
     a.window = window >= capacity ? 0 : (int32_t)window, a.batch = (int32_t)batch, a.heads = q->heads;
     a.kvHeads = cache->heads, a.dim = cache->dim, a.tiles = (a.heads / a.kvHeads + kHeadTile - 1) / kHeadTile;
     a.mostParts = mostPartsOf(capacity, a.window);
