@@ -15,8 +15,9 @@
 // from that lane, if the tokens of k = 8 g + 4 a + r are 16 a + 4 g + r. So a lane loads the values of
 // those tokens and no others, and the running maximum's factor is its own head's everywhere.
 //
-// A sequence is cut into parts by its own length alone, so that its result does not depend on the
-// others; a second launch joins the parts where there may be more than one.
+// Work is shared evenly: the rounds (128 tokens) of all sequences' key heads, one behind the other, are
+// cut into one equal share for each workgroup that runs at a time, whatever the sequences' lengths.
+// A sequence's head that a share's border cuts has its pieces joined by a second launch.
 
 #include "attention_common.hpp"
 
@@ -35,8 +36,8 @@ typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
 constexpr int kHeadTile = 16;    // query heads of a workgroup
 constexpr int kTile = 32;        // tokens of a wave at a time
 constexpr int kRound = kTile * kWavesPerBlock;
-constexpr int kLeastPart = 512;  // tokens of a part
-constexpr int kMostParts = 64;   // of a sequence: longer ones have longer parts
+constexpr uint32_t kLeastShare = 2;   // rounds of a workgroup
+constexpr int kDirect = 512;          // tokens of sequences that are never cut, nor shared evenly
 
 struct AttendArgs {
     const int8_t* k;
@@ -48,30 +49,42 @@ struct AttendArgs {
     float* lse;
     const int32_t* pages;
     const int32_t* lengths;
-    float* parts;          // sums [batch * heads * mostParts][dim], then what they and the sums of p are relative to, and these
+    float* pieces;         // of cut heads: Piece::of
+    int4* ends;            // of each key head and tile, or of each workgroup, whichever are fewer: what of it is to join
     int64_t pageStride, headStride, scalePage, scaleHead;
     int64_t qToken, qHead, outToken, outHead, pagesStride;
     uint32_t tokenStride, pageCount, pageBlocks;   // blocks: of 16 tokens, of a page
     uint32_t pageMagic, pageShift;                 // block / pageBlocks is 16 block times pageMagic, shifted by 32 + pageShift
-    int32_t capacity, window, batch, heads, kvHeads, dim, tiles, mostParts, run;   // run: parts of a workgroup
+    int32_t capacity, window, batch, heads, kvHeads, dim, tiles, tileHeads;   // tileHeads: the most of a tile
+    int32_t byHead;        // whether `ends` are the heads'
     float scale;           // times log2(e): exponentials are powers of two
 };
 
-// What a sequence's length says: its tokens [begin, end), cut from `base` on into `parts` of
-// `each`, whole rounds of a workgroup.
+// What a sequence's length says: its tokens [begin, end), and the rounds of a workgroup from `base` on
+// that hold them.
 struct Range {
-    int32_t begin, end, base, each, parts;
+    int32_t begin, end, base;
+    uint32_t rounds;
     bool bad;
-    __host__ __device__ Range(int32_t length, int32_t capacity, int32_t window) {
+    __device__ Range(int32_t length, int32_t capacity, int32_t window) {
         bad = length < 0 || length > capacity;
         end = bad ? 0 : length;
         begin = window && end > window ? end - window : 0;
         base = begin / 16 * 16;
-        const int32_t n = end - base;
-        each = n <= kLeastPart * kMostParts ? kLeastPart
-                                            : (int32_t)(((int64_t)n + kMostParts * kRound - 1) / (kMostParts * kRound)) * kRound;
-        parts = (int32_t)(((int64_t)n + each - 1) / each);
+        rounds = (uint32_t)(end - base + kRound - 1) / kRound;
     }
+    // One of no tokens has a round too: its results are written.
+    __device__ uint32_t share() const { return max(rounds, 1u); }
+};
+
+// A cut head's piece that a workgroup has computed: its first one, or its last. For each query head the
+// sums of its columns, and then what they and the sum of p are relative to, and this.
+struct Piece {
+    float* at;
+    __device__ Piece(const AttendArgs& a, int index) : at(a.pieces + (int64_t)index * a.tileHeads * (a.dim + 2)) {}
+    __device__ static int of(uint32_t block, bool first) { return 2 * block + !first; }
+    __device__ float* sums(const AttendArgs& a, int head) const { return at + head * a.dim; }
+    __device__ float* ends(const AttendArgs& a, int head) const { return at + a.tileHeads * a.dim + 2 * head; }
 };
 
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -174,7 +187,7 @@ struct Part {
     typedef typename ridge::Memory<T, 8>::Vec Vec;
 
     const AttendArgs& a;
-    const int lane = threadIdx.x % kWave, at = lane % 16, group = lane / 16;
+    const int lane, at = lane % 16, group = lane / 16;
     Half8 q[kKeys][2], qLow[kSplitQ ? kKeys : 1][2];
     float qScale;                                  // of scores, to powers of two
     Float4 sum[kBytes];                            // of value columns kBytes (4 group + r) + i, for head `at`
@@ -182,7 +195,7 @@ struct Part {
     float unit;                                    // a power of two above every value's scale so far
     int exponent;                                  // of unit
 
-    __device__ Part(const AttendArgs& a) : a(a) {}
+    __device__ Part(const AttendArgs& a, int lane) : a(a), lane(lane) {}
 
     __device__ __forceinline__ void clear() {
         top = from = -INFINITY, total = 0.0f, exponent = kLeastExponent, unit = power2(kLeastExponent);
@@ -412,7 +425,7 @@ struct Part {
     }
 };
 
-// The launch's arguments, read again: those that only a part's end uses hold no registers before it.
+// The launch's arguments, read again, so that what follows holds no registers before it.
 __device__ __forceinline__ const AttendArgs& again() {
     typedef const __attribute__((address_space(4))) AttendArgs Constant;
     uintptr_t at = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
@@ -436,40 +449,134 @@ constexpr int wavesOf(int cols) {
     return cols == 64 ? 4 : cols == 128 ? (sizeof(T) == 4 ? 2 : 3) : sizeof(T) == 4 ? 1 : 2;
 }
 
-template <typename T, int COLS>
-__global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendArgs a) {
+// What a workgroup computes: rounds that follow each other, in the order of sequences and heads.
+struct Share {
+    uint32_t size, first, left;   // rounds of every workgroup, before this one's, and of it
+    int32_t b, y;                 // where they begin: the sequence, the key head and 16 of its query heads,
+    uint32_t round;               // and the round
+    int32_t length;               // of that sequence
+};
+
+// An even share of all rounds, found from the sequences' lengths, 64 at a time.
+__device__ __forceinline__ Share shareOf(const AttendArgs& a, uint32_t block, uint32_t blocks) {
+    const int lane = threadIdx.x % kWave, heads = a.kvHeads * a.tiles;
+    int32_t length = 0;
+    auto load = [&](int from) {
+        if (from + lane >= a.batch) return 0u;
+        length = a.lengths[from + lane];
+        return Range(length, a.capacity, a.window).share();
+    };
+    auto sum = [&](uint32_t v) {   // of this lane and those before it
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const uint32_t before = __shfl_up(v, d);
+            v += lane >= d ? before : 0;
+        }
+        return v;
+    };
+    uint32_t total = 0, before = sum(load(0));
+    for (int from = 0;;) {
+        total += uniform(__shfl(before, kWave - 1));
+        if ((from += kWave) >= a.batch) break;
+        before = sum(load(from));
+    }
+    total *= heads;
+    Share share = {};
+    share.size = max(kLeastShare, (total + blocks - 1) / blocks);
+    share.first = block * share.size;
+    if (share.first >= total) return share;
+    share.left = min(share.size, total - share.first);
+    const uint32_t sought = share.first / heads;
+    uint32_t passed = 0;
+    int from = 0;
+    if (a.batch > kWave) before = sum(load(0));
+    while (true) {
+        const uint32_t here = uniform(__shfl(before, kWave - 1));
+        if (passed + here > sought) break;
+        passed += here;
+        from += kWave;
+        before = sum(load(from));
+    }
+    const int behind = uniform(__builtin_ctzll(__builtin_amdgcn_ballot_w64(passed + before > sought)));
+    if (behind) passed += uniform(__shfl(before, behind - 1));
+    share.b = from + behind;
+    const uint32_t in = share.first - passed * heads;
+    share.length = __builtin_amdgcn_readlane(length, behind);
+    const uint32_t each = Range(share.length, a.capacity, a.window).share();
+    share.y = uniform(in / each);
+    share.round = uniform(in - share.y * each);
+    return share;
+}
+
+// EVEN: workgroups share all rounds; else each has one sequence's head.
+template <typename T, int COLS, bool EVEN>
+__global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendArgs args) {
     constexpr int kBytes = COLS / 16;
     __shared__ float froms[kWavesPerBlock][kHeadTile], totals[kWavesPerBlock][kHeadTile];
     __shared__ union {
         float sums[kWavesPerBlock][kHeadTile][COLS + 4];
         Word4 keys[kWavesPerBlock][kTile * Tile<COLS>::kChunks];
     } lds;
-    const int wave = uniform(threadIdx.x / kWave), shared = a.heads / a.kvHeads;
-    const int kvHead = blockIdx.y / a.tiles, tile16 = blockIdx.y - kvHead * a.tiles;
+    const uint32_t block = EVEN ? blockIdx.x : 0;
+    Share share = {};
+    if constexpr (EVEN) {
+        share = shareOf(again(), block, gridDim.x);
+        if (share.left == 0) {
+            if (threadIdx.x == 0 && !again().byHead) again().ends[block] = {1, 0, 0, 0};
+            return;
+        }
+    } else {
+        share.left = 1, share.b = blockIdx.z, share.y = blockIdx.y;
+        share.length = uniformLoad(args.lengths + share.b);
+    }
+    bool isFirst = true;
+    do {
+    AttendArgs const& a = EVEN ? again() : args;
+    int thread = threadIdx.x;
+    if constexpr (EVEN) asm volatile("" : "+v"(thread));   // so that nothing is held from one head to the next
+    const int wave = uniform(thread / kWave), shared = a.heads / a.kvHeads;
+    const int kvHead = share.y / a.tiles, tile16 = share.y - kvHead * a.tiles;
     const int first = kvHead * shared + tile16 * kHeadTile, count = min(kHeadTile, shared - tile16 * kHeadTile);
-    const int64_t b = blockIdx.z;
-    Part<T, COLS> p(a);
+    const int64_t b = share.b;
+    Part<T, COLS> p(a, thread % kWave);
     typename Part<T, COLS>::Query query;
     p.loadQuery(query, (const T*)a.q + b * a.qToken + (first + min(p.at, count - 1)) * a.qHead);
-    const Range range(uniformLoad(a.lengths + b), a.capacity, a.window);
-    int part = blockIdx.x * a.run;
-    if (range.parts == 0) {   // no tokens, or a length outside the cache
-        if (part) return;
-        for (int c = threadIdx.x; c < count * a.dim; c += kBlock)
-            storeOut<T>(a, b, first + c / a.dim, c % a.dim, range.bad ? NAN : 0.0f);
-        if (a.lse && threadIdx.x < count) a.lse[b * a.heads + first + threadIdx.x] = range.bad ? NAN : -INFINITY;
-        return;
+    const Range range(share.length, a.capacity, a.window);
+    const uint32_t rounds = EVEN ? min(share.left, range.share() - share.round) : range.share();
+    const bool cut = EVEN && rounds != range.share();
+    const bool ending = share.round + rounds == range.share();
+    if (EVEN && thread == 0 && (a.byHead ? ending : isFirst)) {
+        // A head's pieces: where it begins, its workgroup's first or last one, and from there on first ones.
+        int4 ends = {1, 0, 0, 0};
+        if (share.round && ending) {
+            const uint32_t begins = share.first - share.round, in = begins / share.size;
+            ends = {Piece::of(in, begins == in * share.size), Piece::of(block, true), (int)(b * a.heads + first), count};
+        }
+        a.ends[a.byHead ? b * a.kvHeads * a.tiles + share.y : block] = ends;
     }
-    if (part >= range.parts) return;
-    int32_t from = range.base + part * range.each;
-    const int32_t to = (int32_t)min((int64_t)range.end, from + (int64_t)a.run * range.each);
+    const int piece = EVEN ? Piece::of(block, isFirst) : 0;
+    int32_t t = range.base + (int32_t)share.round * kRound;
+    const int32_t to = (int32_t)min((int64_t)range.end, t + (int64_t)rounds * kRound);
+    isFirst = false;
+    share.left -= EVEN ? rounds : 1;
+    share.round = 0;
+    if (++share.y == a.kvHeads * a.tiles) {
+        share.y = 0, ++share.b;
+        if (EVEN && share.left) share.length = uniformLoad(a.lengths + share.b);
+    }
+    if (range.rounds == 0) {   // no tokens, or a length outside the cache
+        for (int c = thread; c < count * a.dim; c += kBlock)
+            storeOut<T>(a, b, first + c / a.dim, c % a.dim, range.bad ? NAN : 0.0f);
+        if (a.lse && thread < count) a.lse[b * a.heads + first + thread] = range.bad ? NAN : -INFINITY;
+        continue;
+    }
     const uint32_t lastBlock = (uint32_t)(to - 1) / 16;
     const int32_t* const pages = a.pages + b * a.pagesStride;
     const int8_t *const k = a.k + kvHead * a.headStride, *const v = a.v + kvHead * a.headStride;
     const float *const kScale = a.kScale + kvHead * a.scaleHead, *const vScale = a.vScale + kvHead * a.scaleHead;
-    // Pages are looked up two tiles ahead, keys loaded one ahead, and values behind their predecessors'.
-    Tile<COLS> tile;
-    int32_t t = from + wave * kTile;
+    // Pages are looked up two tiles ahead, keys loaded one ahead, and values behind their predecessors.
+    Tile<COLS> tile = {};
+    t += wave * kTile;
     Blocks blocks = p.find(t, lastBlock, pages);
     if (t < to) {
         p.loadKeys(tile, blocks, k, kScale);
@@ -478,10 +585,8 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
     blocks = p.find(t + kRound, lastBlock, pages);
     p.setQuery(query);
     Word4* const keys = lds.keys[wave];
-    for (;; ++part) {
-        p.clear();
-        const int32_t end = min(to, from + range.each);
-        while (t < end) {
+    p.clear();
+        while (t < to) {
             const int32_t next = t + kRound;
             Word4 own[2][Tile<COLS>::kKeys];
             const Float4 scales[2] = {tile.kScale[0], tile.kScale[1]};
@@ -517,8 +622,7 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
         }
         __syncthreads();
         const AttendArgs& e = again();
-        const bool alone = range.parts == 1;
-        for (int c = threadIdx.x; c < count * COLS; c += kBlock) {
+        for (int c = thread; c < count * COLS; c += kBlock) {
             const int h = c / COLS, col = c % COLS;
             float most = froms[0][h], value = 0.0f, total = 0.0f;
 #pragma unroll
@@ -529,91 +633,83 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
                 total = fmaf(totals[w][h], __builtin_amdgcn_exp2f(froms[w][h] - (most == -INFINITY ? 0.0f : most)), total);
             }
             const int64_t row = b * e.heads + first + h;
-            if (alone) {
+            if (!cut) {
                 if (col < e.dim) storeOut<T>(e, b, first + h, col, value / total);
                 if (col == 0 && e.lse) e.lse[row] = logSum(most, total);
             } else {
-                const int64_t place = row * e.mostParts + part, places = (int64_t)e.batch * e.heads * e.mostParts;
-                if (col < e.dim) e.parts[place * e.dim + col] = value;
-                if (col == 0) {
-                    e.parts[places * e.dim + 2 * place] = most;
-                    e.parts[places * e.dim + 2 * place + 1] = total;
-                }
+                const Piece to(e, piece);
+                if (col < e.dim) to.sums(e, h)[col] = value;
+                if (col == 0) to.ends(e, h)[0] = most, to.ends(e, h)[1] = total;
             }
         }
-        from = end;
-        if (from >= to) return;
-        __syncthreads();
-    }
+        if constexpr (EVEN) __syncthreads();   // before the next head's keys
+    } while (EVEN && share.left > 0);
 }
 
-// One workgroup a result: its parts' sums, from the largest `from` on. The
-// waves take the parts in turn.
+// One workgroup for each query head of each head that ends in a share behind the one it began in: its
+// pieces' sums, from the largest `from` on. The waves take the pieces in turn.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void joinKernel(AttendArgs a) {
-    constexpr int kMost = RIDGE_ATTENTION_MAX_DIM / kWave;
+    constexpr int kMost = RIDGE_ATTENTION_MAX_DIM / kWave, kAtOnce = 8;
     __shared__ float sums[kWavesPerBlock][RIDGE_ATTENTION_MAX_DIM];
-    const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
-    const uint32_t rows = (uint32_t)a.batch * a.heads;
-    for (uint32_t row = blockIdx.x; row < rows; row += kMostBlocks) {
-        const int64_t b = row / a.heads;
-        const int head = row % a.heads;
-        const Range range(uniformLoad(a.lengths + b), a.capacity, a.window);
-        if (range.parts <= 1) continue;
-        const int64_t place = (int64_t)row * a.mostParts, places = (int64_t)rows * a.mostParts;
-        const float* const ends = a.parts + places * a.dim + 2 * place;
-        const float top = lane < range.parts ? ends[2 * lane] : -INFINITY;
-        float most = top;
+    const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), h = blockIdx.y;
+    const int4 ends = a.ends[blockIdx.x];
+    if (ends.x > ends.y || h >= ends.w) return;
+    const int begin = ends.x, block = begin / 2, pieces = ends.y / 2 - block + 1, row = ends.z + h;
+    auto at = [&](int i) { return Piece(a, i == 0 ? begin : 2 * (block + i)); };
+    // The first pieces' sums are on their way with all pieces' ends.
+    float part[kAtOnce][kMost], weight[kAtOnce];
+    auto load = [&](int from) {
 #pragma unroll
-        for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-        const float least = most == -INFINITY ? 0.0f : most;
-        const float weight = lane < range.parts ? __builtin_amdgcn_exp2f(top - least) : 0.0f;
-        const float total = ridge::sumOf<kWave>(lane < range.parts ? weight * ends[2 * lane + 1] : 0.0f);
-        float x[kMost] = {};
-        // Four parts at a time: their loads are on their way together.
-        constexpr int kAtOnce = 4;
-        for (int from = wave; from < range.parts; from += kWavesPerBlock * kAtOnce) {
-            float part[kAtOnce][kMost], w[kAtOnce];
+        for (int n = 0; n < kAtOnce; ++n) {
+            const int i = from + n * kWavesPerBlock;
+            const Piece piece = at(min(i, pieces - 1));
+            weight[n] = piece.ends(a, h)[0];
 #pragma unroll
-            for (int n = 0; n < kAtOnce; ++n) {
-                const int p = from + n * kWavesPerBlock;
-                w[n] = __shfl(weight, min(p, kMostParts - 1));
-                if (p >= range.parts) w[n] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < kMost; ++i) {
-                    const int col = lane + i * kWave;
-                    part[n][i] = p < range.parts && col < a.dim ? a.parts[(place + p) * a.dim + col] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < kAtOnce; ++n)
-#pragma unroll
-                for (int i = 0; i < kMost; ++i) x[i] = fmaf(w[n], part[n][i], x[i]);
+            for (int j = 0; j < kMost; ++j)
+                if (j * kWave < a.dim) part[n][j] = piece.sums(a, h)[min(lane + j * kWave, a.dim - 1)];
         }
-#pragma unroll
-        for (int i = 0; i < kMost; ++i) sums[wave][lane + i * kWave] = x[i];
-        __syncthreads();
-        const int col = threadIdx.x;
-        float value = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWavesPerBlock; ++w) value += sums[w][col];
-        if (col < a.dim) storeOut<T>(a, b, head, col, value / total);
-        if (col == 0 && a.lse) a.lse[row] = logSum(most, total);
-        __syncthreads();
+    };
+    load(wave);
+    float most = -INFINITY, top = -INFINITY, total = 0.0f;
+    for (int i = lane; i < pieces; i += kWave) {   // this lane's pieces
+        const float from = at(i).ends(a, h)[0], sum = at(i).ends(a, h)[1], now = fmaxf(top, from);
+        const float least = now == -INFINITY ? 0.0f : now;
+        total = total * __builtin_amdgcn_exp2f(top - least) + sum * __builtin_amdgcn_exp2f(from - least);
+        top = now;
     }
+    most = top;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+    const float least = most == -INFINITY ? 0.0f : most;
+    total = ridge::sumOf<kWave>(total * __builtin_amdgcn_exp2f(top - least));
+    float x[kMost] = {};
+    for (int from = wave; from < pieces; from += kWavesPerBlock * kAtOnce) {
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+            const float w = from + n * kWavesPerBlock < pieces ? __builtin_amdgcn_exp2f(weight[n] - least) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < kMost; ++j)
+                if (j * kWave < a.dim) x[j] = fmaf(w, part[n][j], x[j]);
+        }
+        if (from + kWavesPerBlock * kAtOnce < pieces) load(from + kWavesPerBlock * kAtOnce);
+    }
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) sums[wave][lane + j * kWave] = x[j];
+    __syncthreads();
+    const int col = threadIdx.x;
+    float value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWavesPerBlock; ++w) value += sums[w][col];
+    if (col < a.dim) storeOut<T>(a, row / a.heads, row % a.heads, col, value / total);
+    if (col == 0 && a.lse) a.lse[row] = logSum(most, total);
 }
 
-// The most parts that any sequence of these pages has.
-int mostPartsOf(int64_t capacity, int64_t window) {
-    const int64_t most = window && window + 15 < capacity ? window + 15 : capacity;
-    return (int)std::clamp<int64_t>((most + kLeastPart - 1) / kLeastPart, 1, kMostParts);
+// Workgroups that run at a time, by columns and the type's bytes.
+int residentOf(int dim, size_t bytes) {
+    const int cols = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+    return 256 * (bytes == 4 ? wavesOf<float>(cols) : wavesOf<_Float16>(cols)) * 4 / kWavesPerBlock;
 }
-
-// A workgroup goes on to the next parts of its sequence where there are more than fill the card.
-#ifndef WANTED
-#define WANTED 3072
-#endif
-constexpr int64_t kWantedBlocks = WANTED;
 
 // A grid has 65535 blocks at the most along its second and third directions.
 constexpr int64_t kMostBatch = 65535;
@@ -621,15 +717,22 @@ constexpr int64_t kMostBatch = 65535;
 template <typename T>
 hipError_t launchTyped(AttendArgs a, hipStream_t stream) {
     const int64_t batch = a.batch;
+    const bool even = a.pieces != nullptr;
+    const unsigned blocks = residentOf(a.dim, sizeof(T));
+    if (even) {   // at a multiple of 16 bytes behind the pieces
+        a.ends = (int4*)(a.pieces + ((int64_t)2 * blocks * a.tileHeads * (a.dim + 2) + 3) / 4 * 4);
+    }
     for (int64_t from = 0; from < batch; from += kMostBatch) {
         a.batch = (int32_t)std::min(batch - from, kMostBatch);
-        a.run = (int32_t)std::clamp<int64_t>((int64_t)a.batch * a.kvHeads * a.tiles * a.mostParts / kWantedBlocks, 1, a.mostParts);
-        const dim3 grid((unsigned)((a.mostParts + a.run - 1) / a.run), (unsigned)(a.kvHeads * a.tiles), (unsigned)a.batch);
-        hipError_t rc = a.dim <= 64    ? ridge::launchKernel(attendKernel<T, 64>, grid, kBlock, stream, a)
-                        : a.dim <= 128 ? ridge::launchKernel(attendKernel<T, 128>, grid, kBlock, stream, a)
-                                       : ridge::launchKernel(attendKernel<T, 256>, grid, kBlock, stream, a);
-        if (rc == hipSuccess && a.mostParts > 1)
-            rc = ridge::launchKernel(joinKernel<T>, (unsigned)std::min<int64_t>((int64_t)a.batch * a.heads, kMostBlocks), kBlock,
+        const int64_t heads = (int64_t)a.batch * a.kvHeads * a.tiles;
+        a.byHead = heads < blocks;
+        const dim3 grid = even ? dim3(blocks) : dim3(1, (unsigned)(a.kvHeads * a.tiles), (unsigned)a.batch);
+        auto launch = [&](auto direct, auto evenly) { return ridge::launchKernel(even ? evenly : direct, grid, kBlock, stream, a); };
+        hipError_t rc = a.dim <= 64    ? launch(attendKernel<T, 64, false>, attendKernel<T, 64, true>)
+                        : a.dim <= 128 ? launch(attendKernel<T, 128, false>, attendKernel<T, 128, true>)
+                                       : launch(attendKernel<T, 256, false>, attendKernel<T, 256, true>);
+        if (rc == hipSuccess && even)
+            rc = ridge::launchKernel(joinKernel<T>, dim3((unsigned)std::min<int64_t>(heads, blocks), (unsigned)a.tileHeads), kBlock,
                                      stream, a);
         if (rc != hipSuccess) return rc;
         a.q = (const T*)a.q + kMostBatch * a.qToken, a.out = (T*)a.out + kMostBatch * a.outToken;
@@ -647,10 +750,13 @@ extern "C" int64_t ridge_attention_workspace(int64_t batch, int32_t heads, int32
         dim > RIDGE_ATTENTION_MAX_DIM || pageSize < 16 || pageSize % 16 || pagesEach < 0 ||
         pagesEach > RIDGE_ATTENTION_MAX_SLOTS / pageSize)
         return -1;
-    // Items, and their tiles of heads with them, are counted in 32 bits.
-    if (batch > (INT32_MAX - 8 * 65536) / kMostParts / std::max(heads, 1)) return -1;
-    const int parts = mostPartsOf(pagesEach * pageSize, 0);
-    return parts == 1 ? 0 : batch * heads * parts * (dim + 2) * 4;
+    // Rounds of all heads are counted in 32 bits.
+    const int64_t capacity = pagesEach * pageSize, rounds = capacity / kRound + 2;
+    if (batch > INT32_MAX / std::max(heads, 1) / rounds) return -1;
+    if (capacity <= kDirect) return 0;
+    // Two pieces of each workgroup, and what ends in it.
+    const int64_t blocks = residentOf(dim, 2), tileHeads = std::min(kHeadTile, std::max(heads / kvHeads, 1));
+    return blocks * (2 * tileHeads * (dim + 2) * 4 + 16);
 }
 
 extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ridge_attention_cache_t* cache,
@@ -671,7 +777,7 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     const int64_t capacity = pagesEach * cache->pageSize;
     AttendArgs a = {};
     a.k = cache->k, a.v = cache->v, a.kScale = cache->kScale, a.vScale = cache->vScale;
-    a.q = q->at, a.out = out->at, a.lse = lse, a.pages = pages, a.lengths = lengths, a.parts = (float*)workspace;
+    a.q = q->at, a.out = out->at, a.lse = lse, a.pages = pages, a.lengths = lengths, a.pieces = wanted ? (float*)workspace : nullptr;
     a.pageStride = cache->pageStride, a.headStride = cache->headStride, a.tokenStride = (uint32_t)cache->tokenStride;
     a.scalePage = cache->scalePage, a.scaleHead = cache->scaleHead;
     a.qToken = q->token, a.qHead = q->head, a.outToken = out->token, a.outHead = out->head, a.pagesStride = pagesStride;
@@ -682,7 +788,7 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     a.pageCount = (uint32_t)cache->pages, a.capacity = (int32_t)capacity;
     a.window = window >= capacity ? 0 : (int32_t)window, a.batch = (int32_t)batch, a.heads = q->heads;
     a.kvHeads = cache->heads, a.dim = cache->dim, a.tiles = (a.heads / a.kvHeads + kHeadTile - 1) / kHeadTile;
-    a.mostParts = mostPartsOf(capacity, a.window);
+    a.tileHeads = std::min(kHeadTile, a.heads / a.kvHeads);
     a.scale = (float)(scale * 1.4426950408889634);
     return ridge::typed(type, [&](auto element) { return launchTyped<decltype(element)>(a, (hipStream_t)stream); });
 }
