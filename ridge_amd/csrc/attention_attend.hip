@@ -646,63 +646,68 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
     } while (EVEN && share.left > 0);
 }
 
-// One workgroup for each query head of each head that ends in a share behind the one it began in: its
-// pieces' sums, from the largest `from` on. The waves take the pieces in turn.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void joinKernel(AttendArgs a) {
-    constexpr int kMost = RIDGE_ATTENTION_MAX_DIM / kWave, kAtOnce = 8;
-    __shared__ float sums[kWavesPerBlock][RIDGE_ATTENTION_MAX_DIM];
+// One workgroup for each query head of each key head that has pieces. The waves take them in turn, each
+// with its own running maximum; what all lanes share is read past the vector unit.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void joinKernel(AttendArgs a) {
+    constexpr int kMost = RIDGE_ATTENTION_MAX_DIM / kWave, kAtOnce = 4;
+    __shared__ float sums[WAVES][RIDGE_ATTENTION_MAX_DIM], froms[WAVES], totals[WAVES];
     const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), h = blockIdx.y;
-    const int4 ends = a.ends[blockIdx.x];
-    if (ends.x > ends.y || h >= ends.w) return;
-    const int begin = ends.x, block = begin / 2, pieces = ends.y / 2 - block + 1, row = ends.z + h;
-    auto at = [&](int i) { return Piece(a, i == 0 ? begin : 2 * (block + i)); };
-    // The first pieces' sums are on their way with all pieces' ends.
-    float part[kAtOnce][kMost], weight[kAtOnce];
-    auto load = [&](int from) {
+    const int32_t* const ends = (const int32_t*)(a.ends + blockIdx.x);
+    const int begin = uniformLoad(ends), last = uniformLoad(ends + 1), row = uniformLoad(ends + 2) + h;
+    if (begin > last || h >= uniformLoad(ends + 3)) return;
+    const int block = begin / 2, pieces = last / 2 - block + 1;
+    float x[kMost] = {}, top = -INFINITY, total = 0.0f;
+    for (int i = wave; i < pieces; i += WAVES * kAtOnce) {
+        float part[kAtOnce][kMost], from[kAtOnce], sum[kAtOnce], now = top;
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-            const int i = from + n * kWavesPerBlock;
-            const Piece piece = at(min(i, pieces - 1));
-            weight[n] = piece.ends(a, h)[0];
+            const int p = i + n * WAVES;
+            from[n] = -INFINITY, sum[n] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kMost; ++j)
-                if (j * kWave < a.dim) part[n][j] = piece.sums(a, h)[min(lane + j * kWave, a.dim - 1)];
+            for (int j = 0; j < kMost; ++j) part[n][j] = 0.0f;
+            if (p < pieces) {
+                const Piece piece(a, p == 0 ? begin : 2 * (block + p));
+                from[n] = __int_as_float(uniformLoad((const int32_t*)piece.ends(a, h)));
+                sum[n] = __int_as_float(uniformLoad((const int32_t*)piece.ends(a, h) + 1));
+#pragma unroll
+                for (int j = 0; j < kMost; ++j)
+                    if (j * kWave < a.dim) part[n][j] = piece.sums(a, h)[min(lane + j * kWave, a.dim - 1)];
+            }
         }
-    };
-    load(wave);
-    float most = -INFINITY, top = -INFINITY, total = 0.0f;
-    for (int i = lane; i < pieces; i += kWave) {   // this lane's pieces
-        const float from = at(i).ends(a, h)[0], sum = at(i).ends(a, h)[1], now = fmaxf(top, from);
-        const float least = now == -INFINITY ? 0.0f : now;
-        total = total * __builtin_amdgcn_exp2f(top - least) + sum * __builtin_amdgcn_exp2f(from - least);
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) now = fmaxf(now, from[n]);
+        const float least = now == -INFINITY ? 0.0f : now, keep = __builtin_amdgcn_exp2f(top - least);
         top = now;
-    }
-    most = top;
+        total *= keep;
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    const float least = most == -INFINITY ? 0.0f : most;
-    total = ridge::sumOf<kWave>(total * __builtin_amdgcn_exp2f(top - least));
-    float x[kMost] = {};
-    for (int from = wave; from < pieces; from += kWavesPerBlock * kAtOnce) {
+        for (int j = 0; j < kMost; ++j) x[j] *= keep;
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-            const float w = from + n * kWavesPerBlock < pieces ? __builtin_amdgcn_exp2f(weight[n] - least) : 0.0f;
+            const float weight = __builtin_amdgcn_exp2f(from[n] - least);
+            total = fmaf(weight, sum[n], total);
 #pragma unroll
-            for (int j = 0; j < kMost; ++j)
-                if (j * kWave < a.dim) x[j] = fmaf(w, part[n][j], x[j]);
+            for (int j = 0; j < kMost; ++j) x[j] = fmaf(weight, part[n][j], x[j]);
         }
-        if (from + kWavesPerBlock * kAtOnce < pieces) load(from + kWavesPerBlock * kAtOnce);
     }
 #pragma unroll
     for (int j = 0; j < kMost; ++j) sums[wave][lane + j * kWave] = x[j];
+    if (lane == 0) froms[wave] = top, totals[wave] = total;
     __syncthreads();
     const int col = threadIdx.x;
-    float value = 0.0f;
+    if (col >= a.dim) return;
+    float most = froms[0], value = 0.0f, all = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWavesPerBlock; ++w) value += sums[w][col];
-    if (col < a.dim) storeOut<T>(a, row / a.heads, row % a.heads, col, value / total);
-    if (col == 0 && a.lse) a.lse[row] = logSum(most, total);
+    for (int w = 1; w < WAVES; ++w) most = fmaxf(most, froms[w]);
+    const float least = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float weight = __builtin_amdgcn_exp2f(froms[w] - least);
+        value = fmaf(weight, sums[w][col], value);
+        all = fmaf(weight, totals[w], all);
+    }
+    storeOut<T>(a, row / a.heads, row % a.heads, col, value / all);
+    if (col == 0 && a.lse) a.lse[row] = logSum(most, all);
 }
 
 // Workgroups that run at a time, by columns and the type's bytes.
@@ -731,9 +736,13 @@ hipError_t launchTyped(AttendArgs a, hipStream_t stream) {
         hipError_t rc = a.dim <= 64    ? launch(attendKernel<T, 64, false>, attendKernel<T, 64, true>)
                         : a.dim <= 128 ? launch(attendKernel<T, 128, false>, attendKernel<T, 128, true>)
                                        : launch(attendKernel<T, 256, false>, attendKernel<T, 256, true>);
-        if (rc == hipSuccess && even)
-            rc = ridge::launchKernel(joinKernel<T>, dim3((unsigned)std::min<int64_t>(heads, blocks), (unsigned)a.tileHeads), kBlock,
-                                     stream, a);
+        if (rc == hipSuccess && even) {
+            // Few heads have many pieces each: us of 8 heads of 93, 4 waves | 16: 9.3 | 4.4.
+            const bool few = heads * a.tileHeads <= 256;
+            const dim3 each((unsigned)std::min<int64_t>(heads, blocks), (unsigned)a.tileHeads);
+            rc = few ? ridge::launchKernel(joinKernel<T, 16>, each, 16 * kWave, stream, a)
+                     : ridge::launchKernel(joinKernel<T, 4>, each, 4 * kWave, stream, a);
+        }
         if (rc != hipSuccess) return rc;
         a.q = (const T*)a.q + kMostBatch * a.qToken, a.out = (T*)a.out + kMostBatch * a.outToken;
         a.pages += kMostBatch * a.pagesStride, a.lengths += kMostBatch;
