@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 namespace ridge {
 
@@ -76,19 +77,35 @@ struct Cut {
     }
 };
 
-// Maximum over the LANES lanes (a power of two) of a row.
+// What op makes of the values of the LANES lanes (a power of two) of a row, in all of them: within 16
+// lanes by exchanges that are part of an instruction, behind that by swaps of registers' halves.
+template <int LANES, typename T, typename Op>
+__device__ __forceinline__ T overLanes(T v, Op op) {
+    auto moved = [](T x, auto control) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(control)::value, 15, 15, true));
+    };
+    auto both = [&](auto halves) {   // an element of a vector has no address for a cast of its bits
+        const unsigned a = halves[0], b = halves[1];
+        return op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+    };
+    if constexpr (LANES >= 2) v = op(v, moved(v, std::integral_constant<int, 0xb1>()));    // lanes 1 0 3 2
+    if constexpr (LANES >= 4) v = op(v, moved(v, std::integral_constant<int, 0x4e>()));    // lanes 2 3 0 1
+    if constexpr (LANES >= 8) v = op(v, moved(v, std::integral_constant<int, 0x141>()));   // 8 lanes mirrored
+    if constexpr (LANES >= 16) v = op(v, moved(v, std::integral_constant<int, 0x140>()));  // 16 lanes mirrored
+    const auto bits = [&] { return __builtin_bit_cast(unsigned, v); };
+    if constexpr (LANES >= 32) v = both(__builtin_amdgcn_permlane16_swap(bits(), bits(), false, false));
+    if constexpr (LANES >= 64) v = both(__builtin_amdgcn_permlane32_swap(bits(), bits(), false, false));
+    return v;
+}
+
 template <int LANES>
 __device__ __forceinline__ uint32_t mostOf(uint32_t top) {
-#pragma unroll
-    for (int d = LANES / 2; d > 0; d /= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    return top;
+    return overLanes<LANES>(top, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
 template <int LANES>
 __device__ __forceinline__ float sumOf(float sum) {
-#pragma unroll
-    for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-    return sum;
+    return overLanes<LANES>(sum, [](float a, float b) { return a + b; });
 }
 
 }  // namespace ridge

@@ -34,11 +34,13 @@ struct RopeArgs {
     float eps;
 };
 
-// The cosines' row of a pair of this token, or null where its position is outside the table.
-__device__ __forceinline__ const float* rotationOf(const RopeArgs& a, int64_t token, int pair) {
+// The cosines of a pair of this token, sines behind them; `there`: whether its position is in the
+// table, whose first row it is otherwise.
+__device__ __forceinline__ const float* rotationOf(const RopeArgs& a, int64_t token, int pair, bool& there) {
     const int axis = (pair >= a.end0) + (pair >= a.end1) + (pair >= a.end2);
     const int32_t position = a.positions[token * a.positionStride + axis];
-    return (uint32_t)position < (uint32_t)a.tableRows ? a.table + position * a.tableStride : nullptr;
+    there = (uint32_t)position < (uint32_t)a.tableRows;
+    return a.table + (there ? position : 0) * a.tableStride + pair;
 }
 
 // A head's sum of squares past the range of f32 would make the root 0 and the head silently so.
@@ -62,8 +64,9 @@ struct Head {
 };
 
 // V pairs a lane, LANES lanes a head: what vectors of V elements hold whole of. The columns that
-// keep their values follow the pairs, two vectors a lane as well.
-template <typename T, typename W, int V, int LANES, bool INTERLEAVED>
+// keep their values follow the pairs, two vectors a lane as well. STREAM: past the caches. MIXED: a
+// section may end inside a vector of pairs.
+template <typename T, typename W, int V, int LANES, bool INTERLEAVED, bool STREAM, bool MIXED>
 __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
     constexpr int kHeads = kWave / LANES;
     const int lane = threadIdx.x % LANES;
@@ -75,25 +78,31 @@ __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
     const bool hasFirst = turns || rest < still, hasSecond = turns || rest + 1 < still;
     const int heads = a.qHeads + a.kHeads;
     ridge::walkParts(a.tokens, a.chunks, [&](int64_t token, int part) {
-        const int from = part * a.each * kHeads;
+        const int from = part * a.each * kHeads + (int)(threadIdx.x % kWave) / LANES;
         float c[V], s[V];
         if (turns) {
-            const float* const row = rotationOf(a, token, pair);
-            if (row) {
-                loadRow<false>(row + pair, c);
-                loadRow<false>(row + a.pairs + pair, s);
+            bool there;
+            if constexpr (!MIXED) {   // a vector's pairs are of one axis
+                const float* const row = rotationOf(a, token, pair, there);
+                loadRow<false>(row, c);
+                loadRow<false>(row + a.pairs, s);
+#pragma unroll
+                for (int e = 0; e < V; ++e) c[e] = there ? c[e] : NAN;
             } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) c[e] = s[e] = NAN;
+                for (int e = 0; e < V; ++e) {
+                    const float* const row = rotationOf(a, token, pair + e, there);
+                    c[e] = there ? row[0] : NAN, s[e] = row[a.pairs];
+                }
             }
         }
         for (int i = 0; i < a.each; ++i) {
-            const int head = from + i * kHeads + (int)(threadIdx.x % kWave) / LANES;
+            const int head = from + i * kHeads;
             if (head >= heads) return;
             const Head<T, W> h(a, token, head);
             float x[2][V] = {};
-            if (hasFirst) loadRow<false>(h.x + first, x[0]);
-            if (hasSecond) loadRow<false>(h.x + second, x[1]);
+            if (hasFirst) loadRow<STREAM>(h.x + first, x[0]);
+            if (hasSecond) loadRow<STREAM>(h.x + second, x[1]);
             if (h.weight) {
                 float squares = 0.0f;
 #pragma unroll
@@ -108,30 +117,24 @@ __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
                     for (int e = 0; e < V; ++e) x[j][e] = x[j][e] * root * w[j][e];
             }
             if (turns) {
-                float y[2][V];
+                // The lane's pairs: of x[0] and x[1], or of each other column of both.
+                constexpr int kBehind = INTERLEAVED && V > 1 ? 1 : V;
+                float* const flat = x[0];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    if constexpr (INTERLEAVED) {   // the lane's 2 V columns are x[0] and then x[1]
-                        constexpr int kHalf = V / 2;
-                        const float y1 = x[e / kHalf][2 * (e % kHalf)], y2 = x[e / kHalf][2 * (e % kHalf) + 1];
-                        y[e / kHalf][2 * (e % kHalf)] = fmaf(y1, c[e], -(y2 * s[e]));
-                        y[e / kHalf][2 * (e % kHalf) + 1] = fmaf(y2, c[e], y1 * s[e]);
-                    } else {
-                        y[0][e] = fmaf(x[0][e], c[e], -(x[1][e] * s[e]));
-                        y[1][e] = fmaf(x[1][e], c[e], x[0][e] * s[e]);
-                    }
+                    float &y1 = flat[kBehind == 1 ? 2 * e : e], &y2 = flat[(kBehind == 1 ? 2 * e : e) + kBehind];
+                    const float turned = fmaf(y1, c[e], -(y2 * s[e]));
+                    y2 = fmaf(y2, c[e], y1 * s[e]);
+                    y1 = turned;
                 }
-                storeRow<false>(h.out + first, y[0]);
-                storeRow<false>(h.out + second, y[1]);
-            } else {
-                if (hasFirst) storeRow<false>(h.out + first, x[0]);
-                if (hasSecond) storeRow<false>(h.out + second, x[1]);
             }
+            if (hasFirst) storeRow<STREAM>(h.out + first, x[0]);
+            if (hasSecond) storeRow<STREAM>(h.out + second, x[1]);
         }
     });
 }
 
-// Any columns, pairs and sections: a wave a head, a column a lane at a time. A column's partner
+// More than 64 odd pairs and columns: a wave a head, a column a lane at a time. A column's partner
 // is read again; every read is before the first write, so that a head may be turned in place.
 template <typename T, typename W>
 __global__ __launch_bounds__(kBlock) void ropeAnyKernel(RopeArgs a) {
@@ -162,8 +165,9 @@ __global__ __launch_bounds__(kBlock) void ropeAnyKernel(RopeArgs a) {
                     const float z = h.weight ? other[i] * root * (float)h.weight[partner] : other[i];
                     const bool isFirst = col < partner;
                     const int pair = a.interleaved ? col / 2 : min(col, partner);
-                    const float* const row = rotationOf(a, token, pair);
-                    const float c = row ? row[pair] : NAN, s = row ? row[a.pairs + pair] : NAN;
+                    bool there;
+                    const float* const row = rotationOf(a, token, pair, there);
+                    const float c = there ? row[0] : NAN, s = row[a.pairs];
                     y = isFirst ? fmaf(y, c, -(z * s)) : fmaf(y, c, z * s);
                 }
                 h.out[col] = (T)y;
@@ -180,25 +184,45 @@ hipError_t launchRope(Kernel kernel, RopeArgs a, int perWave, hipStream_t stream
     return ridge::launchKernel(kernel, cut.blocks, kBlock, stream, a);
 }
 
-template <typename T, typename W, int LANES>
+template <typename T, typename W, int V, int LANES, bool STREAM, bool MIXED>
 hipError_t launchLanes(const RopeArgs& a, hipStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    return a.interleaved ? launchRope(ropeKernel<T, W, V, LANES, true>, a, kWave / LANES, stream)
-                         : launchRope(ropeKernel<T, W, V, LANES, false>, a, kWave / LANES, stream);
+    return a.interleaved ? launchRope(ropeKernel<T, W, V, LANES, true, STREAM, MIXED>, a, kWave / LANES, stream)
+                         : launchRope(ropeKernel<T, W, V, LANES, false, STREAM, MIXED>, a, kWave / LANES, stream);
 }
 
-// 16 bytes a lane and load, where pairs, sections and columns are whole ones.
+template <typename T, typename W, int V, int LANES>
+hipError_t launchLanes(const RopeArgs& a, bool streams, hipStream_t stream) {
+    const bool mixed = a.end0 % V || a.end1 % V || a.end2 % V;
+    if constexpr (V > 1)
+        if (mixed) return launchLanes<T, W, V, LANES, false, true>(a, stream);
+    if constexpr (V * sizeof(T) == 16)
+        if (streams) return launchLanes<T, W, V, LANES, true, false>(a, stream);
+    return launchLanes<T, W, V, LANES, false, false>(a, stream);
+}
+
+// Heads of this size in all, and more, are read and written past the caches: what the attention of
+// a prompt reads next would not find them there.
+constexpr int64_t kStreamBytes = (int64_t)64 << 20;
+
+// The widest vectors that pairs and columns are whole ones of, up to 16 bytes a lane and load.
 template <typename T, typename W>
 hipError_t launchTyped(const RopeArgs& a, hipStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    if (a.pairs % V || (a.dim - 2 * a.pairs) % V || a.end0 % V || a.end1 % V || a.end2 % V)
-        return launchRope(ropeAnyKernel<T, W>, a, 1, stream);
-    const int lanes = a.pairs / V + ((a.dim - 2 * a.pairs) / V + 1) / 2;
-    if (lanes <= 4) return launchLanes<T, W, 4>(a, stream);
-    if (lanes <= 8) return launchLanes<T, W, 8>(a, stream);
-    if (lanes <= 16) return launchLanes<T, W, 16>(a, stream);
-    if constexpr (V == 4) return launchLanes<T, W, 32>(a, stream);
-    return hipErrorInvalidValue;   // 256 columns of 16 bits are 16 lanes
+    constexpr int kWide = 16 / sizeof(T);
+    const int rest = a.dim - 2 * a.pairs;
+    int v = kWide;
+    while (v > 1 && (a.pairs % v || rest % v)) v /= 2;
+    const int lanes = a.pairs / v + (rest / v + 1) / 2;
+    const bool streams = (int64_t)a.tokens * (a.qHeads + a.kHeads) * a.dim * (int64_t)sizeof(T) >= kStreamBytes;
+    if constexpr (kWide == 8) {   // 256 columns are 16 lanes
+        if (v == 8 && lanes <= 4) return launchLanes<T, W, 8, 4>(a, streams, stream);
+        if (v == 8 && lanes <= 8) return launchLanes<T, W, 8, 8>(a, streams, stream);
+        if (v == 8) return launchLanes<T, W, 8, 16>(a, streams, stream);
+    }
+    if (v == 4 && lanes <= 16) return launchLanes<T, W, 4, 16>(a, streams, stream);
+    if (v == 4) return launchLanes<T, W, 4, 32>(a, streams, stream);
+    if (v == 2 && lanes <= 32) return launchLanes<T, W, 2, 32>(a, streams, stream);
+    if (v == 2) return launchLanes<T, W, 2, 64>(a, streams, stream);
+    return lanes <= 64 ? launchLanes<T, W, 1, 64>(a, streams, stream) : launchRope(ropeAnyKernel<T, W>, a, 1, stream);
 }
 
 }  // namespace
