@@ -61,7 +61,7 @@ typedef struct {
  * the angle whose cosine and sine are table[row * stride + p] and [... + pairs + p], row being
  * the token's position on the axis that pair p belongs to: axis 0 turns the first sections[0]
  * pairs, axis 1 the next sections[1], and so on; the sections add up to pairs. Columns from
- * 2 pairs on keep their values. positions is [tokens, axes], its rows positionStride apart. */
+ * 2 pairs on keep their values. The table is less than 4 GiB. positions is [tokens, axes], its rows positionStride apart. */
 typedef struct {
     const float* table;
     int64_t tableStride, tableRows;

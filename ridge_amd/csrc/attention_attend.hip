@@ -27,6 +27,7 @@ using ridge::kBlock;
 using ridge::kMostBlocks;
 using ridge::kWave;
 using ridge::kWavesPerBlock;
+using ridge::uniformLoad;
 
 typedef _Float16 Half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
@@ -88,11 +89,6 @@ struct Piece {
 };
 
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// A whole number of the program's that is the same for all lanes, read past the vector unit.
-__device__ __forceinline__ int32_t uniformLoad(const int32_t* at) {
-    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)at;
-}
 
 // Largest and sum over the four lanes of a head: this one, lane ^ 16, lane ^ 32 and both.
 __device__ __forceinline__ float most4(float v) {

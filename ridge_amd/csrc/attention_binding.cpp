@@ -284,6 +284,7 @@ PyObject* normRopeImpl(PyObject* const* args, Py_ssize_t n) {
     r.table = (const float*)table.data_ptr(), r.tableRows = table.size(0);
     r.tableStride = table.size(0) > 1 ? table.stride(0) : table.size(1);
     if (r.tableStride < table.size(1)) refuse("the rows of table overlap");
+    if (r.tableStride >= ((int64_t)1 << 30) / r.tableRows) refuse("table spans 4 GiB or more");
     integers(positions, positions.dim() == 1 ? 1 : 2, device, "positions");
     const int64_t axes = positions.dim() == 1 ? 1 : positions.size(1);
     if (positions.size(0) != q.tokens || axes < 1 || axes > RIDGE_ATTENTION_MAX_AXES)

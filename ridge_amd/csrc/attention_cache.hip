@@ -44,7 +44,7 @@ template <int LANES, typename F>
 __device__ __forceinline__ void walk(const CacheArgs& a, F&& f) {
     constexpr int kHeads = kWave / LANES;
     ridge::walkParts(a.tokens, a.chunks, [&](int64_t token, int part) {
-        const int32_t slot = a.slots[token];
+        const int32_t slot = ridge::uniformLoad(a.slots + token);
         const int from = part * a.each * kHeads + (int)(threadIdx.x % kWave) / LANES;
         for (int i = 0; i < a.each; ++i) {
             const int head = from + i * kHeads;

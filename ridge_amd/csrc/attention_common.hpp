@@ -53,6 +53,11 @@ hipError_t typed(int type, F&& f) {
     }
 }
 
+// A number that is the same for all lanes, read past the vector unit.
+__device__ __forceinline__ int32_t uniformLoad(const int32_t* at) {
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)at;
+}
+
 // A kernel's tokens are cut into `chunks` parts each, a wave a part. Calls f(token, part) for each
 // part of this wave. There are fewer than 2^32 - kMostBlocks * kWavesPerBlock of them.
 template <typename F>

@@ -26,22 +26,34 @@ struct RopeArgs {
     const void* kWeight;
     const float* table;
     const int32_t* positions;
-    int64_t qToken, qHead, kToken, kHead, qOutToken, qOutHead, kOutToken, kOutHead, tableStride, positionStride;
-    int32_t tokens, qHeads, kHeads, tableRows, pairs, dim;
+    int64_t qToken, qHead, kToken, kHead, qOutToken, qOutHead, kOutToken, kOutHead, positionStride;
+    int32_t tokens, qHeads, kHeads, tableRows, tableStride, pairs, dim;
     int32_t each, chunks;        // heads of a wave at a time and the parts that a token's heads are cut into
-    int32_t end0, end1, end2;    // of the pairs of axes 0, 1 and 2
+    int32_t axes, end0, end1, end2;    // the ends of the pairs of axes 0, 1 and 2
     int32_t interleaved;
     float eps;
 };
 
-// The cosines of a pair of this token, sines behind them; `there`: whether its position is in the
-// table, whose first row it is otherwise.
-__device__ __forceinline__ const float* rotationOf(const RopeArgs& a, int64_t token, int pair, bool& there) {
-    const int axis = (pair >= a.end0) + (pair >= a.end1) + (pair >= a.end2);
-    const int32_t position = a.positions[token * a.positionStride + axis];
-    there = (uint32_t)position < (uint32_t)a.tableRows;
-    return a.table + (there ? position : 0) * a.tableStride + pair;
-}
+// A token's rows of the table, one for each axis: their offsets, or kNowhere for a position outside it.
+// They are the same for all lanes of a wave. A table is less than 4 GiB.
+constexpr uint32_t kNowhere = 0xffffffff;
+struct Rows {
+    uint32_t at[RIDGE_ATTENTION_MAX_AXES];
+    __device__ Rows(const RopeArgs& a, int64_t token) {
+#pragma unroll
+        for (int i = 0; i < RIDGE_ATTENTION_MAX_AXES; ++i) {
+            const uint32_t position = (uint32_t)ridge::uniformLoad(a.positions + token * a.positionStride + min(i, a.axes - 1));
+            at[i] = position < (uint32_t)a.tableRows ? position * (uint32_t)a.tableStride : kNowhere;
+        }
+    }
+    // The cosines of a pair, sines behind them; `there`: whether its position is in the table, whose
+    // first row it is otherwise.
+    __device__ __forceinline__ const float* of(const RopeArgs& a, int pair, bool& there) const {
+        const uint32_t row = pair < a.end0 ? at[0] : pair < a.end1 ? at[1] : pair < a.end2 ? at[2] : at[3];
+        there = row != kNowhere;
+        return a.table + ((there ? row : 0) + (uint32_t)pair);
+    }
+};
 
 // A head's sum of squares past the range of f32 would make the root 0 and the head silently so.
 __device__ __forceinline__ float rootOf(float squares, const RopeArgs& a) {
@@ -63,11 +75,18 @@ struct Head {
     }
 };
 
+template <bool STREAM, typename Vec, typename T>
+__device__ __forceinline__ Vec loadVec(const T* at) {
+    if constexpr (STREAM) return __builtin_nontemporal_load((const Vec*)at);
+    return *(const Vec*)at;
+}
+
 // V pairs a lane, LANES lanes a head: what vectors of V elements hold whole of. The columns that
 // keep their values follow the pairs, two vectors a lane as well. STREAM: past the caches. MIXED: a
 // section may end inside a vector of pairs.
 template <typename T, typename W, int V, int LANES, bool INTERLEAVED, bool STREAM, bool MIXED>
 __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
+    typedef typename ridge::Memory<T, V>::Vec Vec;
     constexpr int kHeads = kWave / LANES;
     const int lane = threadIdx.x % LANES;
     const int turning = a.pairs / V, still = (a.dim - 2 * a.pairs) / V;   // vectors of pairs, and of other columns
@@ -79,19 +98,31 @@ __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
     const int heads = a.qHeads + a.kHeads;
     ridge::walkParts(a.tokens, a.chunks, [&](int64_t token, int part) {
         const int from = part * a.each * kHeads + (int)(threadIdx.x % kWave) / LANES;
+        // Each head's columns are on their way while the one before it is turned, the first one's with
+        // the rotation.
+        Vec next[2] = {};
+        auto load = [&](int head) {
+            const T* const x = Head<T, W>(a, token, head).x;
+            if (hasFirst) next[0] = loadVec<STREAM, Vec>(x + first);
+            if (hasSecond) next[1] = loadVec<STREAM, Vec>(x + second);
+        };
+        if (from < heads) load(from);
+        const Rows rows(a, token);
         float c[V], s[V];
         if (turns) {
             bool there;
             if constexpr (!MIXED) {   // a vector's pairs are of one axis
-                const float* const row = rotationOf(a, token, pair, there);
+                const float* const row = rows.of(a, pair, there);
                 loadRow<false>(row, c);
                 loadRow<false>(row + a.pairs, s);
 #pragma unroll
                 for (int e = 0; e < V; ++e) c[e] = there ? c[e] : NAN;
             } else {
+                int begin = pair;
+                asm volatile("" : "+v"(begin));   // the comparisons of a vector's pairs are not held from token to token
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float* const row = rotationOf(a, token, pair + e, there);
+                    const float* const row = rows.of(a, begin + e, there);
                     c[e] = there ? row[0] : NAN, s[e] = row[a.pairs];
                 }
             }
@@ -100,9 +131,12 @@ __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
             const int head = from + i * kHeads;
             if (head >= heads) return;
             const Head<T, W> h(a, token, head);
-            float x[2][V] = {};
-            if (hasFirst) loadRow<STREAM>(h.x + first, x[0]);
-            if (hasSecond) loadRow<STREAM>(h.x + second, x[1]);
+            float x[2][V];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[j][e] = (float)next[j][e];
+            if (i + 1 < a.each && head + kHeads < heads) load(head + kHeads);
             if (h.weight) {
                 float squares = 0.0f;
 #pragma unroll
@@ -139,12 +173,13 @@ __global__ __launch_bounds__(kBlock) void ropeKernel(RopeArgs a) {
 template <typename T, typename W>
 __global__ __launch_bounds__(kBlock) void ropeAnyKernel(RopeArgs a) {
     constexpr int kMost = RIDGE_ATTENTION_MAX_DIM / kWave;
-    const int lane = threadIdx.x % kWave;
     const int heads = a.qHeads + a.kHeads;
     ridge::walkParts(a.tokens, a.chunks, [&](int64_t token, int part) {
         const int from = part * a.each;
         for (int head = from; head < min(heads, from + a.each); ++head) {
             const Head<T, W> h(a, token, head);
+            int lane = threadIdx.x % kWave;
+            asm volatile("" : "+v"(lane));   // nor are comparisons of columns held here
             float x[kMost], other[kMost], squares = 0.0f;
             auto partnerOf = [&](int col) { return a.interleaved ? col ^ 1 : col < a.pairs ? col + a.pairs : col - a.pairs; };
 #pragma unroll
@@ -163,10 +198,11 @@ __global__ __launch_bounds__(kBlock) void ropeAnyKernel(RopeArgs a) {
                 if (col < 2 * a.pairs) {
                     const int partner = partnerOf(col);
                     const float z = h.weight ? other[i] * root * (float)h.weight[partner] : other[i];
+                    const Rows rows(a, token);
                     const bool isFirst = col < partner;
                     const int pair = a.interleaved ? col / 2 : min(col, partner);
                     bool there;
-                    const float* const row = rotationOf(a, token, pair, there);
+                    const float* const row = rows.of(a, pair, there);
                     const float c = there ? row[0] : NAN, s = row[a.pairs];
                     y = isFirst ? fmaf(y, c, -(z * s)) : fmaf(y, c, z * s);
                 }
@@ -240,7 +276,7 @@ extern "C" int ridge_attention_norm_rope(const ridge_attention_heads_t* q, const
         if (weight && !aligned(weight, sizeOf(weightType))) return hipErrorInvalidValue;
     const ridge_attention_rotation_t& r = *rotation;
     if (r.pairs < 1 || r.pairs > dim / 2 || r.axes < 1 || r.axes > RIDGE_ATTENTION_MAX_AXES || r.tableRows < 1 ||
-        r.tableRows > INT32_MAX || r.tableStride < 2 * r.pairs || r.positionStride < 0 || !aligned(r.table, 4))
+        r.tableRows > INT32_MAX || r.tableStride < 2 * r.pairs || r.tableStride >= (1ll << 30) / r.tableRows || r.positionStride < 0 || !aligned(r.table, 4))
         return hipErrorInvalidValue;
     int ends[RIDGE_ATTENTION_MAX_AXES], end = 0;
     for (int i = 0; i < RIDGE_ATTENTION_MAX_AXES; ++i) {
@@ -259,9 +295,9 @@ extern "C" int ridge_attention_norm_rope(const ridge_attention_heads_t* q, const
     a.table = r.table, a.positions = r.positions;
     a.qToken = q->token, a.qHead = q->head, a.kToken = k->token, a.kHead = k->head;
     a.qOutToken = qOut->token, a.qOutHead = qOut->head, a.kOutToken = kOut->token, a.kOutHead = kOut->head;
-    a.tableStride = r.tableStride, a.positionStride = r.positionStride, a.tokens = (int32_t)tokens;
+    a.tableStride = (int32_t)r.tableStride, a.positionStride = r.positionStride, a.tokens = (int32_t)tokens;
     a.qHeads = q->heads, a.kHeads = k->heads, a.tableRows = (int32_t)r.tableRows, a.pairs = r.pairs, a.dim = dim;
-    a.end0 = ends[0], a.end1 = ends[1], a.end2 = ends[2], a.interleaved = r.interleaved != 0, a.eps = eps;
+    a.end0 = ends[0], a.end1 = ends[1], a.end2 = ends[2], a.interleaved = r.interleaved != 0, a.eps = eps, a.axes = r.axes;
     hipStream_t s = (hipStream_t)stream;
     return ridge::typed(type, [&](auto element) {
         typedef decltype(element) T;

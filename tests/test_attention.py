@@ -85,7 +85,8 @@ def _norm_rope(q=None, k=None, type=0, q_weight=P, k_weight=P, weight_type=0, ep
     ("q's heads", dict(q=_heads(3))), ("k's heads", dict(k_out=_heads(1))), ("stride", dict(k=_heads(2, token=-64))),
     ("head stride", dict(q_out=_heads(head=-1))), ("many heads", dict(q=_heads(65536), q_out=_heads(65536))),
     ("table", dict(rotation=_rotation(table=None))), ("table's stride", dict(rotation=_rotation(tableStride=63))),
-    ("no rows", dict(rotation=_rotation(tableRows=0))), ("positions", dict(rotation=_rotation(positions=None))),
+    ("no rows", dict(rotation=_rotation(tableRows=0))),
+    ("a table of 4 GiB", dict(rotation=_rotation(tableRows=1 << 24))), ("positions", dict(rotation=_rotation(positions=None))),
     ("no pairs", dict(rotation=_rotation((0, 0, 0, 0), pairs=0))), ("axes", dict(rotation=_rotation(axes=0))),
     ("five axes", dict(rotation=_rotation(axes=5))), ("sections", dict(rotation=_rotation((31, 0, 0, 0)))),
     ("sections of two axes", dict(rotation=_rotation((32, 1, 0, 0), axes=2))),
