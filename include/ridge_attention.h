@@ -102,9 +102,11 @@ int64_t ridge_attention_workspace(int64_t batch, int32_t heads, int32_t kvHeads,
  * cache->heads) serves query head h. lse (or null) [b * heads + h] <- log of the sum over t of
  * exp(scale * (q . k_t)). A sequence of no tokens gives zeros, and -inf in lse. A length that is
  * negative or past pagesEach pages, and a page that is none of the cache's where it is read,
- * give NaN. q and out are of `type`; sums are f32. A sequence's result depends on nothing
- * but its own operands. workspace is ridge_attention_workspace bytes, at a multiple of 16, and
- * needs no values; calls that may run at the same time take one each. */
+ * give NaN. q and out are of `type`; sums are f32. All sequences' tokens are shared evenly by the
+ * workgroups that run at a time, so a result's last bits go by the other sequences' lengths; where
+ * pagesEach pages are 512 tokens or fewer, each sequence's key heads have a workgroup each, and its
+ * result depends on nothing but its own operands. workspace is ridge_attention_workspace bytes, at
+ * a multiple of 16, and needs no values; calls that may run at the same time take one each. */
 int ridge_attention_attend(const ridge_attention_heads_t* q, const ridge_attention_cache_t* cache, const int32_t* pages,
                            int64_t pagesStride, int64_t pagesEach, const int32_t* lengths, float scale, int64_t window,
                            const ridge_attention_heads_t* out, float* lse, int type, int64_t batch, void* workspace,

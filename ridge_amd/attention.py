@@ -19,11 +19,13 @@ slot is a token's place in it, page * page_size + offset. The rows are those of
 ridge_amd.int8: a row's largest magnitude over 127 is its scale, and its values over that are
 rounded to the nearest whole number.
 
-Sums, norms and softmax statistics are held in 32 bits, and a token's or a sequence's result
-is the same, bit for bit, whatever is beside it. positions, slots, pages and lengths are int32
-on the device, so what they say cannot be refused: a position outside the table, and a page or
-a length outside the cache, make NaNs of the rows that ask for them; negative slots are
-padding.
+Sums, norms and softmax statistics are held in 32 bits. A call repeated with the same operands
+gives the same bits. Heads that norm_rope turns and rows of the cache do not depend on what is
+beside them; attend shares a batch's work evenly, so the last bits of a sequence's result go by
+the other sequences' lengths (not by what they hold), unless `pages` has room for 512 tokens
+each or fewer. positions, slots, pages and lengths are int32 on the device, so what they say
+cannot be refused: a position outside the table, and a page or a length outside the cache, make
+NaNs of the rows that ask for them; negative slots are padding.
 
 Calls are asynchronous on `stream` (the current one by default) and write into `out` where
 that is given, as those of ridge_amd.int8 do; with all buffers given they can be captured in a

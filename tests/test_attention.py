@@ -177,3 +177,16 @@ def test_host_tensors_are_refused():
     for not_a_cache in (None, x, cache[:3], list(cache), (x, x, x, None)):
         with pytest.raises(A.RidgeAttentionError, match="cache"):
             A.read_cache(not_a_cache, n)
+
+
+def test_without_torch_only_its_extension_is_left_out(monkeypatch, capsys):
+    import sys
+
+    from ridge_amd import build
+    ran = []
+    monkeypatch.setattr(build, "_run", lambda cmd, capture=False: ran.append(cmd) or "")
+    monkeypatch.setattr(build.os, "replace", lambda a, b: None)
+    monkeypatch.setitem(sys.modules, "torch", None)   # import torch raises ImportError
+    assert build.build_attention().endswith("libridge_attention.so")
+    assert len(ran) == len(build.ATTENTION_SRCS) + 1 and not any("binding" in word for cmd in ran for word in cmd)
+    assert "no torch" in capsys.readouterr().out
