@@ -37,8 +37,6 @@ typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
 constexpr int kHeadTile = 16;    // query heads of a workgroup
 constexpr int kTile = 32;        // tokens of a wave at a time
 constexpr int kRound = kTile * kWavesPerBlock;
-constexpr uint32_t kLeastShare = 2;   // rounds of a workgroup
-constexpr int kDirect = 512;          // tokens of sequences that are never cut, nor shared evenly
 
 struct AttendArgs {
     const int8_t* k;
@@ -478,7 +476,7 @@ __device__ __forceinline__ Share shareOf(const AttendArgs& a, uint32_t block, ui
     }
     total *= heads;
     Share share = {};
-    share.size = max(kLeastShare, (total + blocks - 1) / blocks);
+    share.size = (total + blocks - 1) / blocks;
     share.first = block * share.size;
     if (share.first >= total) return share;
     share.left = min(share.size, total - share.first);
@@ -712,6 +710,16 @@ int residentOf(int dim, size_t bytes) {
     return 256 * (bytes == 4 ? wavesOf<float>(cols) : wavesOf<_Float16>(cols)) * 4 / kWavesPerBlock;
 }
 
+// Whether each key head (and tile) has a workgroup, which needs no second launch, instead of an even
+// share of all rounds. us of sequences of one length, each their own | shared, 8 key heads of 128:
+//   1 x 512 9.5 | 9.9, 1 x 768 14 | 10, 16 x 1024 19 | 15, 32 x 1024 21 | 26, 64 x 1024 27 | 37,
+//   32 x 2048 36 | 37, 64 x 2048 48 | 58, 128 x 4096 182 | 192;
+// of lengths from a quarter on: 32 x 1024 20 | 21, 64 x 2048 39 | 45, 128 x 4096 136 | 129. What one long
+// sequence among short ones costs alone (2.2 us for each 128 tokens) bounds the lengths.
+bool eachItsOwn(int64_t batch, int64_t heads, int64_t capacity) {
+    return capacity <= 512 || (capacity <= 1024 && batch * heads >= 256) || (capacity <= 2048 && batch * heads >= 512);
+}
+
 // A grid has 65535 blocks at the most along its second and third directions.
 constexpr int64_t kMostBatch = 65535;
 
@@ -758,9 +766,10 @@ extern "C" int64_t ridge_attention_workspace(int64_t batch, int32_t heads, int32
     // Rounds of all heads are counted in 32 bits.
     const int64_t capacity = pagesEach * pageSize, rounds = capacity / kRound + 2;
     if (batch > INT32_MAX / std::max(heads, 1) / rounds) return -1;
-    if (capacity <= kDirect) return 0;
+    const int64_t shared = heads / kvHeads, tiles = (shared + kHeadTile - 1) / kHeadTile;
+    if (eachItsOwn(batch, kvHeads * tiles, capacity)) return 0;
     // Two pieces of each workgroup, and what ends in it.
-    const int64_t blocks = residentOf(dim, 2), tileHeads = std::min(kHeadTile, std::max(heads / kvHeads, 1));
+    const int64_t blocks = residentOf(dim, 2), tileHeads = std::clamp<int64_t>(shared, 1, kHeadTile);
     return blocks * (2 * tileHeads * (dim + 2) * 4 + 16);
 }
 
@@ -782,7 +791,7 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     const int64_t capacity = pagesEach * cache->pageSize;
     AttendArgs a = {};
     a.k = cache->k, a.v = cache->v, a.kScale = cache->kScale, a.vScale = cache->vScale;
-    a.q = q->at, a.out = out->at, a.lse = lse, a.pages = pages, a.lengths = lengths, a.pieces = wanted ? (float*)workspace : nullptr;
+    a.q = q->at, a.out = out->at, a.lse = lse, a.pages = pages, a.lengths = lengths, a.pieces = nullptr;
     a.pageStride = cache->pageStride, a.headStride = cache->headStride, a.tokenStride = (uint32_t)cache->tokenStride;
     a.scalePage = cache->scalePage, a.scaleHead = cache->scaleHead;
     a.qToken = q->token, a.qHead = q->head, a.outToken = out->token, a.outHead = out->head, a.pagesStride = pagesStride;
@@ -794,6 +803,8 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     a.window = window >= capacity ? 0 : (int32_t)window, a.batch = (int32_t)batch, a.heads = q->heads;
     a.kvHeads = cache->heads, a.dim = cache->dim, a.tiles = (a.heads / a.kvHeads + kHeadTile - 1) / kHeadTile;
     a.tileHeads = std::min(kHeadTile, a.heads / a.kvHeads);
+    const int64_t longest = a.window ? std::min(capacity, (int64_t)a.window + 15) : capacity;   // whole blocks of 16
+    if (!eachItsOwn(batch, (int64_t)a.kvHeads * a.tiles, longest)) a.pieces = (float*)workspace;
     a.scale = (float)(scale * 1.4426950408889634);
     return ridge::typed(type, [&](auto element) { return launchTyped<decltype(element)>(a, (hipStream_t)stream); });
 }

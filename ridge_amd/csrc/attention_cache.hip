@@ -95,12 +95,12 @@ template <typename T, int LANES>
 __global__ __launch_bounds__(kBlock) void writeKernel(CacheArgs a) {
     const int col = threadIdx.x % LANES * kVec, n = a.cache.dim - col;
     walk<LANES>(a, [&](int64_t token, int32_t slot, int head) {
-        if (!holds(a.cache, slot)) return;
-        float k[kVec] = {}, v[kVec] = {};
+        float k[kVec] = {}, v[kVec] = {};   // on their way beside the slot
         if (n > 0) {
             loadPart((const T*)a.k + token * a.kToken + head * a.kHead + col, n, k);
             loadPart((const T*)a.v + token * a.vToken + head * a.vHead + col, n, v);
         }
+        if (!holds(a.cache, slot)) return;
         const Place to(a.cache, slot, head);
         storeRow8<LANES>(k, n, a.cache.k + to.row + col, a.cache.kScale + to.scale);
         storeRow8<LANES>(v, n, a.cache.v + to.row + col, a.cache.vScale + to.scale);

@@ -157,6 +157,9 @@ def test_attend_refuses(what, changes):
 def test_workspace():
     size = A.lib().ridge_attention_workspace
     assert size(3, 8, 2, 128, 32, 16) == 0       # no sequence is cut
+    assert size(128, 8, 2, 128, 64, 16) == 0 < size(127, 8, 2, 128, 64, 16)   # enough heads to fill the card
+    assert size(256, 8, 2, 128, 128, 16) == 0 < min(size(255, 8, 2, 128, 128, 16), size(256, 8, 2, 128, 129, 16))
+    assert size(128, 34, 2, 128, 64, 16) == size(43, 66, 2, 128, 64, 16) == 0   # tiles of 16 heads count
     assert size(3, 8, 2, 128, 33, 16) == size(1, 4, 1, 128, 1 << 20, 16) > 0
     assert size(3, 8, 2, 128, 33, 16) < size(3, 8, 2, 256, 33, 16) and size(1, 64, 1, 128, 33, 16) == size(1, 16, 1, 128, 33, 16)
     for bad in ((-1, 8, 2, 128, 4, 16), (1 << 31, 8, 2, 128, 4, 16), (3, 9, 2, 128, 4, 16), (3, 8, 0, 128, 4, 16),

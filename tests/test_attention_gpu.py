@@ -533,7 +533,7 @@ def test_batches_of_all_sorts(heads, kv_heads, dim, dtype):
     """Shares of rounds that begin and end anywhere: in the first and the last sequence, between sequences
     of none, several heads a workgroup and several workgroups a head, more sequences than a wave has lanes."""
     for lengths in ([0] * 70 + [700], [5000] + [0] * 3, [600], [129] * 63, [129] * 64, [129] * 65 + [3000],
-                    [(i * 389) % 1500 for i in range(150)], [1] * 300, [20000, 1, 1, 20000]):
+                    [(i * 389) % 1500 for i in range(150)], [(i * 389) % 2500 for i in range(300)], [1] * 300, [20000, 1, 1, 20000]):
         b = Batch(lengths, heads, kv_heads, dim, 16, dtype)
         if b.pages.shape[1] <= 32:
             b.pages = torch.cat([b.pages, torch.full((len(lengths), 33), -1, dtype=torch.int32, device=DEV)], dim=1)
