@@ -55,7 +55,7 @@ struct AttendArgs {
     uint32_t tokenStride, pageCount, pageBlocks;   // blocks: of 16 tokens, of a page
     uint32_t pageMagic, pageShift;                 // block / pageBlocks is 16 block times pageMagic, shifted by 32 + pageShift
     int32_t capacity, window, batch, heads, kvHeads, dim, tiles, tileHeads;   // tileHeads: the most of a tile
-    int32_t byHead;        // whether `ends` are the heads'
+    int32_t shared, byHead;   // query heads of a key head; whether `ends` are the heads'
     float scale;           // times log2(e): exponentials are powers of two
 };
 
@@ -525,61 +525,61 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
     }
     bool isFirst = true;
     do {
-    AttendArgs const& a = EVEN ? again() : args;
-    int thread = threadIdx.x;
-    if constexpr (EVEN) asm volatile("" : "+v"(thread));   // so that nothing is held from one head to the next
-    const int wave = uniform(thread / kWave), shared = a.heads / a.kvHeads;
-    const int kvHead = share.y / a.tiles, tile16 = share.y - kvHead * a.tiles;
-    const int first = kvHead * shared + tile16 * kHeadTile, count = min(kHeadTile, shared - tile16 * kHeadTile);
-    const int64_t b = share.b;
-    Part<T, COLS> p(a, thread % kWave);
-    typename Part<T, COLS>::Query query;
-    p.loadQuery(query, (const T*)a.q + b * a.qToken + (first + min(p.at, count - 1)) * a.qHead);
-    const Range range(share.length, a.capacity, a.window);
-    const uint32_t rounds = EVEN ? min(share.left, range.share() - share.round) : range.share();
-    const bool cut = EVEN && rounds != range.share();
-    const bool ending = share.round + rounds == range.share();
-    if (EVEN && thread == 0 && (a.byHead ? ending : isFirst)) {
-        // A head's pieces: where it begins, its workgroup's first or last one, and from there on first ones.
-        int4 ends = {1, 0, 0, 0};
-        if (share.round && ending) {
-            const uint32_t begins = share.first - share.round, in = begins / share.size;
-            ends = {Piece::of(in, begins == in * share.size), Piece::of(block, true), (int)(b * a.heads + first), count};
+        AttendArgs const& a = EVEN ? again() : args;
+        int thread = threadIdx.x;
+        if constexpr (EVEN) asm volatile("" : "+v"(thread));   // so that nothing is held from one head to the next
+        const int wave = uniform(thread / kWave), y = share.y, kvHead = a.tiles == 1 ? y : y / a.tiles;
+        const int tile16 = y - kvHead * a.tiles, first = kvHead * a.shared + tile16 * kHeadTile;
+        const int count = min(kHeadTile, a.shared - tile16 * kHeadTile);
+        const int64_t b = share.b;
+        Part<T, COLS> p(a, thread % kWave);
+        const Range range(share.length, a.capacity, a.window);
+        const uint32_t rounds = EVEN ? min(share.left, range.share() - share.round) : range.share();
+        const bool cut = EVEN && rounds != range.share(), ending = share.round + rounds == range.share();
+        int32_t t = range.base + (int32_t)share.round * kRound;
+        const int32_t to = (int32_t)min((int64_t)range.end, t + (int64_t)rounds * kRound);
+        const uint32_t lastBlock = (uint32_t)max(to - 1, 0) / 16;
+        t += wave * kTile;
+        // Pages are looked up two tiles ahead, keys loaded one ahead, and values behind their predecessors.
+        const int32_t* const pages = a.pages + b * a.pagesStride;
+        Blocks blocks = {};
+        if (range.rounds) blocks = p.find(t, lastBlock, pages);
+        typename Part<T, COLS>::Query query;
+        p.loadQuery(query, (const T*)a.q + b * a.qToken + (first + min(p.at, count - 1)) * a.qHead);
+        if (EVEN && thread == 0 && (a.byHead ? ending : isFirst)) {
+            // A head's pieces: where it begins, its workgroup's first or last one, and from there on first ones.
+            int4 ends = {1, 0, 0, 0};
+            if (share.round && ending) {
+                const uint32_t begins = share.first - share.round, in = begins / share.size;
+                ends = {Piece::of(in, begins == in * share.size), Piece::of(block, true), (int)(b * a.heads + first), count};
+            }
+            a.ends[a.byHead ? b * a.kvHeads * a.tiles + y : block] = ends;
         }
-        a.ends[a.byHead ? b * a.kvHeads * a.tiles + share.y : block] = ends;
-    }
-    const int piece = EVEN ? Piece::of(block, isFirst) : 0;
-    int32_t t = range.base + (int32_t)share.round * kRound;
-    const int32_t to = (int32_t)min((int64_t)range.end, t + (int64_t)rounds * kRound);
-    isFirst = false;
-    share.left -= EVEN ? rounds : 1;
-    share.round = 0;
-    if (++share.y == a.kvHeads * a.tiles) {
-        share.y = 0, ++share.b;
-        if (EVEN && share.left) share.length = uniformLoad(a.lengths + share.b);
-    }
-    if (range.rounds == 0) {   // no tokens, or a length outside the cache
-        for (int c = thread; c < count * a.dim; c += kBlock)
-            storeOut<T>(a, b, first + c / a.dim, c % a.dim, range.bad ? NAN : 0.0f);
-        if (a.lse && thread < count) a.lse[b * a.heads + first + thread] = range.bad ? NAN : -INFINITY;
-        continue;
-    }
-    const uint32_t lastBlock = (uint32_t)(to - 1) / 16;
-    const int32_t* const pages = a.pages + b * a.pagesStride;
-    const int8_t *const k = a.k + kvHead * a.headStride, *const v = a.v + kvHead * a.headStride;
-    const float *const kScale = a.kScale + kvHead * a.scaleHead, *const vScale = a.vScale + kvHead * a.scaleHead;
-    // Pages are looked up two tiles ahead, keys loaded one ahead, and values behind their predecessors.
-    Tile<COLS> tile = {};
-    t += wave * kTile;
-    Blocks blocks = p.find(t, lastBlock, pages);
-    if (t < to) {
-        p.loadKeys(tile, blocks, k, kScale);
-        p.loadValues(tile, blocks, v, vScale);
-    }
-    blocks = p.find(t + kRound, lastBlock, pages);
-    p.setQuery(query);
-    Word4* const keys = lds.keys[wave];
-    p.clear();
+        const int piece = EVEN ? Piece::of(block, isFirst) : 0;
+        isFirst = false;
+        share.left -= EVEN ? rounds : 1;
+        share.round = 0;
+        if (++share.y == a.kvHeads * a.tiles) {
+            share.y = 0, ++share.b;
+            if (EVEN && share.left) share.length = uniformLoad(a.lengths + share.b);
+        }
+        if (range.rounds == 0) {   // no tokens, or a length outside the cache
+            for (int c = thread; c < count * a.dim; c += kBlock)
+                storeOut<T>(a, b, first + c / a.dim, c % a.dim, range.bad ? NAN : 0.0f);
+            if (a.lse && thread < count) a.lse[b * a.heads + first + thread] = range.bad ? NAN : -INFINITY;
+            continue;
+        }
+        const int8_t *const k = a.k + kvHead * a.headStride, *const v = a.v + kvHead * a.headStride;
+        const float *const kScale = a.kScale + kvHead * a.scaleHead, *const vScale = a.vScale + kvHead * a.scaleHead;
+        Tile<COLS> tile = {};
+        if (t < to) {
+            p.loadKeys(tile, blocks, k, kScale);
+            p.loadValues(tile, blocks, v, vScale);
+        }
+        blocks = p.find(t + kRound, lastBlock, pages);
+        p.setQuery(query);
+        Word4* const keys = lds.keys[wave];
+        p.clear();
         while (t < to) {
             const int32_t next = t + kRound;
             Word4 own[2][Tile<COLS>::kKeys];
@@ -802,7 +802,7 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     a.pageCount = (uint32_t)cache->pages, a.capacity = (int32_t)capacity;
     a.window = window >= capacity ? 0 : (int32_t)window, a.batch = (int32_t)batch, a.heads = q->heads;
     a.kvHeads = cache->heads, a.dim = cache->dim, a.tiles = (a.heads / a.kvHeads + kHeadTile - 1) / kHeadTile;
-    a.tileHeads = std::min(kHeadTile, a.heads / a.kvHeads);
+    a.shared = a.heads / a.kvHeads, a.tileHeads = std::min(kHeadTile, a.shared);
     const int64_t longest = a.window ? std::min(capacity, (int64_t)a.window + 15) : capacity;   // whole blocks of 16
     if (!eachItsOwn(batch, (int64_t)a.kvHeads * a.tiles, longest)) a.pieces = (float*)workspace;
     a.scale = (float)(scale * 1.4426950408889634);
