@@ -260,6 +260,23 @@ def test_rows_of_zeros_tiny_values_and_none_numbers():
     assert not bool(A.read_cache(cache, _ints([2, 3]), dtype=torch.float32)[0].isfinite().any())
 
 
+def test_rows_of_every_magnitude_have_quantizes_bits():
+    g = torch.Generator(device=DEV).manual_seed(3)
+    power = torch.arange(-149, 128, device=DEV).repeat_interleave(8)
+    x = (torch.rand((len(power), 2, 64), generator=g, device=DEV) * 2 - 1) * torch.ldexp(torch.ones((), device=DEV), power // 2)[:, None, None]
+    x = x * torch.ldexp(torch.ones((), device=DEV), power - power // 2)[:, None, None]
+    x[::2, :, 0] *= 2   # and a largest value that may be any
+    x[::5, :, 1] = x[::5, :, 0] / 2
+    x = torch.where(x.isfinite(), x, torch.ones_like(x))
+    cache = A.empty_cache(len(power) // 16 + 1, 16, 2, 64)
+    slots = torch.arange(len(power), device=DEV).int()
+    A.write_cache(cache, slots, x, x.flip(2))
+    got = _at(cache, slots)
+    for rows, q, scale in ((x, *got[:2]), (x.flip(2), *got[2:])):
+        want = I.quantize(rows.reshape(-1, 64))
+        assert torch.equal(q.reshape(-1, 64), want[0]) and torch.equal(scale.reshape(-1), want[1])
+
+
 def _strided_caches(pages, page_size, heads, dim):
     """The same cache laid out in other orders: heads behind tokens, k and v between each other, pages apart."""
     wide = (dim + 15) // 16 * 16
