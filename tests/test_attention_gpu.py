@@ -557,6 +557,53 @@ def test_batches_of_all_sorts(heads, kv_heads, dim, dtype):
         b.check()
 
 
+@pytest.mark.parametrize("width", [1, 130])
+def test_more_sequences_than_one_launch_takes(width):
+    # All of them on one page; in 130 pages each they share their rounds, in one each has its own.
+    n, cache = 66001, _filled(2, 16, 1, 16, 1)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    cache[0].copy_(torch.randint(-127, 128, cache[0].shape, generator=g, device=DEV))
+    cache[2].copy_(torch.randint(-127, 128, cache[2].shape, generator=g, device=DEV))
+    cache[1].fill_(0.01), cache[3].fill_(0.02)
+    q = torch.randn((n, 2, 16), generator=g, device=DEV).half()
+    lengths = torch.randint(0, 17, (n,), generator=g, device=DEV, dtype=torch.int32)
+    pages = torch.ones((n, 1), dtype=torch.int32, device=DEV).expand(n, width).contiguous()
+    lse = torch.empty((n, 2), device=DEV)
+    got = A.attend(q, cache, pages, lengths, lse_out=lse)
+    k, v = cache[0][1, 0].double() * cache[1][1, 0].double()[:, None], cache[2][1, 0].double() * cache[3][1, 0].double()[:, None]
+    s = q.double() @ k.t() / 4
+    s = torch.where(torch.arange(16, device=DEV) < lengths[:, None, None], s, -math.inf)
+    want = torch.softmax(s, dim=2).nan_to_num(nan=0.0) @ v
+    # 16 products and 16 tokens: 2^-16 of the magnitudes is far more than f32 loses.
+    _close(got, want, 2.0 ** -16 * 127 * 0.02, torch.float16)
+    exact = torch.logsumexp(s, dim=2)
+    assert torch.equal(lse == -math.inf, exact == -math.inf)
+    assert float((lse.double() - exact)[lse.isfinite()].abs().max()) < 1e-4
+
+
+@pytest.mark.parametrize("dim", [64, 80, 33, 256])
+def test_queries_and_results_of_any_stride(dim):
+    b = Batch([700, 33, 0, 5], 6, 2, dim, 16, torch.bfloat16)
+    want = A.attend(b.q, b.cache, b.pages, b.lengths)
+    memory = torch.zeros((6, 4, 2 * dim + 3), dtype=torch.bfloat16, device=DEV)
+    q, out = memory[..., 1:1 + dim].transpose(0, 1), memory[..., dim + 2:2 * dim + 2].transpose(0, 1)
+    q.copy_(b.q)
+    pages = torch.full((4, 2 * b.pages.shape[1] + 5), -1, dtype=torch.int32, device=DEV)[:, 3:3 + b.pages.shape[1]]
+    pages.copy_(b.pages)
+    assert A.attend(q, b.cache, pages, b.lengths, out=out) is out
+    assert torch.equal(out, want) and torch.equal(q, b.q)
+    assert float(memory[..., 0].abs().max()) == 0 and float(memory[..., dim + 1].abs().max()) == 0
+
+
+def test_sequences_that_share_their_pages():
+    b = Batch([640], 4, 2, 64, 16, torch.float16)
+    pages, lengths = b.pages.expand(3, -1), _ints([640, 100, 639])
+    q = _randn((3, 4, 64), torch.float16, 8)
+    got = A.attend(q, b.cache, pages, lengths)
+    for i, n in enumerate((640, 100, 639)):
+        assert _near(got[i], A.attend(q[i:i + 1], b.cache, b.pages, _ints([n]))[0])
+
+
 def test_no_sequences_and_no_pages():
     b = Batch([5, 0], 4, 2, 64, 16, torch.float16)
     assert A.attend(b.q[:0], b.cache, b.pages[:0], b.lengths[:0]).shape == (0, 4, 64)
