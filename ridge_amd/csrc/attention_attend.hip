@@ -460,17 +460,23 @@ __device__ __forceinline__ Share shareOf(const AttendArgs& a, uint32_t block, ui
         length = a.lengths[from + lane];
         return Range(length, a.capacity, a.window).share();
     };
-    auto sum = [&](uint32_t v) {   // of this lane and those before it
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint32_t before = __shfl_up(v, d);
-            v += lane >= d ? before : 0;
-        }
+    auto sum = [&](uint32_t v) {   // of this lane and those before it: in rows of 16 lanes, then rows
+        auto from = [&](auto control, auto rows) {
+            return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(control)::value, decltype(rows)::value, 15, false);
+        };
+        typedef std::integral_constant<int, 15> All;
+        v += from(std::integral_constant<int, 0x111>(), All());   // 1, 2, 4 and 8 lanes before
+        v += from(std::integral_constant<int, 0x112>(), All());
+        v += from(std::integral_constant<int, 0x114>(), All());
+        v += from(std::integral_constant<int, 0x118>(), All());
+        v += from(std::integral_constant<int, 0x142>(), std::integral_constant<int, 10>());   // the row's last before
+        v += from(std::integral_constant<int, 0x143>(), std::integral_constant<int, 12>());   // lane 31
         return v;
     };
+    auto lastOf = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1); };
     uint32_t total = 0, before = sum(load(0));
     for (int from = 0;;) {
-        total += uniform(__shfl(before, kWave - 1));
+        total += lastOf(before);
         if ((from += kWave) >= a.batch) break;
         before = sum(load(from));
     }
@@ -485,14 +491,14 @@ __device__ __forceinline__ Share shareOf(const AttendArgs& a, uint32_t block, ui
     int from = 0;
     if (a.batch > kWave) before = sum(load(0));
     while (true) {
-        const uint32_t here = uniform(__shfl(before, kWave - 1));
+        const uint32_t here = lastOf(before);
         if (passed + here > sought) break;
         passed += here;
         from += kWave;
         before = sum(load(from));
     }
     const int behind = uniform(__builtin_ctzll(__builtin_amdgcn_ballot_w64(passed + before > sought)));
-    if (behind) passed += uniform(__shfl(before, behind - 1));
+    if (behind) passed += (uint32_t)__builtin_amdgcn_readlane((int)before, behind - 1);
     share.b = from + behind;
     const uint32_t in = share.first - passed * heads;
     share.length = __builtin_amdgcn_readlane(length, behind);
