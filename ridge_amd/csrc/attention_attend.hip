@@ -242,7 +242,11 @@ struct Part {
                     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[i][j][e]));
             down = max(-96, exponentOf(most4(most)) - 14);
         }
-        const float up = a.scale < 0.0f ? -power2(-down) : power2(-down);
+        // qScale is never 0, as a masked score of -inf stays one; what it lacks below FLT_MIN = 2^-126, all
+        // of it for a scale of 0, is the query's.
+        const float wanted = ldexpf(fabsf(a.scale), down - kByteExponent);
+        qScale = fmaxf(wanted, FLT_MIN);
+        const float up = copysignf(power2(-down) * fminf(1.0f, wanted * power2(126)), a.scale);
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
 #pragma unroll
@@ -258,8 +262,6 @@ struct Part {
                         if constexpr (kSplitQ) qLow[i][j][e + n] = (_Float16)rest[n];
                     }
                 }
-        // Never 0: a masked score of -inf stays one.
-        qScale = fmaxf(ldexpf(fabsf(a.scale), down - kByteExponent), FLT_MIN);
     }
 
     // The blocks of the 32 tokens from t on; those behind `lastBlock` are that one, which is masked.

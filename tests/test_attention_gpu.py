@@ -422,6 +422,14 @@ def test_scales(scale):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_a_scale_of_zero_weighs_all_tokens_alike(dtype):
+    """Whatever the keys: times a scale of 0 in place of f32's smallest, they would count by some hundredths."""
+    b = Batch([300, 1, 700, 0], 8, 2, 128, 16, dtype)
+    b.cache[1].mul_(1e38)
+    b.check(scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_scores_and_values_of_any_size(dtype):
     """Softmaxes of one token, scores far from zero, values of all magnitudes in one sequence."""
     b = Batch([700, 300, 40], 8, 2, 128, 16, dtype)
