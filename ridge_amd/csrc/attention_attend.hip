@@ -6,8 +6,11 @@
 // in one pass over the cache, whose bytes bound it: a workgroup takes one key head of a part of a
 // sequence, its four waves 32 tokens at a time in turn, and each wave keeps the running maximum
 // and sum of the softmax and the weighted values of up to 16 query heads that share the key head.
-// Both products are matrix instructions (16 x 16 x 32, f16): 8-bit whole numbers are exact in f16,
-// a query in 16 bits is too (of f32, and of p, two f16 parts are taken), and sums are f32.
+// Both products are matrix instructions (16 x 16 x 32) with sums in f32, and 8-bit whole numbers are exact in
+// them. Scores are f16 products (a query of f32 is two parts of them). p vScale, of 24 bits and any size, is
+// three parts of bf16, and values are bf16: two parts of f16 would take 4 instructions less for 8 values and
+// 269 us, not 273, for 64 x 16384 tokens, but beside the largest scale they hold 2^-40 of it, and values beside
+// a far larger one lost their bits, whatever its p.
 //
 // No operand goes through LDS or moves between lanes. The scores are computed transposed, keys as
 // rows and heads as columns, so that a lane ends with 4 tokens of each 16 for one head; those are
@@ -31,6 +34,7 @@ using ridge::uniformLoad;
 
 typedef _Float16 Half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
+typedef __bf16 Brain8 __attribute__((ext_vector_type(8)));
 typedef float Float4 __attribute__((ext_vector_type(4)));
 typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
 
@@ -130,6 +134,21 @@ __device__ __forceinline__ Half8 join(Half2 a, Half2 b, Half2 c, Half2 d) {
     return Half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// The upper halves of two floats: as bf16 they are the floats but for their last 16 bits.
+__device__ __forceinline__ uint32_t tops(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+// Two bf16 of the whole numbers in byte `byte` of two words.
+__device__ __forceinline__ uint32_t wholes(uint32_t a, uint32_t b, int byte) {
+    return tops((float)(int8_t)(a >> 8 * byte), (float)(int8_t)(b >> 8 * byte));
+}
+// What a float's upper half leaves: exact, so that three halves in turn are all of its 24 bits. (Not
+// joined with a product that the float is: that would be the remainder of another number.)
+__device__ __forceinline__ float restOf(float v) {
+#pragma clang fp contract(off)
+    return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+}
+
 // Where a wave's 32 tokens are: two blocks of 16, each in one page. The same for all its lanes.
 struct Blocks {
     uint32_t page[2], in[2];   // the cache's page, and the first token in it
@@ -169,15 +188,18 @@ __device__ __forceinline__ void loadWords(uint32_t (&to)[n], __amdgpu_buffer_rsr
     }
 }
 
-// One wave's tokens of a part of a sequence, for 16 query heads. Probabilities are relative:
-// 2^(score - from), which is 2^15 / unit for the largest score, so that times a value's scale they are
-// at most 2^15.
+// One wave's tokens of a part of a sequence, for 16 query heads. Probabilities are relative,
+// 2^(score - from), 1 for the largest score; the sum of them goes by nothing else. The sums of values are
+// of scales times 2^-exponent, which is 0 but where the largest scale so far is far from one:
+// they have room for 2^31 tokens of any scale, and the three parts of p times a scale of FLT_MIN are
+// normal numbers as well.
 template <typename T, int COLS>
 struct Part {
     static constexpr int kKeys = Tile<COLS>::kKeys;
     static constexpr int kBytes = COLS / 16;       // of a value that a lane loads, and sums of 16 columns that it holds 4 of
     static constexpr bool kSplitQ = sizeof(T) == 4;
-    static constexpr int kLeastExponent = -90;     // of unit: sums of 2^15 / unit stay in f32's range
+    static constexpr int kSmall = -40, kLarge = 47;                    // exponents,
+    static constexpr float kMostSmall = 0x1p-40f, kMostPlain = 0x1p80f;   // of scales up to this, and past that
     typedef typename ridge::Memory<T, 8>::Vec Vec;
 
     const AttendArgs& a;
@@ -186,13 +208,13 @@ struct Part {
     float qScale;                                  // of scores, to powers of two
     Float4 sum[kBytes];                            // of value columns kBytes (4 group + r) + i, for head `at`
     float top, from, total;                        // the largest score, and this lane's part of the sum of p
-    float unit;                                    // a power of two above every value's scale so far
-    int exponent;                                  // of unit
+    float most;                                    // of scales that the exponent is for
+    int exponent;                                  // of the sums; the same for all lanes
 
     __device__ Part(const AttendArgs& a, int lane) : a(a), lane(lane) {}
 
     __device__ __forceinline__ void clear() {
-        top = from = -INFINITY, total = 0.0f, exponent = kLeastExponent, unit = power2(kLeastExponent);
+        top = from = -INFINITY, total = 0.0f, exponent = kSmall, most = kMostSmall;
 #pragma unroll
         for (int j = 0; j < kBytes; ++j) sum[j] = 0.0f;
     }
@@ -369,54 +391,59 @@ struct Part {
                     tile.vScale[b][r] = counts ? tile.vScale[b][r] : 0.0f;
                 }
         }
-        float most = s[0][0], scale = fabsf(tile.vScale[0][0]);
+        float highest = s[0][0], scale = fabsf(tile.vScale[0][0]);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) most = fmaxf(most, s[b][r]), scale = fmaxf(scale, fabsf(tile.vScale[b][r]));
-        // Few tiles have a new maximum or a new largest scale: the sums are rescaled in a branch.
-        if (__builtin_amdgcn_ballot_w64(most > top || scale > unit)) {
-            scale = most4(scale);   // the 16 heads' lanes have the same tokens
-            if (scale > unit) exponent = min(127, exponentOf(scale) + 1), unit = power2(exponent);
+            for (int r = 0; r < 4; ++r) highest = fmaxf(highest, s[b][r]), scale = fmaxf(scale, fabsf(tile.vScale[b][r]));
+        // Few tiles have a new maximum or a scale that wants another exponent: the sums are rescaled in a branch.
+        if (__builtin_amdgcn_ballot_w64(highest > top || scale > most)) {
+            const int before = exponent;
+            if (__builtin_amdgcn_ballot_w64(scale > most)) {   // the 16 heads' lanes have the same tokens
+                const bool large = __builtin_amdgcn_ballot_w64(scale > kMostPlain);
+                exponent = large ? kLarge : 0, most = large ? INFINITY : kMostPlain;
+            }
             const bool none = top == -INFINITY;
-            top = fmaxf(top, most4(most));
-            const float now = top == -INFINITY ? -INFINITY : fmaf(top, qScale, (float)(exponent - 15));
-            const float factor = none ? 0.0f : __builtin_amdgcn_exp2f(from - now);
+            top = fmaxf(top, most4(highest));
+            const float now = top == -INFINITY ? -INFINITY : top * qScale;
+            const float factor = none ? 0.0f : __builtin_amdgcn_exp2f(from - now), down = factor * power2(before - exponent);
             from = now;
             total *= factor;
 #pragma unroll
-            for (int i = 0; i < kBytes; ++i) sum[i] *= factor;
+            for (int i = 0; i < kBytes; ++i) sum[i] *= down;
+        }
+        if (exponent) {
+            const float down = power2(-exponent);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) tile.vScale[b] *= down;
         }
         const float least = top == -INFINITY ? 0.0f : from;
-        Half8 high, low;
+        Word4 high, middle, low;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {
-                float weight[2], rest[2];
+                float weight[2];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(s[b][r + n], qScale, -least));
                     total += p;
                     weight[n] = p * tile.vScale[b][r + n];
                 }
-                Half2 both;
-                split(weight[0], weight[1], both, rest[0], rest[1]);
-#pragma unroll
-                for (int n = 0; n < 2; ++n) high[4 * b + r + n] = both[n], low[4 * b + r + n] = (_Float16)rest[n];
+                const int at = 2 * b + r / 2;
+                high[at] = tops(weight[0], weight[1]);
+                for (float& w : weight) w = restOf(w);
+                middle[at] = tops(weight[0], weight[1]);
+                for (float& w : weight) w = restOf(w);
+                low[at] = tops(weight[0], weight[1]);
             }
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int i = 0; i < Tile<COLS>::kWords; ++i) tile.v[b][r][i] ^= 0x80808080u;
-#pragma unroll
         for (int i = 0; i < kBytes; ++i) {
-            auto pair = [&](int b, int r) { return halves(tile.v[b][r + 1][i / 4], tile.v[b][r][i / 4], i % 4, i % 4); };
-            const Half8 values = join(pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2));
-            sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, high, sum[i], 0, 0, 0);
-            sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values, low, sum[i], 0, 0, 0);
+            auto pair = [&](int b, int r) { return wholes(tile.v[b][r][i / 4], tile.v[b][r + 1][i / 4], i % 4); };
+            const Word4 values = {pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2)};
+            for (const Word4& part : {high, middle, low})
+                sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Brain8, values),
+                                                                 __builtin_bit_cast(Brain8, part), sum[i], 0, 0, 0);
         }
     }
 };
@@ -609,13 +636,15 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
             t = next;
         }
         // The waves' sums, from the largest `from` on, are added in their order.
-        p.total = sum4(p.total);
+        // (With the exponent in both, the sum of p is relative to what the sums are.)
+        p.total = sum4(p.total) * power2(-p.exponent);
+        p.from += (float)p.exponent;
         if (p.group == 0) froms[wave][p.at] = p.from, totals[wave][p.at] = p.total;
         __syncthreads();   // and the keys' LDS becomes the sums'
         float most = froms[0][p.at];
 #pragma unroll
         for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, froms[w][p.at]);
-        const float factor = __builtin_amdgcn_exp2f(p.from - (most == -INFINITY ? 0.0f : most) - kByteExponent);
+        const float factor = __builtin_amdgcn_exp2f(p.from - (most == -INFINITY ? 0.0f : most));
         if (p.at < count) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)

@@ -1,0 +1,103 @@
+"""attend where values, scales and scores lie far apart, against 64 bits.
+
+Tolerances. u = 2^-24 is half a unit of f32. A score is a sum of D products, at most D + 6 roundings of the
+sum of their magnitudes; as the exponent of p it carries that as a relative error, with 4 u of
+its own size and of the maximum's. p carries 4 u more, its product with a value's scale u, and sums of three
+parts of n terms 3 n u. out's numerator and denominator each carry that, relative to the sum of
+|p v|; a p below 2^-126 of the largest (2^-78 beside scales past 2^80) may count nothing, which is within
+that many times the sum of |v|.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from ridge_amd import attention as A  # noqa: E402
+from test_attention_gpu import DEV, TYPES, U, Batch, _close  # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    A.lib()
+    yield
+    torch.cuda.synchronize()
+
+
+def _check(b, scale=None, lost=2.0 ** -126, query=0.0):
+    """attend of a Batch against 64 bits: lost, the p that may count nothing; query, what a query's columns lose."""
+    B, H, D = b.q.shape
+    lse = torch.empty((B, H), device=DEV)
+    got = A.attend(b.q, b.cache, b.pages, b.lengths, scale=scale, lse_out=lse)
+    scale = D ** -0.5 if scale is None else scale
+    for i, n in enumerate(b.sizes):
+        if n == 0:
+            continue
+        k, v = b.rows(i)
+        q = b.q[i].double().reshape(k.shape[0], -1, D)
+        s = q @ k.transpose(1, 2).contiguous() * scale
+        most = q.abs() @ k.abs().transpose(1, 2).contiguous() * abs(scale)
+        p = torch.softmax(s, dim=2)
+        off = ((D + 6) * U + query) * most + 4 * U * (s.abs() + s.amax(dim=2, keepdim=True).abs()) + (5 + 3 * n) * U
+        mass = (p * off).sum(dim=2, keepdim=True) + lost * n
+        slack = (p * off) @ v.abs() + mass * (p @ v.abs()) + lost * v.abs().sum(dim=1, keepdim=True)
+        _close(got[i], (p @ v).reshape(H, D), slack.reshape(H, D), b.q.dtype)
+        want = torch.logsumexp(s, dim=2).reshape(H)
+        assert bool(((lse[i].double() - want).abs() <= mass.reshape(H) + 8 * U * want.abs() + 4 * U).all())
+    return got
+
+
+def _tokens(b, i, where):
+    """(pages, offsets) of the tokens of sequence i where `where` (of a token's number) is true."""
+    t = torch.tensor([t for t in range(b.sizes[i]) if where(t)], device=DEV)
+    P = b.cache[0].shape[2]
+    return b.pages[i].long()[t // P], t % P
+
+
+# What a query of f32 loses where it is held in two parts of f16.
+QUERY = {torch.float16: 0.0, torch.bfloat16: 0.0, torch.float32: 2.0 ** -22}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("power", [10, 20, 24, 31, 34, 38, 42, 60, 100])
+def test_a_far_larger_value_of_no_weight_hides_nothing(power, dtype):
+    for heads, kv_heads, dim in ((8, 2, 128), (3, 1, 64), (2, 1, 256)):
+        b = Batch([700, 300, 40, 3000], heads, kv_heads, dim, 16, dtype)
+        b.q[..., 0] = 16
+        b.cache[0][..., 0] = 0
+        for i, t in ((0, 5), (0, 650), (1, 299), (2, 0), (3, 1500)):
+            at = _tokens(b, i, lambda x: x == t)
+            b.cache[0][at[0], :, at[1]] = 0
+            b.cache[0][at[0], :, at[1], 0] = -127
+            b.cache[1][at[0], :, at[1]] = 1.0           # scores of 16 * 127 / 16 and less below the others
+            b.cache[3][at[0], :, at[1]] = 0.02 * 2.0 ** power
+        _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78, query=QUERY[dtype])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [30, 36, 40, 70, 90, 110])
+def test_rows_of_zeros_keep_their_weight_beside_large_values(power, dtype):
+    """Equal scores: the rows of zeros, whose scale is the least there is, count as much as the others,
+    be they in a tile before, in another wave's, or in another piece."""
+    for first in (32, 128, 256, 2000):
+        b = Batch([first + 32, first + 200, 2 * first + 5000], 4, 2, 128, 16, dtype)
+        b.q.zero_()
+        for i in range(3):
+            at = _tokens(b, i, lambda t: t < first)
+            b.cache[2][at[0], :, at[1]] = 0
+            b.cache[3][at[0], :, at[1]] = 2.0 ** -126
+            at = _tokens(b, i, lambda t: t >= first)
+            b.cache[3][at[0], :, at[1]] = 2.0 ** power
+        _check(b, lost=2.0 ** -126 if power < 80 else 2.0 ** -78)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [-105, -60, -39, -33, 86, 119])
+def test_values_that_are_all_tiny_or_huge(power, dtype):
+    b = Batch([700, 1, 40, 5000], 8, 2, 128, 16, dtype)
+    b.cache[3].mul_(2.0 ** power)
+    _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78, query=QUERY[dtype])
