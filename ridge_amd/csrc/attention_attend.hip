@@ -6,11 +6,11 @@
 // in one pass over the cache, whose bytes bound it: a workgroup takes one key head of a part of a
 // sequence, its four waves 32 tokens at a time in turn, and each wave keeps the running maximum
 // and sum of the softmax and the weighted values of up to 16 query heads that share the key head.
-// Both products are matrix instructions (16 x 16 x 32) with sums in f32, and 8-bit whole numbers are exact in
-// them. Scores are f16 products (a query of f32 is two parts of them). p vScale, of 24 bits and any size, is
-// three parts of bf16, and values are bf16: two parts of f16 would take 4 instructions less for 8 values and
-// 269 us, not 273, for 64 x 16384 tokens, but beside the largest scale they hold 2^-40 of it, and values beside
-// a far larger one lost their bits, whatever its p.
+// Both products are matrix instructions (16 x 16 x 32) with sums in f32, and no operand of them is rounded:
+// 8-bit whole numbers are exact in bf16 and f16. A query of f16 or bf16 is of its own type, one of f32 three
+// parts of bf16, and so is p vScale, which has 24 bits and any size. In one or two parts of f16 (64 x 16384
+// tokens 270 us for 279, in f32 286 for 311) a query's columns 2^-32 of its largest lost their bits,
+// and values beside a far larger one, whatever its p.
 //
 // No operand goes through LDS or moves between lanes. The scores are computed transposed, keys as
 // rows and heads as columns, so that a lane ends with 4 tokens of each 16 for one head; those are
@@ -110,24 +110,13 @@ __device__ __forceinline__ float sum4(float v) {
 __device__ __forceinline__ float power2(int n) { return __int_as_float((n + 127) << 23); }
 __device__ __forceinline__ int exponentOf(float v) { return (int)(__float_as_uint(v) >> 23 & 255) - 127; }
 
-// Two f16 of the whole numbers in bytes `lo` of low and `hi` of high (biased by 128), times 2^-9:
+// Two f16 of the whole numbers in bytes `lo` of low and `hi` of high (biased by 128), times 2^-9, in 5
+// instructions for 4 where bf16 takes 6:
 // the byte as a f16 below the normal ones is its 2^-24th, which the product lifts and the sum unbiases.
 __device__ __forceinline__ Half2 halves(uint32_t high, uint32_t low, int hi, int lo) {
     const uint32_t both = __builtin_amdgcn_perm(high, low, 0x0c000c00u | (uint32_t)(4 + hi) << 16 | (uint32_t)lo);
     const Half2 lift = {(_Float16)32768.0f, (_Float16)32768.0f}, bias = {(_Float16)-0.25f, (_Float16)-0.25f};
     return __builtin_elementwise_fma(__builtin_bit_cast(Half2, both), lift, bias);
-}
-constexpr int kByteExponent = -9;
-
-// Two values in f16, and what they leave. The compiler may convert a product with one rounding at one
-// place and with two at another: the empty statement has the remainder taken of what was in fact
-// rounded (without it a few heads in 1000 had a p off by 2^-11).
-__device__ __forceinline__ void split(float a, float b, Half2& high, float& restA, float& restB) {
-    uint32_t both = __builtin_bit_cast(uint32_t, Half2{(_Float16)a, (_Float16)b});
-    asm("" : "+v"(both));
-    high = __builtin_bit_cast(Half2, both);
-    restA = a - (float)high.x;
-    restB = b - (float)high.y;
 }
 
 __device__ __forceinline__ Half8 join(Half2 a, Half2 b, Half2 c, Half2 d) {
@@ -138,9 +127,9 @@ __device__ __forceinline__ Half8 join(Half2 a, Half2 b, Half2 c, Half2 d) {
 __device__ __forceinline__ uint32_t tops(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
-// Two bf16 of the whole numbers in byte `byte` of two words.
-__device__ __forceinline__ uint32_t wholes(uint32_t a, uint32_t b, int byte) {
-    return tops((float)(int8_t)(a >> 8 * byte), (float)(int8_t)(b >> 8 * byte));
+// Two bf16 of the whole numbers in bytes i of a and j of b.
+__device__ __forceinline__ uint32_t wholes(uint32_t a, int i, uint32_t b, int j) {
+    return tops((float)(int8_t)(a >> 8 * i), (float)(int8_t)(b >> 8 * j));
 }
 // What a float's upper half leaves: exact, so that three halves in turn are all of its 24 bits. (Not
 // joined with a product that the float is: that would be the remainder of another number.)
@@ -197,14 +186,16 @@ template <typename T, int COLS>
 struct Part {
     static constexpr int kKeys = Tile<COLS>::kKeys;
     static constexpr int kBytes = COLS / 16;       // of a value that a lane loads, and sums of 16 columns that it holds 4 of
-    static constexpr bool kSplitQ = sizeof(T) == 4;
+    static constexpr bool kHalf = std::is_same_v<T, _Float16>;
+    static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;   // of a query: bf16, or f16 where it is that
+    static constexpr int kByteExponent = kHalf ? -9 : 0;    // of keys
     static constexpr int kSmall = -40, kLarge = 47;                    // exponents,
     static constexpr float kMostSmall = 0x1p-40f, kMostPlain = 0x1p80f;   // of scales up to this, and past that
     typedef typename ridge::Memory<T, 8>::Vec Vec;
 
     const AttendArgs& a;
     const int lane, at = lane % 16, group = lane / 16;
-    Half8 q[kKeys][2], qLow[kSplitQ ? kKeys : 1][2];
+    Word4 q[kParts][kKeys][2];
     float qScale;                                  // of scores, to powers of two
     Float4 sum[kBytes];                            // of value columns kBytes (4 group + r) + i, for head `at`
     float top, from, total;                        // the largest score, and this lane's part of the sum of p
@@ -241,8 +232,10 @@ struct Part {
             }
     }
 
-    // Its fragments. A head of bf16 or f32 is scaled by a power of two so that its largest column is
-    // 2^14 to 2^15. A negative scale turns the query, so that the largest score has the largest p.
+    // Its fragments, in bf16 or f16 without a rounding (of a scale that has all its bits). A head of bf16 or
+    // f32 is taken times a power of two so that its largest column is about 2^14, or what keeps
+    // qScale a number where the scale is far from one. A negative scale turns the query, so that the
+    // largest score has the largest p.
     __device__ __forceinline__ void setQuery(const Query& query) {
         float x[kKeys][2][8];
 #pragma unroll
@@ -253,20 +246,22 @@ struct Part {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[i][j][e] = has ? (float)query.x[i][j][e] : 0.0f;
             }
-        float most = 0.0f;
+        // qScale is never 0, as a masked score of -inf stays one: of a scale of 0 the query is.
+        const float scale = fabsf(a.scale);
         int down = 0;
-        if constexpr (!std::is_same_v<T, _Float16>) {
+        if constexpr (!kHalf) {
+            float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < kKeys; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[i][j][e]));
-            down = max(-96, exponentOf(most4(most)) - 14);
+            const int exponent = exponentOf(most4(most));
+            down = max(-96, exponent - 14);
         }
-        // qScale is never 0, as a masked score of -inf stays one; what it lacks below FLT_MIN = 2^-126, all
-        // of it for a scale of 0, is the query's.
-        const float wanted = ldexpf(fabsf(a.scale), down - kByteExponent);
+        // What a f16 query's qScale lacks below FLT_MIN is the query's.
+        const float wanted = ldexpf(scale, down - kByteExponent);
         qScale = fmaxf(wanted, FLT_MIN);
         const float up = copysignf(power2(-down) * fminf(1.0f, wanted * power2(126)), a.scale);
 #pragma unroll
@@ -275,13 +270,15 @@ struct Part {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    Half2 high;
-                    float rest[2];
-                    split(x[i][j][e] * up, x[i][j][e + 1] * up, high, rest[0], rest[1]);
+                    float u = x[i][j][e] * up, w = x[i][j][e + 1] * up;
+                    if constexpr (kHalf) {
+                        q[0][i][j][e / 2] = __builtin_bit_cast(uint32_t, Half2{(_Float16)u, (_Float16)w});
+                    } else {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        q[i][j][e + n] = high[n];
-                        if constexpr (kSplitQ) qLow[i][j][e + n] = (_Float16)rest[n];
+                        for (int n = 0; n < kParts; ++n) {
+                            q[n][i][j][e / 2] = tops(u, w);
+                            u = restOf(u), w = restOf(w);
+                        }
                     }
                 }
     }
@@ -364,13 +361,20 @@ struct Part {
             Float4 score = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < kKeys; ++i) {
-                const Word4 w = k[b][i] ^ 0x80808080u;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t x = w[2 * j], y = w[2 * j + 1];
-                    const Half8 keys = join(halves(x, x, 1, 0), halves(x, x, 3, 2), halves(y, y, 1, 0), halves(y, y, 3, 2));
-                    score = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, q[i][j], score, 0, 0, 0);
-                    if constexpr (kSplitQ) score = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, qLow[i][j], score, 0, 0, 0);
+                    if constexpr (kHalf) {
+                        const uint32_t x = k[b][i][2 * j] ^ 0x80808080u, y = k[b][i][2 * j + 1] ^ 0x80808080u;
+                        const Half8 keys = join(halves(x, x, 1, 0), halves(x, x, 3, 2), halves(y, y, 1, 0), halves(y, y, 3, 2));
+                        score = __builtin_amdgcn_mfma_f32_16x16x32_f16(keys, __builtin_bit_cast(Half8, q[0][i][j]), score, 0, 0, 0);
+                    } else {
+                        const uint32_t x = k[b][i][2 * j], y = k[b][i][2 * j + 1];
+                        const Word4 keys = {wholes(x, 0, x, 1), wholes(x, 2, x, 3), wholes(y, 0, y, 1), wholes(y, 2, y, 3)};
+#pragma unroll
+                        for (int n = 0; n < kParts; ++n)
+                            score = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Brain8, keys),
+                                                                            __builtin_bit_cast(Brain8, q[n][i][j]), score, 0, 0, 0);
+                    }
                 }
             }
 #pragma unroll
@@ -439,7 +443,7 @@ struct Part {
             }
 #pragma unroll
         for (int i = 0; i < kBytes; ++i) {
-            auto pair = [&](int b, int r) { return wholes(tile.v[b][r][i / 4], tile.v[b][r + 1][i / 4], i % 4); };
+            auto pair = [&](int b, int r) { return wholes(tile.v[b][r][i / 4], i % 4, tile.v[b][r + 1][i / 4], i % 4); };
             const Word4 values = {pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2)};
             for (const Word4& part : {high, middle, low})
                 sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Brain8, values),

@@ -1,7 +1,7 @@
 """attend where values, scales and scores lie far apart, against 64 bits.
 
-Tolerances. u = 2^-24 is half a unit of f32. A score is a sum of D products, at most D + 6 roundings of the
-sum of their magnitudes; as the exponent of p it carries that as a relative error, with 4 u of
+Tolerances. u = 2^-24 is half a unit of f32. A score is a sum of D exact products (of 3 D for a query of f32,
+whose columns are three parts of bf16), at most as many roundings and 6 of the sum of their magnitudes; as the exponent of p it carries that as a relative error, with 4 u of
 its own size and of the maximum's. p carries 4 u more, its product with a value's scale u, and sums of three
 parts of n terms 3 n u. out's numerator and denominator each carry that, relative to the sum of
 |p v|; a p below 2^-126 of the largest (2^-78 beside scales past 2^80) may count nothing, which is within
@@ -28,8 +28,8 @@ def _gpu():
     torch.cuda.synchronize()
 
 
-def _check(b, scale=None, lost=2.0 ** -126, query=0.0):
-    """attend of a Batch against 64 bits: lost, the p that may count nothing; query, what a query's columns lose."""
+def _check(b, scale=None, lost=2.0 ** -126):
+    """attend of a Batch against 64 bits: lost, the p that may count nothing."""
     B, H, D = b.q.shape
     lse = torch.empty((B, H), device=DEV)
     got = A.attend(b.q, b.cache, b.pages, b.lengths, scale=scale, lse_out=lse)
@@ -42,7 +42,8 @@ def _check(b, scale=None, lost=2.0 ** -126, query=0.0):
         s = q @ k.transpose(1, 2).contiguous() * scale
         most = q.abs() @ k.abs().transpose(1, 2).contiguous() * abs(scale)
         p = torch.softmax(s, dim=2)
-        off = ((D + 6) * U + query) * most + 4 * U * (s.abs() + s.amax(dim=2, keepdim=True).abs()) + (5 + 3 * n) * U
+        products = 3 * D if b.q.dtype == torch.float32 else D
+        off = (products + 6) * U * most + 4 * U * (s.abs() + s.amax(dim=2, keepdim=True).abs()) + (5 + 3 * n) * U
         mass = (p * off).sum(dim=2, keepdim=True) + lost * n
         slack = (p * off) @ v.abs() + mass * (p @ v.abs()) + lost * v.abs().sum(dim=1, keepdim=True)
         _close(got[i], (p @ v).reshape(H, D), slack.reshape(H, D), b.q.dtype)
@@ -58,10 +59,6 @@ def _tokens(b, i, where):
     return b.pages[i].long()[t // P], t % P
 
 
-# What a query of f32 loses where it is held in two parts of f16.
-QUERY = {torch.float16: 0.0, torch.bfloat16: 0.0, torch.float32: 2.0 ** -22}
-
-
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("power", [10, 20, 24, 31, 34, 38, 42, 60, 100])
 def test_a_far_larger_value_of_no_weight_hides_nothing(power, dtype):
@@ -75,7 +72,7 @@ def test_a_far_larger_value_of_no_weight_hides_nothing(power, dtype):
             b.cache[0][at[0], :, at[1], 0] = -127
             b.cache[1][at[0], :, at[1]] = 1.0           # scores of 16 * 127 / 16 and less below the others
             b.cache[3][at[0], :, at[1]] = 0.02 * 2.0 ** power
-        _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78, query=QUERY[dtype])
+        _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -100,4 +97,22 @@ def test_rows_of_zeros_keep_their_weight_beside_large_values(power, dtype):
 def test_values_that_are_all_tiny_or_huge(power, dtype):
     b = Batch([700, 1, 40, 5000], 8, 2, 128, 16, dtype)
     b.cache[3].mul_(2.0 ** power)
-    _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78, query=QUERY[dtype])
+    _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78)
+
+
+@pytest.mark.parametrize("dtype,power", [(torch.float16, 10), (torch.float16, 20)] +
+                         [(t, p) for t in TYPES[1:] for p in (10, 20, 32, 40, 60, 100)])
+def test_a_querys_large_column_hides_no_other(dtype, power):
+    """The keys are 0 where the query is large, and its other columns are 2^-power of that."""
+    for heads, kv_heads, dim in ((8, 2, 128), (3, 1, 40), (2, 1, 256)):
+        b = Batch([700, 300, 40, 3000], heads, kv_heads, dim, 16, dtype)
+        b.q.copy_(b.q.double() * 2.0 ** -power)
+        b.q[..., 3] = 1.5
+        b.cache[0][..., 3] = 0
+        for sign in (1, -1):
+            _check(b, scale=sign * dim ** -0.5 * 2.0 ** power)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (3, 1, 64), (2, 1, 256), (5, 1, 33)])
+def test_queries_of_32_bits_count_with_all_of_them(heads, kv_heads, dim):
+    _check(Batch([700, 1, 300, 40, 3000], heads, kv_heads, dim, 16, torch.float32))
