@@ -335,8 +335,14 @@ struct Part {
     }
 
     // Keys go through LDS of the wave's own, from whole rows to the 16 bytes of a token that a lane's
-    // scores take; chunks of a row are swapped so that neither side meets another lane's bank.
+    // scores take; chunks of a row are swapped so that neither side meets another lane's bank. A wave's
+    // accesses of LDS are done in their order, so the lanes wait for nothing: the compiler alone is told, before
+    // a lane reads what another one wrote and before it writes where another one read.
     static constexpr bool kThroughLds = COLS > 64;
+    __device__ static __forceinline__ void handOver() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+    }
     __device__ static __forceinline__ int swap(int row) { return COLS == 128 ? row / 2 % 8 : row % 16; }
     __device__ __forceinline__ void putKeys(const Tile<COLS>& tile, Word4* lds) const {
         constexpr int kChunks = Tile<COLS>::kChunks, kRows = kWave / kChunks;
@@ -625,13 +631,17 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
             const Float4 scales[2] = {tile.kScale[0], tile.kScale[1]};
             if constexpr (Part<T, COLS>::kThroughLds) {
                 p.putKeys(tile, keys);
+                p.handOver();
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) own[h][0] = tile.k[h];
             }
             const Blocks ahead = p.find(next + kRound, lastBlock, pages);
             if (next < to) p.loadKeys(tile, blocks, k, kScale);
-            if constexpr (Part<T, COLS>::kThroughLds) p.getKeys(own, keys);
+            if constexpr (Part<T, COLS>::kThroughLds) {
+                p.getKeys(own, keys);
+                p.handOver();
+            }
             float s[2][4];
             p.score(own, scales, s);
             p.add(tile, s, t, range.begin, to);
