@@ -178,7 +178,8 @@ def attend(q, cache, pages, lengths, scale=None, window=None, lse_out=None, out=
     """out [sequences, heads, columns]: for each head of q, the softmax of scale * (q . k_t) over
     the sequence's tokens t, times v_t. Sequence b has lengths[b] tokens, the new one among them,
     in the pages pages[b]; key head h / (q's heads / the cache's) serves query head h. window:
-    only the last that many tokens. scale is 1 / sqrt(columns) by default. lse_out (float32
+    only the last that many tokens. scale is 1 / sqrt(columns) by default (2^118 at the most for
+    float16). lse_out (float32
     [sequences, heads]) gets the logarithm of the sum of exp(scale * (q . k_t)), by which the
     results over two parts of a sequence are joined. A sequence of no tokens gives zeros, and
     -inf in lse_out. Narrow `pages` to the longest sequence: its columns are what a launch is

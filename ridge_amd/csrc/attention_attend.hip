@@ -60,7 +60,8 @@ struct AttendArgs {
     uint32_t pageMagic, pageShift;                 // block / pageBlocks is 16 block times pageMagic, shifted by 32 + pageShift
     int32_t capacity, window, batch, heads, kvHeads, dim, tiles, tileHeads;   // tileHeads: the most of a tile
     int32_t shared, byHead;   // query heads of a key head; whether `ends` are the heads'
-    float scale;           // times log2(e): exponentials are powers of two
+    float scale;           // times log2(e), as exponentials are powers of two, and times 2^-scaleExponent: 1 to 2
+    int32_t scaleExponent;
 };
 
 // What a sequence's length says: its tokens [begin, end), and the rounds of a workgroup from `base` on
@@ -232,10 +233,10 @@ struct Part {
             }
     }
 
-    // Its fragments, in bf16 or f16 without a rounding (of a scale that has all its bits). A head of bf16 or
-    // f32 is taken times a power of two so that its largest column is about 2^14, or what keeps
-    // qScale a number where the scale is far from one. A negative scale turns the query, so that the
-    // largest score has the largest p.
+    // Its fragments, in bf16 or f16 without a rounding: the query times a power of two that makes the largest
+    // column of a bf16 or f32 head about 2^14, and that keeps qScale a normal number, whatever the scale
+    // (of f16 it is 1 but for scales below 2^-135, beside which small columns lose bits). A
+    // negative scale turns the query, so that the largest score has the largest p.
     __device__ __forceinline__ void setQuery(const Query& query) {
         float x[kKeys][2][8];
 #pragma unroll
@@ -246,8 +247,6 @@ struct Part {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[i][j][e] = has ? (float)query.x[i][j][e] : 0.0f;
             }
-        // qScale is never 0, as a masked score of -inf stays one: of a scale of 0 the query is.
-        const float scale = fabsf(a.scale);
         int down = 0;
         if constexpr (!kHalf) {
             float most = 0.0f;
@@ -259,11 +258,12 @@ struct Part {
                     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[i][j][e]));
             const int exponent = exponentOf(most4(most));
             down = max(-96, exponent - 14);
+            down = max(min(down, 126 - a.scaleExponent), exponent - 104);
         }
-        // What a f16 query's qScale lacks below FLT_MIN is the query's.
-        const float wanted = ldexpf(scale, down - kByteExponent);
-        qScale = fmaxf(wanted, FLT_MIN);
-        const float up = copysignf(power2(-down) * fminf(1.0f, wanted * power2(126)), a.scale);
+        down = max(down, -126 + kByteExponent - a.scaleExponent);
+        // Never 0, as a masked score of -inf stays one: of a scale of 0 the query is.
+        qScale = fmaxf(ldexpf(fabsf(a.scale), a.scaleExponent + down - kByteExponent), FLT_MIN);
+        const float up = a.scale == 0.0f ? 0.0f : copysignf(power2(-down), a.scale);
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
 #pragma unroll
@@ -830,7 +830,7 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
                                       int64_t batch, void* workspace, int64_t workspaceBytes, void* stream) {
     if (!ridge::isType(type) || !ridge::cacheFits(cache) || !ridge::headsFit(q, type, batch) ||
         !ridge::headsFit(out, type, batch) || q->heads != out->heads || !(std::fabs(scale) <= FLT_MAX / 2) || window < 0 ||
-        pagesStride < 0)
+        pagesStride < 0 || (type == RIDGE_F16 && std::fabs(scale) > 0x1p118f))
         return hipErrorInvalidValue;
     const int64_t wanted =
         ridge_attention_workspace(batch, q->heads, cache->heads, cache->dim, pagesEach, cache->pageSize);
@@ -856,6 +856,7 @@ extern "C" int ridge_attention_attend(const ridge_attention_heads_t* q, const ri
     a.shared = a.heads / a.kvHeads, a.tileHeads = std::min(kHeadTile, a.shared);
     const int64_t longest = a.window ? std::min(capacity, (int64_t)a.window + 15) : capacity;   // whole blocks of 16
     if (!eachItsOwn(batch, (int64_t)a.kvHeads * a.tiles, longest)) a.pieces = (float*)workspace;
-    a.scale = (float)(scale * 1.4426950408889634);
+    const double wide = scale * 1.4426950408889634;
+    a.scaleExponent = scale == 0.0f ? 0 : std::ilogb(wide), a.scale = (float)std::scalbn(wide, -a.scaleExponent);
     return ridge::typed(type, [&](auto element) { return launchTyped<decltype(element)>(a, (hipStream_t)stream); });
 }

@@ -436,6 +436,7 @@ PyObject* attendImpl(PyObject* const* args, Py_ssize_t n) {
         refuse("pages and lengths must have a row and a contiguous number for each of q's %lld", (long long)q.tokens);
     const double scale = args[4] == Py_None ? 1.0 / std::sqrt((double)q.dim) : number(args[4]);
     if (!(std::fabs((float)scale) <= FLT_MAX / 2)) refuse("scale must be finite, not %g", scale);
+    if (code == kF16 && std::fabs((float)scale) > 0x1p118f) refuse("scale must be 2^118 at the most for float16, not %g", scale);
     const int64_t window = args[5] == Py_None ? 0 : whole(args[5]);
     if (window < 0 || (window == 0 && args[5] != Py_None)) refuse("window must be positive, not %lld", (long long)window);
     const On on(device, args[8]);

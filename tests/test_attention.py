@@ -193,3 +193,12 @@ def test_without_torch_only_its_extension_is_left_out(monkeypatch, capsys):
     assert build.build_attention().endswith("libridge_attention.so")
     assert len(ran) == len(build.ATTENTION_SRCS) + 1 and not any("binding" in word for cmd in ran for word in cmd)
     assert "no torch" in capsys.readouterr().out
+
+
+def test_attend_refuses_scales_that_float16_has_no_scores_for():
+    def attend(type, scale):
+        return A.lib().ridge_attention_attend(_heads(), _cache(), P, 4, 4, P, scale, 0, _heads(), None, type, 3, None, 0, None)
+    for scale in (2.0 ** 119, -1.01 * 2.0 ** 118):
+        assert attend(0, scale) == INVALID
+    for type in (0, 1, 2):
+        assert attend(type, 2.0 ** 127) == INVALID

@@ -116,3 +116,30 @@ def test_a_querys_large_column_hides_no_other(dtype, power):
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (3, 1, 64), (2, 1, 256), (5, 1, 33)])
 def test_queries_of_32_bits_count_with_all_of_them(heads, kv_heads, dim):
     _check(Batch([700, 1, 300, 40, 3000], heads, kv_heads, dim, 16, torch.float32))
+
+
+FAR_SCALES = [(t, *powers) for t in TYPES[1:] for powers in ((104, 30, -126), (126, 0, -120), (-146, 16, 126), (-130, 0, 126), (-60, -60, 116))]
+
+
+@pytest.mark.parametrize("dtype,scale,query,key", FAR_SCALES + [(torch.float16, 118, -10, -108), (torch.float16, -140, 10, 126)])
+def test_scales_far_from_one(dtype, scale, query, key):
+    """Scores of some units, by a scale, query and keys of these powers of two; scores of 0 among them."""
+    b = Batch([700, 1, 40, 3000], 4, 2, 128, 16, dtype)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    b.q.zero_()
+    b.q[..., 5] = (1.5 + torch.rand(b.q.shape[:2], generator=g, device=DEV) / 2).to(dtype) * 2.0 ** query
+    most = max(1, min(127, int(2.0 ** -(scale + query + key))))
+    b.cache[0].copy_(torch.randint(-most, most + 1, b.cache[0].shape, generator=g, device=DEV))
+    b.cache[1][b.cache[1].isfinite()] = 2.0 ** key
+    for sign in (1, -1):
+        _check(b, scale=sign * 1.25 * 2.0 ** scale if scale < 118 else sign * 2.0 ** scale)
+
+
+def test_scales_without_scores_are_refused():
+    b = Batch([5], 4, 2, 64, 16, torch.float16)
+    for scale in (2.0 ** 119, -2.0 ** 119, 2.0 ** 127, math.inf):
+        with pytest.raises(A.RidgeAttentionError, match="scale"):
+            A.attend(b.q, b.cache, b.pages, b.lengths, scale=scale)
+    A.attend(b.q.bfloat16(), b.cache, b.pages, b.lengths, scale=2.0 ** 119)
+    with pytest.raises(A.RidgeAttentionError, match="scale"):
+        A.attend(b.q.bfloat16(), b.cache, b.pages, b.lengths, scale=2.0 ** 127)
