@@ -393,3 +393,53 @@ def test_the_command():
             "--steps", "3"]
     assert B.main(args) == 0
     assert B.main(args + ["--graph", "--dtype", "bfloat16", "--page-size", "16"]) == 0
+
+
+@pytest.mark.parametrize("handle", [False, True])
+def test_a_call_on_a_stream_has_its_memory_from_there(handle):
+    """The workspace and the result: the current stream, which runs ahead, is given none of it."""
+    b = Batch([3000, 100, 9000, 0], 8, 2, 64, 16, torch.float16)
+    bytes_ = A.lib().ridge_attention_workspace(4, 8, 2, 64, b.pages.shape[1], 16)
+    want = A.attend(b.q, b.cache, b.pages, b.lengths)
+    busy = torch.zeros((4096, 4096), device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    side = torch.cuda.Stream()
+
+    def held():
+        return sum(s["total_size"] for s in torch.cuda.memory_snapshot() if s["stream"] == side.cuda_stream)
+    before = held()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            for _ in range(8):
+                busy.add_(1)
+        got = A.attend(b.q, b.cache, b.pages, b.lengths, stream=side.cuda_stream if handle else side)
+        others = [torch.full((bytes_,), 255, dtype=torch.uint8, device=DEV) for _ in range(4)]
+        others += [torch.full_like(got, math.nan) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del others
+    assert bytes_ > 0 and held() - before >= bytes_
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+
+
+def test_functional_transforms_and_tensors_without_memory_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    o = _operands()
+    two = {n: torch.stack([t, t]) for n, t in o.items() if n != "cache"}
+    for name, call in (("q", _norm_rope), ("positions", _norm_rope), ("k", _write), ("slots", _write), ("slots", _read), ("q", _attend),
+                       ("lengths", _attend), ("pages", _attend)):
+        print(name, flush=True)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(lambda t: call(o, **{name: t}))(two[name])
+    for call in (lambda t: _norm_rope(o, q=t)[0], lambda t: _attend(o, q=t)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (o["q"],), (torch.ones_like(o["q"]),))
+        with pytest.raises(RuntimeError):
+            torch.func.vjp(call, o["q"])
+    with FakeTensorMode() as mode:
+        fake = {n: mode.from_tensor(t) for n, t in o.items() if n != "cache"}
+        fake["cache"] = tuple(mode.from_tensor(t) for t in o["cache"])
+        for call in (_norm_rope, _write, _read, _attend):
+            with pytest.raises(A.RidgeAttentionError):
+                call(fake)
