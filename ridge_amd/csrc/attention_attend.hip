@@ -190,8 +190,8 @@ struct Part {
     static constexpr bool kHalf = std::is_same_v<T, _Float16>;
     static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;   // of a query: bf16, or f16 where it is that
     static constexpr int kByteExponent = kHalf ? -9 : 0;    // of keys
-    static constexpr int kSmall = -40, kLarge = 47;                    // exponents,
-    static constexpr float kMostSmall = 0x1p-40f, kMostPlain = 0x1p80f;   // of scales up to this, and past that
+    static constexpr int kSmall = -40, kLarge = 39;                    // exponents,
+    static constexpr float kMostSmall = 0x1p-40f, kMostPlain = 0x1p88f;   // of scales up to this, and past that
     typedef typename ridge::Memory<T, 8>::Vec Vec;
 
     const AttendArgs& a;
@@ -650,7 +650,8 @@ __global__ __launch_bounds__(kBlock, wavesOf<T>(COLS)) void attendKernel(AttendA
             t = next;
         }
         // The waves' sums, from the largest `from` on, are added in their order.
-        // (With the exponent in both, the sum of p is relative to what the sums are.)
+        // With the exponent in both, the sum of p is relative to what the sums are. (Where one wave has scales up
+        // to 2^-40 alone and another one scales past 2^88, a p below 2^-47 of the largest may so count nothing.)
         p.total = sum4(p.total) * power2(-p.exponent);
         p.from += (float)p.exponent;
         if (p.group == 0) froms[wave][p.at] = p.from, totals[wave][p.at] = p.total;

@@ -1,11 +1,12 @@
 """attend where values, scales and scores lie far apart, against 64 bits.
 
-Tolerances. u = 2^-24 is half a unit of f32. A score is a sum of D exact products (of 3 D for a query of f32,
-whose columns are three parts of bf16), at most as many roundings and 6 of the sum of their magnitudes; as the exponent of p it carries that as a relative error, with 4 u of
-its own size and of the maximum's. p carries 4 u more, its product with a value's scale u, and sums of three
-parts of n terms 3 n u. out's numerator and denominator each carry that, relative to the sum of
-|p v|; a p below 2^-126 of the largest (2^-78 beside scales past 2^80) may count nothing, which is within
-that many times the sum of |v|.
+Tolerances. u = 2^-24 is half a unit of f32. A score is a sum of D exact products (of 3 D for a query of
+f32, whose columns are three parts of bf16), at most as many roundings and 6 of the sum of their
+magnitudes; as the exponent of p it carries that as a relative error, with 4 u of its own size and of
+the maximum's. p carries 4 u more, its product with a value's scale u, and sums of three parts of n
+terms 3 n u. out's numerator and denominator each carry that, relative to the sum of |p v|; a p below
+2^-126 of the largest may count nothing, which is within that many times the sum of |v|. (2^-47 where scales
+up to 2^-40 alone and past 2^88 meet: no test here has such a p.)
 """
 import math
 
@@ -28,8 +29,9 @@ def _gpu():
     torch.cuda.synchronize()
 
 
-def _check(b, scale=None, lost=2.0 ** -126):
-    """attend of a Batch against 64 bits: lost, the p that may count nothing."""
+def _check(b, scale=None):
+    """attend of a Batch against 64 bits."""
+    lost = 2.0 ** -126
     B, H, D = b.q.shape
     lse = torch.empty((B, H), device=DEV)
     got = A.attend(b.q, b.cache, b.pages, b.lengths, scale=scale, lse_out=lse)
@@ -72,7 +74,7 @@ def test_a_far_larger_value_of_no_weight_hides_nothing(power, dtype):
             b.cache[0][at[0], :, at[1], 0] = -127
             b.cache[1][at[0], :, at[1]] = 1.0           # scores of 16 * 127 / 16 and less below the others
             b.cache[3][at[0], :, at[1]] = 0.02 * 2.0 ** power
-        _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78)
+        _check(b)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -89,15 +91,15 @@ def test_rows_of_zeros_keep_their_weight_beside_large_values(power, dtype):
             b.cache[3][at[0], :, at[1]] = 2.0 ** -126
             at = _tokens(b, i, lambda t: t >= first)
             b.cache[3][at[0], :, at[1]] = 2.0 ** power
-        _check(b, lost=2.0 ** -126 if power < 80 else 2.0 ** -78)
+        _check(b)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("power", [-105, -60, -39, -33, 86, 119])
+@pytest.mark.parametrize("power", [-105, -60, -39, -33, 92, 119])
 def test_values_that_are_all_tiny_or_huge(power, dtype):
     b = Batch([700, 1, 40, 5000], 8, 2, 128, 16, dtype)
     b.cache[3].mul_(2.0 ** power)
-    _check(b, lost=2.0 ** -126 if power < 85 else 2.0 ** -78)
+    _check(b)
 
 
 @pytest.mark.parametrize("dtype,power", [(torch.float16, 10), (torch.float16, 20)] +
