@@ -102,8 +102,13 @@ int64_t ridge_attention_workspace(int64_t batch, int32_t heads, int32_t kvHeads,
  * cache->heads) serves query head h. lse (or null) [b * heads + h] <- log of the sum over t of
  * exp(scale * (q . k_t)). A sequence of no tokens gives zeros, and -inf in lse. A length that is
  * negative or past pagesEach pages, and a page that is none of the cache's where it is read,
- * give NaN. scale is FLT_MAX / 2 at the most, 2^118 for RIDGE_F16. q and out are of `type`; sums are f32. All sequences' tokens are shared evenly by the
- * workgroups that run at a time, so a result's last bits go by the other sequences' lengths; where
+ * give NaN. scale is FLT_MAX / 2 at the most, 2^118 for RIDGE_F16 (of which small columns lose
+ * bits beside scales below 2^-135). q and out are of `type`; nothing but out is rounded to fewer
+ * bits than f32's, whatever the sizes of queries and values (a p below 2^-126 of the largest may
+ * count nothing, and below 2^-47 where values' scales up to 2^-40 and past 2^88 meet).
+ *
+ * All sequences' tokens are shared evenly by the workgroups that run at a time, so a result's
+ * last bits go by the other sequences' lengths; where
  * pagesEach pages are 512 tokens or fewer, each sequence's key heads have a workgroup each, and its
  * result depends on nothing but its own operands. workspace is ridge_attention_workspace bytes, at
  * a multiple of 16, and needs no values; calls that may run at the same time take one each. */

@@ -12,15 +12,15 @@ projections.
     attend(q, cache, pages, lengths) -> the attention of each sequence's newest token
 
 Heads are [tokens, heads, columns] of float16, bfloat16 or float32, of any stride and offset
-whose columns are contiguous (views of a projection's rows among them), of up to 256
-columns. A cache is paged: k and v are int8 [pages, heads, page_size, columns] with a float32
+whose columns are contiguous and which do not overlap (views of a projection's rows among them),
+of up to 256 columns. A cache is paged: k and v are int8 [pages, heads, page_size, columns] with a float32
 scale for each row, page_size a multiple of 16, rows that start at multiples of 16 bytes. A
 slot is a token's place in it, page * page_size + offset. The rows are those of
 ridge_amd.int8: a row's largest magnitude over 127 is its scale, and its values over that are
 rounded to the nearest whole number.
 
-Sums, norms and softmax statistics are held in 32 bits. A call repeated with the same operands
-gives the same bits. Heads that norm_rope turns and rows of the cache do not depend on what is
+Sums, norms, softmax statistics and what they are made of are held in 32 bits. A call repeated
+with the same operands gives the same bits. Heads that norm_rope turns and rows of the cache do not depend on what is
 beside them; attend shares a batch's work evenly, so the last bits of a sequence's result go by
 the other sequences' lengths (not by what they hold), unless `pages` has room for 512 tokens
 each or fewer. positions, slots, pages and lengths are int32 on the device, so what they say

@@ -9,14 +9,15 @@
 // Both products are matrix instructions (16 x 16 x 32) with sums in f32, and no operand of them is rounded:
 // 8-bit whole numbers are exact in bf16 and f16. A query of f16 or bf16 is of its own type, one of f32 three
 // parts of bf16, and so is p vScale, which has 24 bits and any size. In one or two parts of f16 (64 x 16384
-// tokens 270 us for 279, in f32 286 for 311) a query's columns 2^-32 of its largest lost their bits,
+// tokens 269 us for 275, in f32 286 for 305) a query's columns 2^-32 of its largest lost their bits,
 // and values beside a far larger one, whatever its p.
 //
-// No operand goes through LDS or moves between lanes. The scores are computed transposed, keys as
-// rows and heads as columns, so that a lane ends with 4 tokens of each 16 for one head; those are
-// the k's that the second product, values as rows (transposed too) and heads as columns, wants
-// from that lane, if the tokens of k = 8 g + 4 a + r are 16 a + 4 g + r. So a lane loads the values of
-// those tokens and no others, and the running maximum's factor is its own head's everywhere.
+// No value and no probability goes through LDS or moves between lanes (keys of more than 64 columns do, so
+// that a load covers whole cache lines). The scores are computed transposed, keys as rows and heads as
+// columns, so that a lane ends with 4 tokens of each 16 for one head; those are the k's that the
+// second product, values as rows (transposed too) and heads as columns, wants from that lane, if the tokens
+// of k = 8 g + 4 a + r are 16 a + 4 g + r. So a lane loads the values of those tokens and no others, and the
+// running maximum's factor is its own head's everywhere.
 //
 // Work is shared evenly: the rounds (128 tokens) of all sequences' key heads, one behind the other, are
 // cut into one equal share for each workgroup that runs at a time, whatever the sequences' lengths.
@@ -27,7 +28,6 @@
 namespace {
 
 using ridge::kBlock;
-using ridge::kMostBlocks;
 using ridge::kWave;
 using ridge::kWavesPerBlock;
 using ridge::uniformLoad;
@@ -156,7 +156,8 @@ struct Tile {
     Float4 kScale[2], vScale[2];
 };
 
-// Loads past the caches (bit 1): a key or value is read once, and its cache line whole by one load.
+// Loads past the caches (bit 1): a key or value is read once by a workgroup, and its cache line whole by one
+// load. (More than 16 query heads of a key head are several workgroups' work, each of which reads it.)
 constexpr int kStream = 2;
 
 // Memory from `at` on, for offsets of 32 bits: no lane computes an address.
@@ -764,10 +765,11 @@ int residentOf(int dim, size_t bytes) {
 
 // Whether each key head (and tile) has a workgroup, which needs no second launch, instead of an even
 // share of all rounds. us of sequences of one length, each their own | shared, 8 key heads of 128:
-//   1 x 512 9.5 | 9.9, 1 x 768 14 | 10, 16 x 1024 19 | 15, 32 x 1024 21 | 26, 64 x 1024 27 | 37,
-//   32 x 2048 36 | 37, 64 x 2048 48 | 58, 128 x 4096 182 | 192;
-// of lengths from a quarter on: 32 x 1024 20 | 21, 64 x 2048 39 | 45, 128 x 4096 136 | 129. What one long
-// sequence among short ones costs alone (2.2 us for each 128 tokens) bounds the lengths.
+//   1 x 512 10.1 | 9.7, 1 x 768 13 | 10, 16 x 1024 20 | 15, 32 x 1024 22 | 25, 64 x 1024 28 | 37,
+//   32 x 2048 38 | 37, 64 x 2048 50 | 58, 128 x 4096 185 | 193;
+// of lengths from a quarter on: 32 x 1024 21 | 21, 64 x 2048 40 | 46, 128 x 4096 140 | 130. What one long
+// sequence among short ones costs alone (2.2 us for each 128 tokens) bounds the lengths. Up to 512 tokens a
+// result depends on no other sequence.
 bool eachItsOwn(int64_t batch, int64_t heads, int64_t capacity) {
     return capacity <= 512 || (capacity <= 1024 && batch * heads >= 256) || (capacity <= 2048 && batch * heads >= 512);
 }
